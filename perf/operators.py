@@ -110,7 +110,8 @@ def _quantise(x):
     x = x.float()
     zero = x.amin(-1).to(torch.bfloat16)
     span = x.amax(-1) - zero.float()
-    step = torch.where(span > 0, span / 15.0, torch.zeros_like(span)).to(torch.bfloat16)
+    # a tensor of fifteens: by a plain number torch multiplies with its reciprocal
+    step = torch.where(span > 0, span / torch.full_like(span, 15.0), torch.zeros_like(span)).to(torch.bfloat16)
     ok = torch.isfinite(x).all(-1) & torch.isfinite(step.float()) & torch.isfinite(zero.float())
     live = ok & (step.float() > 0)
     # 64 bits: whether a value lies above or below the middle of two codes
@@ -397,7 +398,8 @@ def _exact_append(s):
         # the zero and the step are what is kept: 16-bit values, chosen in 32 bits
         zero = x.min(-1, keepdim=True).values.bfloat16().double()
         reach = (x.max(-1, keepdim=True).values - zero).float()
-        step = (reach.clamp(min=0) / 15).bfloat16().double()
+        fifteen = torch.full_like(reach, 15, dtype=torch.float64)
+        step = (reach.clamp(min=0).double() / fifteen).float().bfloat16().double()
         code = torch.clamp(torch.round((x - zero) / torch.where(step > 0, step, 1.0)), 0, 15) * (step > 0)
         back = zero + code * step
         back[s["slots"] < 0] = 0
