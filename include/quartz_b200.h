@@ -441,6 +441,94 @@ int qz_fused_mlp_decode_peer(const int8_t* gu_q, const float* gu_s, int64_t ng, 
 int qz_rmsnorm_peer_sum(const qz_peer_sum* ps, int64_t n, const float* w, float eps, float* h,
                         float* xn, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Paged 4-bit KV cache: sequences of uneven length that share one pool of
+ * pages. quartz has no counterpart (one growing fp32 cache per model,
+ * quartz/cache.py:26-46).
+ *
+ * Pool of one layer: uint8 [pages, n_kv, page_size * (hd + 8)], 16-byte
+ * aligned. A block (one page of one kv head) holds the K codes [page_size,
+ * hd / 2], the V codes, then K's and V's bf16 pairs (s, z) [page_size, 2].
+ * Byte j of a code row has element 2j in its low half and 2j + 1 in its high
+ * half; a row stands for z + c * s. page_size is 16, 32, 64, 128 or 256; hd 64
+ * or 128. Position p of a request lies in page block_table[b, p / page_size];
+ * a slot is page * page_size + offset.
+ * ------------------------------------------------------------------------ */
+
+/* dtype of k, v, q and out in the calls below. */
+#define QZ_F32 0
+#define QZ_BF16 1
+#define QZ_F16 2
+
+/*
+ * Block tables and slot maps from request lengths. Request b < B (1 .. 4096)
+ * holds lens[b] positions; new_rows[b] rows join it in this step. Requests
+ * are served in order; request b is granted when
+ *   - the rows up to and including its own fit `rows`,
+ *   - its pages ceil((lens + new_rows) / page_size) fit the table's `width`,
+ *   - it needs no new page, or *used plus the new pages of the requests up to
+ *     and including it (those that pass the first two) is at most n_free.
+ * A granted request gets the next new pages of free_pages (int32 [n_free], of
+ * which the first *used are taken) into block_table [B, width] (in place, new
+ * entries only) and lens_out[b] = lens[b] + new_rows[b]. A refused one (also
+ * one with a negative length or row count, which counts as no rows) keeps its
+ * length and pages and its rows get slot -1. Outputs: cu_rows [B + 1] (rows of
+ * request b are cu_rows[b] .. cu_rows[b + 1] - 1, cut at `rows`), used_out[0],
+ * and per row slots[r] and positions[r] (both -1 for rows behind the last
+ * request's). lens_out may be lens and used_out may be used; no other output
+ * may overlap an input. Deterministic.
+ */
+int qz_kv4_plan(const int64_t* lens, const int64_t* new_rows, int64_t B, int32_t* block_table,
+                int64_t width, const int32_t* free_pages, int64_t n_free, const int64_t* used,
+                int64_t page_size, int64_t rows, int64_t* cu_rows, int64_t* lens_out,
+                int64_t* used_out, int64_t* slots, int64_t* positions, void* stream);
+
+/*
+ * Quantise row r of k and v ([n, nkv, hd], strides in elements, hd contiguous)
+ * and store it at slots[r]; a slot outside [0, pages * page_size) stores
+ * nothing. Per row of hd values x, in fp32:
+ *   z = bf16(min x);  s = bf16((max x - z) / 15), 0 when max x <= z;
+ *   c = clamp(round_half_even((x - z) / s), 0, 15), decided on the real quotient.
+ * A row with a non-finite value (or whose z or s is not finite in bf16) reads
+ * back as NaN. A slot must not appear twice in one call.
+ */
+int qz_kv4_append(const void* k, const void* v, int dtype, int64_t k_row_stride,
+                  int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t n,
+                  int nkv, int hd, uint8_t* pool, int64_t pages, int64_t page_size,
+                  const int64_t* slots, void* stream);
+
+/* k, v [n, nkv, hd] fp32 (16-byte aligned): the values z + c * s at slots[r];
+ * zeros for a slot outside the pool. */
+int qz_kv4_gather(const uint8_t* pool, int64_t pages, int64_t page_size, int nkv, int hd,
+                  const int64_t* slots, int64_t n, float* k, float* v, void* stream);
+
+/* Workspace bytes of qz_kv4_attention on the current device (256-byte aligned,
+ * zeroed once before its first use and left ready for the next call; calls
+ * sharing it must not overlap on the GPU). */
+int qz_kv4_attention_workspace_bytes(int nq, int nkv, int hd, int64_t max_rows, int64_t* bytes);
+
+/*
+ * Attention of query rows over the paged cache. Rows cu_rows[b] .. cu_rows[b +
+ * 1] - 1 of q [n, nq, hd] are request b's last rows: with n_b of them and
+ * lens[b] positions (this step's included), its row i sees positions
+ * [0, lens[b] - n_b + i + 1), so 0 .. its own; a row that sees nothing gives
+ * zeros. cu_rows NULL: row b is request b's one row. max_rows bounds n_b;
+ * requests with more rows are not handled (their rows of out stay as they
+ * were), like rows of no request. out[r, h] = softmax(scale * q K^T) V over kv
+ * head h / (nq / nkv), fp32 sums, one rounding to dtype; strides are in
+ * elements, hd contiguous. out must not overlap q unless they are the same
+ * with the same strides. Positions beyond the table (lens[b] > width *
+ * page_size) are not seen; table entries outside [0, pages) are not read and
+ * their positions count as unseen. B <= 4096, width * page_size <= 2^30.
+ * The result does not depend on timing.
+ */
+int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_head_stride,
+                     void* out, int64_t out_row_stride, int64_t out_head_stride,
+                     const uint8_t* pool, int64_t pages, int64_t page_size,
+                     const int32_t* block_table, int64_t width, const int64_t* lens,
+                     const int64_t* cu_rows, int64_t B, int64_t n, int64_t max_rows, int nq,
+                     int nkv, int hd, float scale, void* ws, size_t ws_bytes, void* stream);
+
 /* Read the device status word of the current device into words[0..3]
  * ({error bits, first error site, block of first error, error count}); when
  * clear != 0 reset it to zero afterwards. Synchronises the device. */

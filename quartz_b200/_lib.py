@@ -20,6 +20,8 @@ QZ_ERR_UNSUPPORTED = 3
 # Every symbol include/quartz_b200.h declares, with its ctypes signature.
 # activation prologues of qz_gemm_w8_act_ws (include/quartz_b200.h)
 QZ_ACT_NONE, QZ_ACT_RMSNORM, QZ_ACT_SILU_MUL = 0, 1, 2
+# dtypes of the paged cache's rows (include/quartz_b200.h)
+QZ_F32, QZ_BF16, QZ_F16 = 0, 1, 2
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -81,6 +83,15 @@ SIGNATURES = {
     "qz_decode_layers": ([_vp, _int, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _int, _int, _int,
                           _int, _int, _i64, ctypes.c_float, ctypes.c_float, _vp, ctypes.c_size_t,
                           _vp, _vp], _int),
+    "qz_kv4_plan": ([_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp,
+                     _vp, _vp], _int),
+    "qz_kv4_append": ([_vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp, _i64, _i64,
+                       _vp, _vp], _int),
+    "qz_kv4_gather": ([_vp, _i64, _i64, _int, _int, _vp, _i64, _vp, _vp, _vp], _int),
+    "qz_kv4_attention_workspace_bytes": ([_int, _int, _int, _i64, ctypes.POINTER(_i64)], _int),
+    "qz_kv4_attention": ([_vp, _int, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp,
+                          _vp, _i64, _i64, _i64, _int, _int, _int, ctypes.c_float, _vp,
+                          ctypes.c_size_t, _vp], _int),
     "qz_device_status": ([ctypes.POINTER(ctypes.c_uint32), _int], _int),
     "qz_sync": ([_vp], _int),
 }

@@ -1611,3 +1611,5 @@ int qz_sync(void* stream) {
 }
 
 }  // extern "C"
+
+#include "qz_kv4_api.cuh"

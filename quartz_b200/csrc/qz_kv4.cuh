@@ -1,0 +1,947 @@
+// qz_kv4.cuh -- the paged 4-bit KV cache: block tables and slot maps built from
+// request lengths, 4-bit append and read back, and decode attention over the
+// packed pages.
+//
+// Pool layout (one layer): uint8 [pages, n_kv, ps * (hd + 8)]. One block is a
+// page (ps positions) of one kv head:
+//   K codes [ps, hd / 2] | V codes [ps, hd / 2] | K (s, z) [ps, 2] | V (s, z) [ps, 2]
+// Codes are unsigned 4-bit, two per byte, element 2j in the low half of byte
+// j; s (step) and z (zero) are bf16. A row stands for z + c * s.
+//
+// z and s are bf16 because they are read with every row: 4 bytes beside hd/2
+// of codes instead of 8 (11 % of the traffic at hd = 64). Rounding them costs
+// nothing in the codes, which are chosen against the rounded z and s; only the
+// smallest values of a row can fall below z, by at most |z| * 2^-9.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "qz_device.cuh"
+
+namespace qz {
+namespace kv4 {
+
+enum : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// n consecutive elements as fp32; `vec`: p is 16-byte aligned and n * sizeof(T)
+// a multiple of 16.
+template <int n, class T>
+__device__ __forceinline__ void load_row(const T* p, bool vec, float (&x)[n]) {
+  if (vec) {
+    constexpr int per = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < n / per; ++j) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + j);
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int k = 0; k < per; ++k) x[j * per + k] = to_f(e[k]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < n; ++j) x[j] = to_f(p[j]);
+  }
+}
+
+// (s, z) of a packed parameter word: s in the low half, z in the high half.
+__device__ __forceinline__ float par_s(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float par_z(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// ---------------------------------------------------------------------------
+// block tables and slot maps
+// ---------------------------------------------------------------------------
+// Requests in order: request b holds lens[b] positions and new_rows[b] rows
+// join. It is granted when its rows fit the row capacity, its pages the
+// table's width, and the free pages left by the requests before it suffice;
+// a refused request keeps its length and its rows get slot -1. Page j of a
+// request's new ones is free[used + (pages of the requests before it) + j].
+//
+// Latency-bound (a few hundred bytes to about a megabyte): one launch, no
+// atomics. Every CTA scans all requests in shared memory, then CTAs share out
+// rows (binary search of the row's request) and requests (table entries). Up
+// to kPlanCluster CTAs form one cluster whose barrier separates the reading
+// of lens / used from the writing of their successors, so both may be updated
+// in place.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanPer = 4;
+constexpr int kPlanMaxB = kPlanThreads * kPlanPer;
+constexpr int kPlanCluster = 8;
+
+struct PlanArgs {
+  const int64_t* lens;
+  const int64_t* joins;
+  int32_t* table;
+  const int32_t* free_pages;
+  const int64_t* used;
+  int64_t* cu_rows;
+  int64_t* lens_out;
+  int64_t* used_out;
+  int64_t* slots;
+  int64_t* positions;
+  int64_t width, n_free, rows;
+  int B, shift;   // page size = 1 << shift
+};
+
+__host__ __device__ constexpr int plan_smem(int B) { return 512 + B * 16 + 16; }
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// Exclusive prefix of v over the block; total: the sum.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  *total = warp_sums[31];
+  return x - v + (warp ? warp_sums[warp - 1] : 0);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+  extern __shared__ __align__(16) uint8_t plan_sh[];
+  int64_t* warp_sums = reinterpret_cast<int64_t*>(plan_sh);             // [32] (+ 32 spare)
+  int64_t* s_len = reinterpret_cast<int64_t*>(plan_sh + 512);           // [B]
+  int32_t* s_page = reinterpret_cast<int32_t*>(s_len + a.B);            // [B] free index, -1: refused
+  int32_t* s_cu = s_page + a.B;                                         // [B + 1]
+  const int tid = threadIdx.x, B = a.B, shift = a.shift;
+  const int64_t ps = int64_t(1) << shift, cap = a.width << shift;
+
+  pdl_wait();
+  int64_t len[kPlanPer], n[kPlanPer], need[kPlanPer];
+  bool ok[kPlanPer];
+  int64_t mine = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanPer; ++k) {
+    const int b = tid * kPlanPer + k;
+    len[k] = b < B ? a.lens[b] : 0;
+    n[k] = b < B ? a.joins[b] : 0;
+    ok[k] = len[k] >= 0 && n[k] >= 0 && len[k] <= cap;
+    n[k] = n[k] < 0 ? 0 : (n[k] > a.rows ? a.rows + 1 : n[k]);
+    mine += n[k];
+  }
+  const int64_t used = *a.used;
+  const int64_t left = used < 0 || used > a.n_free ? 0 : a.n_free - used;
+  int64_t total;
+  int64_t row = block_scan(mine, warp_sums, &total);
+  if (tid == 0) s_cu[0] = 0;
+  mine = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanPer; ++k) {
+    const int b = tid * kPlanPer + k;
+    row += n[k];
+    if (b < B) {
+      s_len[b] = len[k];
+      s_cu[b + 1] = static_cast<int32_t>(row < a.rows ? row : a.rows);
+    }
+    need[k] = 0;
+    if (ok[k]) {
+      const int64_t want = (len[k] + n[k] + ps - 1) >> shift;
+      ok[k] = row <= a.rows && want <= a.width;
+      if (ok[k]) need[k] = want - ((len[k] + ps - 1) >> shift);
+    }
+    mine += need[k];
+  }
+  int64_t at = block_scan(mine, warp_sums, &total);
+  int64_t granted = 0;   // pages handed out to this thread's requests
+#pragma unroll
+  for (int k = 0; k < kPlanPer; ++k) {
+    const int b = tid * kPlanPer + k;
+    const bool g = ok[k] && (need[k] == 0 || at + need[k] <= left);
+    if (b < B) s_page[b] = g ? static_cast<int32_t>(need[k] ? used + at : 0) : -1;
+    granted += g ? need[k] : 0;
+    at += need[k];
+  }
+  block_scan(granted, warp_sums, &total);   // also orders the shared arrays before their use
+  cluster_sync_all();
+
+  const int nthreads = gridDim.x * kPlanThreads, gt = blockIdx.x * kPlanThreads + tid;
+  for (int b = gt; b < B; b += nthreads) {
+    a.cu_rows[b + 1] = s_cu[b + 1];
+    const int64_t l = s_len[b];
+    const int64_t j = a.joins[b];
+    a.lens_out[b] = s_page[b] >= 0 ? l + j : l;
+  }
+  if (gt == 0) {
+    a.cu_rows[0] = 0;
+    *a.used_out = used + total;
+  }
+  const int live = s_cu[B];
+  for (int64_t r = gt; r < a.rows; r += nthreads) {
+    int64_t slot = -1, pos = -1;
+    if (r < live) {
+      int lo = 0, hi = B - 1;   // the first request whose rows end after r
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_cu[mid + 1] > r) hi = mid; else lo = mid + 1;
+      }
+      const int64_t l = s_len[lo];
+      pos = l + r - s_cu[lo];
+      const int32_t first = s_page[lo];
+      if (first >= 0) {
+        const int64_t have = (l + ps - 1) >> shift, p = pos >> shift;
+        const int64_t page = p < have ? a.table[static_cast<int64_t>(lo) * a.width + p]
+                                      : a.free_pages[first + (p - have)];
+        if (page >= 0) slot = (page << shift) + (pos & (ps - 1));
+      }
+    }
+    a.slots[r] = slot;
+    a.positions[r] = pos;
+  }
+  // new table entries (the entries read above are the ones before them)
+  const int lane = tid & 31;
+  for (int b = gt >> 5; b < B; b += nthreads >> 5) {
+    const int32_t first = s_page[b];
+    if (first < 0) continue;
+    const int64_t l = s_len[b], have = (l + ps - 1) >> shift;
+    const int64_t want = (l + (s_cu[b + 1] - s_cu[b]) + ps - 1) >> shift;
+    for (int64_t j = have + lane; j < want; j += 32)
+      a.table[static_cast<int64_t>(b) * a.width + j] = a.free_pages[first + (j - have)];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// append: rows of K and V -> 4-bit codes at their slots
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// The parameter word and the fp32 values of s and z for a row's extremes. A row
+// with a non-finite value, or whose z or s leaves bf16's range, gets NaN for
+// both (it reads back as NaN); a row whose maximum does not exceed z gets s = 0.
+__device__ __forceinline__ uint32_t row_params(float mn, float mx, float& s, float& z) {
+  const uint32_t zb = __bfloat16_as_ushort(__float2bfloat16_rn(mn));
+  z = __uint_as_float(zb << 16);
+  const float span = __fsub_rn(mx, z);
+  const float st = span > 0.f ? __fdiv_rn(span, 15.0f) : 0.0f;
+  const uint32_t sb = __bfloat16_as_ushort(__float2bfloat16_rn(st));
+  s = __uint_as_float(sb << 16);
+  if (!(isfinite(mn) && isfinite(mx) && isfinite(s) && isfinite(z))) {
+    s = 0.f;
+    return 0x7FC07FC0u;
+  }
+  return sb | (zb << 16);
+}
+
+// Codes of 16 values: clamp(round((x - z) / s), 0, 15) of the real quotient,
+// ties to even. t = (x - z) * (1 / s) in fp32 is within 3 * 2^-24 * |t| < 1e-5
+// of it, so only a t that close to the middle of two codes (1e-4 is taken) is
+// decided again in fp64, where x - z and the comparison lose nothing that
+// matters. Adding 1.5 * 2^23 rounds t to an integer in the low mantissa bits.
+__device__ __forceinline__ uint2 codes16(const float (&x)[16], float s, float z) {
+  if (!(s > 0.f)) return make_uint2(0u, 0u);
+  const bool tiny = s < 1e-30f;   // 1 / s would overflow
+  const float inv = tiny ? 0.f : 1.0f / s;
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    float t = __fsub_rn(x[j], z) * inv;
+    t = fminf(fmaxf(t, 0.f), 15.f);
+    const float r = __fadd_rn(t, 12582912.0f);
+    uint32_t c = __float_as_uint(r) & 15u;
+    if (tiny || fabsf(t - __fsub_rn(r, 12582912.0f)) > 0.4999f) {
+      const double d = rint((static_cast<double>(x[j]) - static_cast<double>(z)) / static_cast<double>(s));
+      c = d >= 15.0 ? 15u : (d > 0.0 ? static_cast<uint32_t>(d) : 0u);
+    }
+    w[j >> 3] |= c << (4 * (j & 7));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+struct AppendArgs {
+  const void* k;
+  const void* v;
+  int64_t k_rs, k_hs, v_rs, v_hs;   // element strides of rows and heads
+  uint8_t* pool;
+  const int64_t* slots;
+  int64_t n, slots_max;             // slots_max = pages * page size
+  int nkv, shift;
+  int vec;                          // 16-byte loads are aligned
+};
+
+constexpr int kAppendThreads = 256;
+
+// Bound by HBM (the rows are read once, hd/2 + 4 bytes written). HD / 16 lanes
+// take one row, 16 values each: three (two) shuffle rounds find its extremes,
+// and each lane stores its 16 codes as 8 bytes. One value per lane and row
+// would spend as many instructions on shuffles as on the quotients.
+template <class T, int HD>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+  constexpr int LPR = HD / 16;
+  const int lane = threadIdx.x & (LPR - 1);
+  const int64_t total = a.n * a.nkv * 2;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kAppendThreads / LPR);
+  pdl_wait();
+  // warp-uniform loop: all lanes run the same number of rounds for the shuffles
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / LPR);
+  for (int64_t base = first; base < total; base += step) {
+    const int64_t id = base + threadIdx.x / LPR;
+    const int64_t nk = id / a.nkv;
+    const int h = static_cast<int>(id - nk * a.nkv);
+    const int64_t row = nk >> 1;
+    const bool is_v = nk & 1;
+    const int64_t slot = id < total ? __ldg(a.slots + row) : -1;
+    const bool live = slot >= 0 && slot < a.slots_max;
+    float x[16];
+    if (live) {
+      const T* p = static_cast<const T*>(is_v ? a.v : a.k) +
+                   row * (is_v ? a.v_rs : a.k_rs) + h * (is_v ? a.v_hs : a.k_hs) + lane * 16;
+      load_row(p, a.vec, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = 0.f;
+    }
+    float mn = x[0], mx = x[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) {
+      mn = min_nan(mn, x[j]);
+      mx = max_nan(mx, x[j]);
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) {
+      mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (!live) continue;
+    float s, z;
+    const uint32_t par = row_params(mn, mx, s, z);
+    const uint2 c = codes16(x, s, z);
+    const int64_t ps = int64_t(1) << a.shift, off = slot & (ps - 1);
+    uint8_t* blk = a.pool + ((slot >> a.shift) * a.nkv + h) * (ps * (HD + 8));
+    *reinterpret_cast<uint2*>(blk + (is_v ? ps * (HD / 2) : 0) + off * (HD / 2) + lane * 8) = c;
+    if (lane == 0)
+      *reinterpret_cast<uint32_t*>(blk + ps * HD + (is_v ? ps * 4 : 0) + off * 4) = par;
+  }
+}
+
+struct GatherArgs {
+  const uint8_t* pool;
+  const int64_t* slots;
+  float* k;
+  float* v;
+  int64_t n, slots_max;
+  int nkv, shift;
+};
+
+constexpr int kGatherThreads = 256;
+
+// The values of rows: z + c * s (one rounding), fp32 [n, nkv, hd]; zeros for a
+// slot outside the pool. Bound by the fp32 stores: HD / 4 lanes take a row,
+// each reads 2 bytes of codes and stores one float4.
+template <int HD>
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const GatherArgs a) {
+  constexpr int LPR = HD / 4;
+  const int lane = threadIdx.x & (LPR - 1);
+  const int64_t total = a.n * a.nkv * 2;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kGatherThreads / LPR);
+  pdl_wait();
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * (kGatherThreads / LPR) + threadIdx.x / LPR;
+       id < total; id += step) {
+    const int64_t nk = id / a.nkv;
+    const int h = static_cast<int>(id - nk * a.nkv);
+    const int64_t row = nk >> 1;
+    const bool is_v = nk & 1;
+    const int64_t slot = __ldg(a.slots + row);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (slot >= 0 && slot < a.slots_max) {
+      const int64_t ps = int64_t(1) << a.shift, off = slot & (ps - 1);
+      const uint8_t* blk = a.pool + ((slot >> a.shift) * a.nkv + h) * (ps * (HD + 8));
+      const uint32_t c = *reinterpret_cast<const uint16_t*>(
+          blk + (is_v ? ps * (HD / 2) : 0) + off * (HD / 2) + lane * 2);
+      const uint32_t par = *reinterpret_cast<const uint32_t*>(
+          blk + ps * HD + (is_v ? ps * 4 : 0) + off * 4);
+      const float s = par_s(par), z = par_z(par);
+      o.x = fmaf(static_cast<float>(c & 15u), s, z);
+      o.y = fmaf(static_cast<float>((c >> 4) & 15u), s, z);
+      o.z = fmaf(static_cast<float>((c >> 8) & 15u), s, z);
+      o.w = fmaf(static_cast<float>(c >> 12), s, z);
+    }
+    reinterpret_cast<float4*>((is_v ? a.v : a.k) + (row * a.nkv + h) * HD)[lane] = o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// attention, rows against a long context
+// ---------------------------------------------------------------------------
+// o = sum_t softmax(scale * q . k_t) v_t with k_t = zk_t + sk_t c_t and
+// v_t = zv_t + sv_t d_t, so with the integer codes as one MMA operand
+//   q . k_t = sk_t (q . c_t) + zk_t sum(q)
+//   o       = sum_t (p_t sv_t) (d_t - 8) + sum_t p_t (zv_t + 8 sv_t)
+// The codes are exact in fp16, so only q and the weights p sv are rounded:
+// each is split into two fp16 values (22 bits), which stand as two columns of
+// the other operand. A warp handles 16 positions at a time with m16n8k16 MMAs:
+//   S [16 positions x 8 columns]  = K codes x q    (4 queries x {hi, lo})
+//   O [hd x 8 columns]           += (V codes - 8)^T x w
+// These MMAs see 8 columns per kv head and position block; the pages stream at
+// HBM speed and the tensor pipe is not the bound, so mma.sync serves here (a
+// tcgen05 tile of 128 rows would be 94 % padding).
+//
+// Fragments come straight from the packed pages: a lane's share of a K row is
+// 16 (hd 64: 8) consecutive bytes. The order of dimensions inside an MMA's K
+// axis is free as long as q has the same one, so nibbles 0 and 4 of a word
+// (w & 0x000F000F) form one fp16 pair: the bits c are the subnormal c * 2^-24,
+// exact. Nibbles 1 and 5 lie four bits higher, as 16 c * 2^-24; q's values for
+// them are divided by 16. For V, pairs run along positions: one PRMT joins the
+// halves of two positions' words; 0x6400 | d is 1024 + d, and one HADD2 (HFMA2
+// for the nibbles four bits higher) leaves d - 8. Centring V keeps the running
+// sum as small as its result; the MMA's accumulation truncates.
+//
+// Work is cut into steps of 64 positions over all (request, kv head, block of
+// queries), shared out evenly over a fixed grid whatever the lengths, which
+// only the device knows (graph replay). A CTA's share may begin or end within an item; those partials
+// (max, sum, accumulator) go to the workspace and the last of an item's CTAs
+// to arrive merges them in CTA order, so results do not depend on timing.
+//
+// The running maximum is only renewed when a score passes it by 2^4 (weights
+// stay below 2^4 relative to it): one vote per tile instead of a reduction.
+
+constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kAttnTile = 16;
+constexpr int kAttnStep = kAttnWarps * kAttnTile;
+constexpr int kAttnMaxB = 4096;
+
+struct AttnArgs {
+  const void* q;
+  void* out;
+  int64_t q_rs, q_hs, o_rs, o_hs;   // element strides of rows and heads
+  const uint8_t* pool;
+  const int32_t* table;
+  const int64_t* lens;
+  const int64_t* cu;                // [B + 1] or null: request b has row b
+  float* part;
+  unsigned int* tickets;
+  int64_t pages, width, n;
+  int B, nkv, group, shift;
+  float scale;                      // softmax scale * log2(e)
+  int vec;                          // q rows are 16-byte aligned
+  int rows_lo, rows_hi;             // requests with rows_lo < rows <= rows_hi are handled
+};
+
+// CTAs per SM that the register file holds without spills.
+__host__ __device__ constexpr int attn_per_sm(int hd, int nb) {
+  return nb == 1 ? (hd == 64 ? 4 : 3) : (hd == 64 ? 3 : 2);
+}
+template <int HD, int NB>
+__host__ __device__ constexpr int attn_queries() { return 4 * NB; }
+template <int HD, int NB>
+__host__ __device__ constexpr int attn_part_floats() { return 4 * NB * (HD + 2); }
+template <int HD, int NB>
+__host__ __device__ constexpr int attn_smem() {
+  return kAttnThreads * 8 + 64 + kAttnWarps * attn_part_floats<HD, NB>() * 4;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_h2(__half lo, __half hi) {
+  return static_cast<uint32_t>(__half_as_ushort(lo)) |
+         (static_cast<uint32_t>(__half_as_ushort(hi)) << 16);
+}
+
+// x as fp16 hi (low half of the word) and the fp16 of what hi leaves (high half).
+__device__ __forceinline__ uint32_t split_h2(float x) {
+  const __half hi = __float2half_rn(x);
+  return pack_h2(hi, __float2half_rn(x - __half2float(hi)));
+}
+
+// 2^e for e in [-126, 127].
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// The four position pairs of one 16-bit half of two rows' words, less 8:
+// h[n] = (d(row a, nibble n) - 8, d(row b, nibble n) - 8) as fp16.
+__device__ __forceinline__ void centred4(uint32_t x, uint32_t (&h)[4]) {
+  const uint32_t y = x >> 8;
+  const __half2 m8 = __half2half2(__ushort_as_half(0xE408));    // -1032
+  const __half2 m72 = __half2half2(__ushort_as_half(0xD480));   // -72
+  const __half2 r16 = __half2half2(__ushort_as_half(0x2C00));   // 1 / 16
+  auto put = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
+  auto get = [](__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); };
+  h[0] = get(__hadd2(put((x & 0x000F000Fu) | 0x64006400u), m8));
+  h[1] = get(__hfma2(put((x & 0x00F000F0u) | 0x64006400u), r16, m72));
+  h[2] = get(__hadd2(put((y & 0x000F000Fu) | 0x64006400u), m8));
+  h[3] = get(__hfma2(put((y & 0x00F000F0u) | 0x64006400u), r16, m72));
+}
+
+template <int W>
+__device__ __forceinline__ void ld_stream(const uint8_t* p, uint32_t (&v)[W]) {
+  if constexpr (W == 4)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(p));
+  else if constexpr (W == 2)
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
+                 : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+  else
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+}
+
+// A lane's share of a 16-position tile.
+template <int HD>
+struct Tile {
+  uint32_t k[2][HD / 32];   // K codes of positions g, g + 8
+  uint32_t v[4][HD / 64];   // V codes of positions 2i, 2i + 1, 2i + 8, 2i + 9
+  uint32_t kp[2], vp[2];    // (s, z) of positions g, g + 8
+  bool ok;                  // the table entry is a page of the pool
+
+  __device__ __forceinline__ void load(const AttnArgs& a, int h, int page, int pos, int g, int i) {
+    ok = page >= 0 && page < a.pages;
+    if (!ok) return;
+    const int64_t ps = int64_t(1) << a.shift;
+    const int off = pos & static_cast<int>(ps - 1);
+    const uint8_t* blk = a.pool + (static_cast<int64_t>(page) * a.nkv + h) * (ps * (HD + 8));
+    const uint8_t* kc = blk + (off + g) * (HD / 2) + i * (HD / 8);
+    ld_stream(kc, k[0]);
+    ld_stream(kc + 8 * (HD / 2), k[1]);
+    const uint8_t* vc = blk + ps * (HD / 2) + (off + 2 * i) * (HD / 2) + g * (HD / 16);
+    ld_stream(vc, v[0]);
+    ld_stream(vc + HD / 2, v[1]);
+    ld_stream(vc + 8 * (HD / 2), v[2]);
+    ld_stream(vc + 9 * (HD / 2), v[3]);
+    const uint8_t* par = blk + ps * HD + (off + g) * 4;
+    uint32_t w[1];
+    ld_stream(par, w);
+    kp[0] = w[0];
+    ld_stream(par + 32, w);
+    kp[1] = w[0];
+    ld_stream(par + ps * 4, w);
+    vp[0] = w[0];
+    ld_stream(par + ps * 4 + 32, w);
+    vp[1] = w[0];
+  }
+};
+
+__device__ __forceinline__ int64_t rows_of(const AttnArgs& a, int64_t b, int64_t* first) {
+  int64_t r0 = b, r1 = b + 1;
+  if (a.cu) {
+    r0 = a.cu[b];
+    r1 = a.cu[b + 1];
+  }
+  r0 = r0 < 0 ? 0 : r0;
+  r1 = r1 > a.n ? a.n : r1;
+  *first = r0;
+  const int64_t n = r1 > r0 ? r1 - r0 : 0;
+  return n > a.rows_lo && n <= a.rows_hi ? n : 0;
+}
+
+template <int NB>
+__device__ __forceinline__ int64_t steps_of(const AttnArgs& a, int64_t len) {
+  const int64_t cap = a.width << a.shift;
+  const int64_t t = len < 0 ? 0 : (len > cap ? cap : len);
+  const int64_t s = (t + kAttnStep - 1) / kAttnStep;
+  return s > 0 ? s : 1;   // an empty context still has its (zero) rows to write
+}
+
+template <class T, int HD, int NB>
+__global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel(const AttnArgs a) {
+  constexpr int Q = attn_queries<HD, NB>();   // queries (row, head) of an item
+  constexpr int KS = HD / 16;                 // MMAs along the head dimension, and O tiles
+  constexpr int KW = HD / 32;                 // K words of a lane and row
+  constexpr int VW = HD / 64;                 // V words of a lane and position
+  constexpr float kNegInf = -INFINITY;
+  extern __shared__ __align__(16) uint8_t attn_sh[];
+  int64_t* s_scan = reinterpret_cast<int64_t*>(attn_sh);                        // [threads]
+  int64_t* s_at = reinterpret_cast<int64_t*>(attn_sh + kAttnThreads * 8);       // {b, its first unit}
+  int* s_last = reinterpret_cast<int*>(s_at + 2);
+  float* s_o = reinterpret_cast<float*>(attn_sh + kAttnThreads * 8 + 64);       // [warps][Q][HD]
+  float* s_ml = s_o + kAttnWarps * Q * HD;                                      // [warps][Q][2]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
+
+  pdl_wait();
+  // ---- this CTA's share [u0, u1) of all units --------------------------------
+  const int per_thread = (a.B + kAttnThreads - 1) / kAttnThreads;
+  auto units = [&](int64_t b) -> int64_t {
+    int64_t r0;
+    const int64_t n = rows_of(a, b, &r0);
+    if (n == 0) return 0;
+    return a.nkv * ((n * a.group + Q - 1) / Q) * steps_of<NB>(a, a.lens[b]);
+  };
+  int64_t mine = 0;
+  for (int k = 0; k < per_thread; ++k) {
+    const int64_t b = static_cast<int64_t>(tid) * per_thread + k;
+    if (b < a.B) mine += units(b);
+  }
+  s_scan[tid] = mine;
+  __syncthreads();
+  int64_t before = 0, U = 0;
+  for (int k = 0; k * per_thread < a.B; ++k) {
+    const int64_t v = s_scan[k];
+    before += k < tid ? v : 0;
+    U += v;
+  }
+  if (U == 0) return;
+  const int64_t C = U < gridDim.x ? U : gridDim.x;
+  const int64_t c = blockIdx.x;
+  if (c >= C) return;
+  const int64_t u0 = c * U / C, u1 = (c + 1) * U / C;
+  if (u0 >= before && u0 < before + mine) {
+    int64_t b = static_cast<int64_t>(tid) * per_thread, at = before;
+    for (int64_t n = units(b); u0 >= at + n; n = units(b)) {
+      at += n;
+      ++b;
+    }
+    s_at[0] = b;
+    s_at[1] = at;
+  }
+  __syncthreads();
+  int64_t b = s_at[0], ub = s_at[1];
+
+  for (int64_t u = u0; u < u1;) {
+    int64_t r0;
+    const int64_t n = rows_of(a, b, &r0);
+    const int64_t len = n ? a.lens[b] : 0;
+    const int64_t steps = steps_of<NB>(a, len);
+    const int64_t nqb = (n * a.group + Q - 1) / Q;
+    const int64_t all = a.nkv * nqb * steps;
+    if (u >= ub + all) {
+      ub += all;
+      ++b;
+      continue;
+    }
+    const int64_t item = (u - ub) / steps, i0 = ub + item * steps;
+    const int64_t s0 = u - i0, s1 = steps < s0 + (u1 - u) ? steps : s0 + (u1 - u);
+    const int h = static_cast<int>(item / nqb);
+    const int64_t q0 = (item - h * nqb) * Q;   // first query of the item
+    const int64_t nqueries = n * a.group;
+
+    // positions [0, lim) that a query sees
+    const int64_t cap = a.width << a.shift;
+    auto limit = [&](int64_t qi) -> int {
+      if (qi >= nqueries) return 0;
+      const int64_t l = len - n + qi / a.group + 1;
+      return static_cast<int>(l < 0 ? 0 : (l > cap ? cap : l));
+    };
+    int lim[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) lim[nb] = limit(q0 + nb * 4 + i);
+    const int64_t last_q = q0 + Q < nqueries ? q0 + Q - 1 : nqueries - 1;
+    const int seen = limit(last_q);   // the last query of the block sees most
+
+    // ---- q: two fp16 columns per query, scaled by a power of two --------------
+    uint32_t qf[NB][KS][2];
+    float F[NB], Qs[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int64_t qi = q0 + nb * 4 + (g >> 1);
+      float x[HD / 4];
+      if (qi < nqueries) {
+        const int64_t r = qi / a.group;
+        const T* p = static_cast<const T*>(a.q) + (r0 + r) * a.q_rs +
+                     (h * a.group + (qi - r * a.group)) * a.q_hs + i * (HD / 4);
+        load_row(p, a.vec, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < HD / 4; ++j) x[j] = 0.f;
+      }
+      float mx = 0.f, sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < HD / 4; ++j) {
+        mx = fmaxf(mx, fabsf(x[j]));
+        sum += x[j];
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
+      // |x| * 2^(14 - e) < 2^15 for the row's largest; e bounded so that both
+      // powers of two are normal
+      int e = static_cast<int>((__float_as_uint(mx) >> 23) & 255u) - 127;
+      e = e < -113 ? -113 : (e > 117 ? 117 : e);
+      const float up = pow2i(14 - e);
+      const float f = pow2i(10 + e) * a.scale, qs = sum * a.scale;
+      F[nb] = __shfl_sync(0xffffffffu, f, 8 * i);
+      Qs[nb] = __shfl_sync(0xffffffffu, qs, 8 * i);
+      auto limb = [&](float v) -> __half {
+        const uint32_t w = split_h2(v * up);
+        return __ushort_as_half(static_cast<unsigned short>(g & 1 ? w >> 16 : w & 0xFFFFu));
+      };
+      const __half r16 = __ushort_as_half(0x2C00);   // 1 / 16
+#pragma unroll
+      for (int m = 0; m < KW; ++m) {
+        const float* e8 = x + 8 * m;
+        qf[nb][2 * m][0] = pack_h2(limb(e8[0]), limb(e8[4]));
+        qf[nb][2 * m][1] = pack_h2(__hmul(limb(e8[1]), r16), __hmul(limb(e8[5]), r16));
+        qf[nb][2 * m + 1][0] = pack_h2(limb(e8[2]), limb(e8[6]));
+        qf[nb][2 * m + 1][1] = pack_h2(__hmul(limb(e8[3]), r16), __hmul(limb(e8[7]), r16));
+      }
+    }
+
+    float acc[NB][KS][4], m[NB], l[NB], zs[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = kNegInf;
+      l[nb] = zs[nb] = 0.f;
+#pragma unroll
+      for (int t = 0; t < KS; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nb][t][j] = 0.f;
+    }
+    int ev = -100;                       // weights are p * s * 2^(9 - ev)
+    float s_lim = pow2i(ev + 1), w_up = pow2i(9 - ev);
+
+    // ---- tiles of this warp ----------------------------------------------------
+    const int32_t* tab = a.table + b * a.width;
+    const int64_t t_end64 = (s1 * kAttnStep < seen ? s1 * kAttnStep : seen);
+    const int t_end = static_cast<int>(t_end64);
+    int pos = static_cast<int>(s0 * kAttnStep) + warp * kAttnTile;
+    auto page_at = [&](int p) -> int { return p < t_end ? __ldg(tab + (p >> a.shift)) : -1; };
+    Tile<HD> cur, nxt;
+    cur.ok = nxt.ok = false;
+    if (pos < t_end) cur.load(a, h, page_at(pos), pos, g, i);
+    int page_next = page_at(pos + kAttnStep);
+    for (; pos < t_end; pos += kAttnStep) {
+      nxt.ok = false;
+      if (pos + kAttnStep < t_end) {
+        nxt.load(a, h, page_next, pos + kAttnStep, g, i);
+        page_next = page_at(pos + 2 * kAttnStep);
+      }
+      if (cur.ok) {
+        // scores
+        float sc[NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[nb][j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const uint32_t x = cur.k[0][w], y = cur.k[1][w];
+          const uint32_t x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            mma_f16(sc[nb], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u,
+                    qf[nb][2 * w][0], qf[nb][2 * w][1]);
+            mma_f16(sc[nb], x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u,
+                    y8 & 0x00F000F0u, qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
+          }
+        }
+        const float sk0 = par_s(cur.kp[0]), zk0 = par_z(cur.kp[0]);
+        const float sk1 = par_s(cur.kp[1]), zk1 = par_z(cur.kp[1]);
+        const float sv0 = par_s(cur.vp[0]), sv1 = par_s(cur.vp[1]);
+        const float zc0 = fmaf(8.f, sv0, par_z(cur.vp[0]));
+        const float zc1 = fmaf(8.f, sv1, par_z(cur.vp[1]));
+        float x0[NB], x1[NB];
+        bool v0[NB], v1[NB], renew = false;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          v0[nb] = pos + g < lim[nb];
+          v1[nb] = pos + g + 8 < lim[nb];
+          x0[nb] = v0[nb] ? fmaf((sc[nb][0] + sc[nb][1]) * F[nb], sk0, zk0 * Qs[nb]) : kNegInf;
+          x1[nb] = v1[nb] ? fmaf((sc[nb][2] + sc[nb][3]) * F[nb], sk1, zk1 * Qs[nb]) : kNegInf;
+          renew = renew || x0[nb] > m[nb] + 4.f || x1[nb] > m[nb] + 4.f ||
+                  (v0[nb] && sv0 >= s_lim) || (v1[nb] && sv1 >= s_lim);
+        }
+        if (__any_sync(0xffffffffu, renew)) {
+          // new maximum per query and new exponent of V's steps
+          float sm = 0.f;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            if (v0[nb]) sm = fmaxf(sm, sv0);
+            if (v1[nb]) sm = fmaxf(sm, sv1);
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, o));
+          const int es = static_cast<int>((__float_as_uint(sm) >> 23) & 255u) - 127;
+          const int ev_old = ev;
+          ev = es > ev ? es : ev;
+          s_lim = ev >= 127 ? INFINITY : pow2i(ev + 1);
+          w_up = pow2i(9 - ev);
+          const float down = ev_old - ev < -126 ? 0.f : pow2i(ev_old - ev);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float t = fmaxf(x0[nb], x1[nb]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            const float mn = fmaxf(m[nb], t);
+            const float al = m[nb] == kNegInf ? 1.f : ex2(m[nb] - mn);
+            m[nb] = mn;
+            l[nb] *= al;
+            zs[nb] *= al;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[nb][k][j] *= al * down;
+          }
+        }
+        uint32_t wb[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          // selected, not multiplied, away: a hidden position may hold anything
+          const float p0 = v0[nb] ? ex2(x0[nb] - m[nb]) : 0.f;
+          const float p1 = v1[nb] ? ex2(x1[nb] - m[nb]) : 0.f;
+          l[nb] += p0 + p1;
+          zs[nb] = fmaf(p0, v0[nb] ? zc0 : 0.f, fmaf(p1, v1[nb] ? zc1 : 0.f, zs[nb]));
+          wb[nb][0] = trans8x8(split_h2(v0[nb] ? p0 * (sv0 * w_up) : 0.f));
+          wb[nb][1] = trans8x8(split_h2(v1[nb] ? p1 * (sv1 * w_up) : 0.f));
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7632u : 0x5410u;
+            uint32_t ha[4], hb[4];
+            centred4(prmt(cur.v[0][w], cur.v[1][w], sel), ha);
+            centred4(prmt(cur.v[2][w], cur.v[3][w], sel), hb);
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                mma_f16(acc[nb][w * 4 + half * 2 + p], ha[2 * p], ha[2 * p + 1], hb[2 * p],
+                        hb[2 * p + 1], wb[nb][0], wb[nb][1]);
+          }
+        }
+      }
+      cur = nxt;
+    }
+
+    // ---- the warps' partials, relative to each warp's maximum -----------------
+    const float w_down = pow2i(ev - 9);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], o);
+        zs[nb] += __shfl_xor_sync(0xffffffffu, zs[nb], o);
+      }
+      float* o = s_o + (warp * Q + nb * 4 + i) * HD + g * (HD / 8);
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        o[2 * t] = fmaf(acc[nb][t][0] + acc[nb][t][1], w_down, zs[nb]);
+        o[2 * t + 1] = fmaf(acc[nb][t][2] + acc[nb][t][3], w_down, zs[nb]);
+      }
+      if (g == 0) {
+        s_ml[(warp * Q + nb * 4 + i) * 2] = m[nb];
+        s_ml[(warp * Q + nb * 4 + i) * 2 + 1] = l[nb];
+      }
+    }
+    __syncthreads();
+
+    // ---- merge: the warps, then (for a shared item) the CTAs -------------------
+    const int64_t c_first = ((i0 + 1) * C - 1) / U, c_last = ((i0 + steps) * C - 1) / U;
+    const int parts = static_cast<int>(c_last - c_first) + 1;
+    auto store = [&](int qq, int d, float o, float lsum) {
+      const int64_t qi = q0 + qq;
+      if (qi >= nqueries) return;
+      const int64_t r = qi / a.group;
+      static_cast<T*>(a.out)[(r0 + r) * a.o_rs + (h * a.group + (qi - r * a.group)) * a.o_hs + d] =
+          from_f<T>(lsum == 0.f ? 0.f : o / lsum);
+    };
+    float* mypart = a.part + (c * 2 + (c == c_first && u0 < i0 ? 1 : 0)) * (Q * (HD + 2));
+    for (int e = tid; e < Q * HD; e += kAttnThreads) {
+      const int qq = e / HD, d = e - qq * HD;
+      float M = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, s_ml[(w * Q + qq) * 2]);
+      float o = 0.f, ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) {
+        const float mw = s_ml[(w * Q + qq) * 2];
+        const float f = mw == kNegInf ? 0.f : ex2(mw - M);
+        o = fmaf(f, s_o[(w * Q + qq) * HD + d], o);
+        ls = fmaf(f, s_ml[(w * Q + qq) * 2 + 1], ls);
+      }
+      if (parts == 1) {
+        store(qq, d, o, ls);
+      } else {
+        __stcg(mypart + qq * HD + d, o);
+        if (d == 0) {
+          __stcg(mypart + Q * HD + qq * 2, M);
+          __stcg(mypart + Q * HD + qq * 2 + 1, ls);
+        }
+      }
+    }
+    if (parts > 1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned old = atomicAdd(a.tickets + c_first, 1u);
+        *s_last = old == static_cast<unsigned>(parts - 1);
+      }
+      __syncthreads();
+      if (*s_last) {
+        __threadfence();
+        // an item begins in its first CTA's last segment (slot 1 unless that CTA begins with
+        // it) and is the first segment (slot 0) of the others
+        const int64_t first_u0 = c_first * U / C;
+        auto part = [&](int k) -> const float* {
+          const int64_t slot = k == 0 && first_u0 < i0 ? 1 : 0;
+          return a.part + ((c_first + k) * 2 + slot) * (Q * (HD + 2));
+        };
+        for (int e = tid; e < Q * HD; e += kAttnThreads) {
+          const int qq = e / HD, d = e - qq * HD;
+          float M = kNegInf;
+          for (int k = 0; k < parts; ++k) M = fmaxf(M, __ldcg(part(k) + Q * HD + qq * 2));
+          float o = 0.f, ls = 0.f;
+          for (int k = 0; k < parts; ++k) {
+            const float* p = part(k);
+            const float mk = __ldcg(p + Q * HD + qq * 2);
+            const float f = mk == kNegInf ? 0.f : ex2(mk - M);
+            o = fmaf(f, __ldcg(p + qq * HD + d), o);
+            ls = fmaf(f, __ldcg(p + Q * HD + qq * 2 + 1), ls);
+          }
+          store(qq, d, o, ls);
+        }
+        if (tid == 0) a.tickets[c_first] = 0u;   // ready for the next call
+      }
+    }
+    __syncthreads();   // shared memory is reused by the next segment
+    u += s1 - s0;
+  }
+}
+
+}  // namespace kv4
+}  // namespace qz

@@ -1,0 +1,253 @@
+// qz_kv4_api.cuh -- C entry points of the paged 4-bit KV cache (the last part of
+// qz_api.cu's translation unit): argument checks, variant choice, launches.
+#pragma once
+
+#include "qz_kv4.cuh"
+
+namespace {
+
+// Programmatic dependent launch of a kernel that waits for its predecessors
+// itself (pdl_wait), optionally as clusters of `cluster` CTAs.
+template <class A>
+int launch_kv4(void (*fn)(A), int grid, int threads, int smem, cudaStream_t st, const A& args,
+               int cluster = 1) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[n].val.programmaticStreamSerializationAllowed = 1;
+  ++n;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = static_cast<unsigned>(n);
+  QZ_CUDA(cudaLaunchKernelEx(&cfg, fn, args));
+  return QZ_OK;
+}
+
+// log2 of a page size the kernels take (16 .. 256, a power of two), else -1.
+int page_shift(int64_t page_size) {
+  for (int s = 4; s <= 8; ++s)
+    if (page_size == (int64_t(1) << s)) return s;
+  return -1;
+}
+
+int check_kv4_pool(const void* pool, int64_t pages, int64_t page_size, int nkv, int hd,
+                   const std::string& who) {
+  if (nkv < 1) return fail(QZ_ERR_INVALID, who + ": n_kv must be >= 1");
+  if (hd != 64 && hd != 128) return fail(QZ_ERR_INVALID, who + ": head_dim must be 64 or 128");
+  if (page_shift(page_size) < 0)
+    return fail(QZ_ERR_INVALID, who + ": page size must be 16, 32, 64, 128 or 256");
+  if (pages < 1 || pages > 0x7FFFFFFFll) return fail(QZ_ERR_INVALID, who + ": bad page count");
+  if (!pool || !aligned16(pool))
+    return fail(QZ_ERR_INVALID, who + ": null or unaligned pool (16 bytes)");
+  return QZ_OK;
+}
+
+int check_kv4_heads(int nq, int nkv, const std::string& who) {
+  if (nq < 1 || nkv < 1 || nq % nkv)
+    return fail(QZ_ERR_INVALID, who + ": query heads must be a multiple of kv heads");
+  return QZ_OK;
+}
+
+int dtype_bytes(int dtype) { return dtype == qz::kv4::kF32 ? 4 : 2; }
+
+// Whether rows of `hd` elements at p + i * rs + j * hs all start on 16 bytes.
+bool rows_aligned(const void* p, int64_t rs, int64_t hs, int dtype) {
+  const int64_t b = dtype_bytes(dtype);
+  return aligned16(p) && (rs * b) % 16 == 0 && (hs * b) % 16 == 0;
+}
+
+template <class T>
+int launch_append(const DeviceInfo& d, int hd, const qz::kv4::AppendArgs& a, cudaStream_t st) {
+  const int per_block = qz::kv4::kAppendThreads / (hd / 16);
+  const int64_t want = qz::cdiv(a.n * a.nkv * 2, per_block);
+  const int grid = static_cast<int>(std::min<int64_t>(want, int64_t(d.sms) * 8));
+  return hd == 64 ? launch_kv4(qz::kv4::append_kernel<T, 64>, grid, qz::kv4::kAppendThreads, 0, st, a)
+                  : launch_kv4(qz::kv4::append_kernel<T, 128>, grid, qz::kv4::kAppendThreads, 0, st, a);
+}
+
+// 4 queries (row, head) of a kv head per item where no request has more, else
+// 8; the grid is the CTAs that fit the GPU at once.
+int attn_blocks(int64_t max_rows, int group) { return max_rows * group > 4 ? 2 : 1; }
+
+struct Kv4AttnLayout {
+  int grid;
+  int64_t part_off, total;
+};
+
+Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int nb, int hd) {
+  Kv4AttnLayout l;
+  l.grid = d.sms * qz::kv4::attn_per_sm(hd, nb);
+  l.part_off = qz::cdiv(int64_t(l.grid) * 4, 256) * 256;
+  l.total = l.part_off + int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4;
+  return l;
+}
+
+template <class T, int HD, int NB>
+int launch_kv4_attn(const qz::kv4::AttnArgs& a, int grid, cudaStream_t st) {
+  return launch_kv4(qz::kv4::attn_kernel<T, HD, NB>, grid, qz::kv4::kAttnThreads,
+                    qz::kv4::attn_smem<HD, NB>(), st, a);
+}
+
+template <class T>
+int launch_kv4_attn_t(int hd, int nb, const qz::kv4::AttnArgs& a, int grid, cudaStream_t st) {
+  if (hd == 64)
+    return nb == 1 ? launch_kv4_attn<T, 64, 1>(a, grid, st) : launch_kv4_attn<T, 64, 2>(a, grid, st);
+  return nb == 1 ? launch_kv4_attn<T, 128, 1>(a, grid, st) : launch_kv4_attn<T, 128, 2>(a, grid, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int qz_kv4_plan(const int64_t* lens, const int64_t* new_rows, int64_t B, int32_t* block_table,
+                int64_t width, const int32_t* free_pages, int64_t n_free, const int64_t* used,
+                int64_t page_size, int64_t rows, int64_t* cu_rows, int64_t* lens_out,
+                int64_t* used_out, int64_t* slots, int64_t* positions, void* stream) {
+  if (B < 1 || B > qz::kv4::kPlanMaxB)
+    return fail(QZ_ERR_INVALID, "qz_kv4_plan: requests must be 1 .. 4096");
+  const int shift = page_shift(page_size);
+  if (shift < 0)
+    return fail(QZ_ERR_INVALID, "qz_kv4_plan: page size must be 16, 32, 64, 128 or 256");
+  if (width < 1 || width > (int64_t(1) << 30) / page_size)
+    return fail(QZ_ERR_INVALID, "qz_kv4_plan: table width must be 1 .. 2^30 / page size");
+  if (n_free < 0 || n_free > 0x7FFFFFFFll || rows < 0 || rows > (int64_t(1) << 30))
+    return fail(QZ_ERR_INVALID, "qz_kv4_plan: bad free-page or row count");
+  if (!lens || !new_rows || !block_table || (n_free && !free_pages) || !used || !cu_rows ||
+      !lens_out || !used_out || (rows && (!slots || !positions)))
+    return fail(QZ_ERR_INVALID, "qz_kv4_plan: null pointer");
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  qz::kv4::PlanArgs a{lens, new_rows, block_table, free_pages, used, cu_rows, lens_out, used_out,
+                      slots, positions, width, n_free, rows, static_cast<int>(B), shift};
+  const int smem = qz::kv4::plan_smem(static_cast<int>(B));
+  if (smem > 48 * 1024)
+    QZ_CUDA(allow_smem(qz::kv4::plan_kernel, qz::kv4::plan_smem(qz::kv4::kPlanMaxB)));
+  // one CTA writes a small plan; a large one is shared out over a cluster
+  const int grid = rows + 4 * B > 4096 ? qz::kv4::kPlanCluster : 1;
+  return launch_kv4(qz::kv4::plan_kernel, grid, qz::kv4::kPlanThreads, smem,
+                    static_cast<cudaStream_t>(stream), a, grid);
+}
+
+int qz_kv4_append(const void* k, const void* v, int dtype, int64_t k_row_stride,
+                  int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t n,
+                  int nkv, int hd, uint8_t* pool, int64_t pages, int64_t page_size,
+                  const int64_t* slots, void* stream) {
+  if (int rc = check_kv4_pool(pool, pages, page_size, nkv, hd, "qz_kv4_append")) return rc;
+  if (dtype < 0 || dtype > 2) return fail(QZ_ERR_INVALID, "qz_kv4_append: unknown dtype");
+  if (n < 0 || n > (int64_t(1) << 40) / nkv) return fail(QZ_ERR_INVALID, "qz_kv4_append: bad row count");
+  if (n == 0) return QZ_OK;
+  if (!k || !v || !slots) return fail(QZ_ERR_INVALID, "qz_kv4_append: null pointer");
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  qz::kv4::AppendArgs a{k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride, pool,
+                        slots, n, pages * page_size, nkv, page_shift(page_size), 0};
+  a.vec = rows_aligned(k, k_row_stride, k_head_stride, dtype) &&
+          rows_aligned(v, v_row_stride, v_head_stride, dtype);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case qz::kv4::kF32: return launch_append<float>(*d, hd, a, st);
+    case qz::kv4::kBF16: return launch_append<__nv_bfloat16>(*d, hd, a, st);
+    default: return launch_append<__half>(*d, hd, a, st);
+  }
+}
+
+int qz_kv4_gather(const uint8_t* pool, int64_t pages, int64_t page_size, int nkv, int hd,
+                  const int64_t* slots, int64_t n, float* k, float* v, void* stream) {
+  if (int rc = check_kv4_pool(pool, pages, page_size, nkv, hd, "qz_kv4_gather")) return rc;
+  if (n < 0 || n > (int64_t(1) << 40) / nkv) return fail(QZ_ERR_INVALID, "qz_kv4_gather: bad row count");
+  if (n == 0) return QZ_OK;
+  if (!k || !v || !slots) return fail(QZ_ERR_INVALID, "qz_kv4_gather: null pointer");
+  if (!aligned16(k) || !aligned16(v))
+    return fail(QZ_ERR_INVALID, "qz_kv4_gather: k and v must be 16-byte aligned");
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  const qz::kv4::GatherArgs a{pool, slots, k, v, n, pages * page_size, nkv, page_shift(page_size)};
+  const int per_block = qz::kv4::kGatherThreads / (hd / 4);
+  const int grid = static_cast<int>(
+      std::min<int64_t>(qz::cdiv(n * nkv * 2, per_block), int64_t(d->sms) * 8));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return hd == 64 ? launch_kv4(qz::kv4::gather_kernel<64>, grid, qz::kv4::kGatherThreads, 0, st, a)
+                  : launch_kv4(qz::kv4::gather_kernel<128>, grid, qz::kv4::kGatherThreads, 0, st, a);
+}
+
+int qz_kv4_attention_workspace_bytes(int nq, int nkv, int hd, int64_t max_rows, int64_t* bytes) {
+  if (!bytes) return fail(QZ_ERR_INVALID, "qz_kv4_attention_workspace_bytes: null pointer");
+  if (int rc = check_kv4_heads(nq, nkv, "qz_kv4_attention_workspace_bytes")) return rc;
+  if (hd != 64 && hd != 128)
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention_workspace_bytes: head_dim must be 64 or 128");
+  if (max_rows < 1)
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention_workspace_bytes: max_rows must be >= 1");
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  *bytes = kv4_attn_layout(*d, attn_blocks(max_rows, nq / nkv), hd).total;
+  return QZ_OK;
+}
+
+int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_head_stride,
+                     void* out, int64_t out_row_stride, int64_t out_head_stride,
+                     const uint8_t* pool, int64_t pages, int64_t page_size,
+                     const int32_t* block_table, int64_t width, const int64_t* lens,
+                     const int64_t* cu_rows, int64_t B, int64_t n, int64_t max_rows, int nq,
+                     int nkv, int hd, float scale, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_kv4_heads(nq, nkv, "qz_kv4_attention")) return rc;
+  if (int rc = check_kv4_pool(pool, pages, page_size, nkv, hd, "qz_kv4_attention")) return rc;
+  if (dtype < 0 || dtype > 2) return fail(QZ_ERR_INVALID, "qz_kv4_attention: unknown dtype");
+  if (B < 0 || B > qz::kv4::kAttnMaxB)
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention: requests must be 0 .. 4096");
+  if (n < 0 || n > (int64_t(1) << 30)) return fail(QZ_ERR_INVALID, "qz_kv4_attention: bad row count");
+  if (width < 1 || width > (int64_t(1) << 30) / page_size)
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention: table width must be 1 .. 2^30 / page size");
+  if (max_rows < 1 || (!cu_rows && max_rows != 1))
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention: max_rows must be >= 1, and 1 without cu_rows");
+  if (B == 0 || n == 0) return QZ_OK;
+  if (!q || !out || !block_table || !lens || !ws)
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention: null pointer");
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  const int group = nq / nkv, nb = attn_blocks(max_rows, group);
+  const Kv4AttnLayout L = kv4_attn_layout(*d, nb, hd);
+  if (static_cast<int64_t>(ws_bytes) < L.total || !aligned_to(ws, 256))
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention: workspace too small or not 256-byte aligned");
+  qz::kv4::AttnArgs a{};
+  a.q = q;
+  a.out = out;
+  a.q_rs = q_row_stride;
+  a.q_hs = q_head_stride;
+  a.o_rs = out_row_stride;
+  a.o_hs = out_head_stride;
+  a.pool = pool;
+  a.table = block_table;
+  a.lens = lens;
+  a.cu = cu_rows;
+  a.tickets = static_cast<unsigned*>(ws);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + L.part_off);
+  a.pages = pages;
+  a.width = width;
+  a.n = n;
+  a.B = static_cast<int>(B);
+  a.nkv = nkv;
+  a.group = group;
+  a.shift = page_shift(page_size);
+  a.scale = scale * 1.44269504088896341f;
+  a.vec = rows_aligned(q, q_row_stride, q_head_stride, dtype);
+  a.rows_lo = 0;
+  a.rows_hi = static_cast<int>(std::min<int64_t>(max_rows, 0x7FFFFFFF));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case qz::kv4::kF32: return launch_kv4_attn_t<float>(hd, nb, a, L.grid, st);
+    case qz::kv4::kBF16: return launch_kv4_attn_t<__nv_bfloat16>(hd, nb, a, L.grid, st);
+    default: return launch_kv4_attn_t<__half>(hd, nb, a, L.grid, st);
+  }
+}
+
+}  // extern "C"

@@ -19,11 +19,23 @@ Decode-step glue (the fp32 work between the int8 matmuls of one token):
     attention_decode_qkv(qkv, ...)           the two above plus the KV append, one launch
     attention_prefill(q, kc, vc, pos0)       quartz/attention.py:15-43 (causal rows)
     argmax(logits)               -> tokens   quartz/sample.py:21-22
+
+Paged 4-bit KV cache (no counterpart in quartz): sequences of uneven length
+over one pool of pages. ``quartz_b200.paged`` decodes with it.
+
+    kv4_pool(pages, n_kv, hd, page_size)       the zeroed pool of one layer
+    kv4_plan(lens, new_rows, table, free, used, page_size, rows)
+                                               block tables, slots, positions
+    kv4_append(k, v, pool, slots)              quantise and store rows
+    kv4_gather(pool, slots, hd)  -> k, v       the values the rows stand for
+    kv4_attention(q, pool, table, lens, ...)   one row, a few rows or a prompt
 """
 
 from __future__ import annotations
 
+import ctypes
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -538,3 +550,278 @@ def argmax(logits, tokens=None, pos_dev=None, pos_step=0, keys=None):
                                          tokens.data_ptr(), _ptr(pos_dev), int(pos_step),
                                          _stream_ptr(logits.device)))
     return tokens
+
+
+# ---------------------------------------------------------------------------
+# paged 4-bit KV cache
+# ---------------------------------------------------------------------------
+
+KV4_PAGE_SIZES = (16, 32, 64, 128, 256)
+KV4_HEAD_DIMS = (64, 128)
+_KV4_DTYPES = {torch.float32: _lib.QZ_F32, torch.bfloat16: _lib.QZ_BF16,
+               torch.float16: _lib.QZ_F16}
+_kv4_ws: dict[tuple[int, int], torch.Tensor] = {}
+_kv4_ws_need: dict[tuple, int] = {}
+
+
+class KV4Plan(NamedTuple):
+    """What kv4_plan returns: int64 tensors. Rows of request b are
+    cu_rows[b] .. cu_rows[b + 1] - 1; lens and used are the successors of the
+    arguments; slots and positions are per row (-1: no place in the cache, and
+    rows behind the last request's)."""
+    cu_rows: torch.Tensor
+    lens: torch.Tensor
+    used: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+
+
+class _on:
+    """Makes the tensors' device current for a library call (nothing to do in
+    the usual case that it is)."""
+    __slots__ = ("idx", "prev")
+
+    def __init__(self, dev: torch.device):
+        self.idx = dev.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.prev != self.idx:
+            torch.cuda.set_device(self.prev)
+
+
+def kv4_block_bytes(page_size: int, head_dim: int) -> int:
+    """Bytes of one page of one kv head: K and V codes and their (s, z) pairs."""
+    if page_size not in KV4_PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {KV4_PAGE_SIZES}, got {page_size}")
+    if head_dim not in KV4_HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {KV4_HEAD_DIMS}, got {head_dim}")
+    return page_size * (head_dim + 8)
+
+
+def kv4_pool(pages: int, n_kv: int, head_dim: int, page_size: int, device=None) -> torch.Tensor:
+    """The zeroed pool of one layer, uint8 [pages, n_kv, page_size * (head_dim + 8)]."""
+    nbytes = kv4_block_bytes(page_size, head_dim)
+    return torch.zeros((pages, n_kv, nbytes), dtype=torch.uint8,
+                       device=torch.device("cuda", ensure_device(device)))
+
+
+def _kv4_page_size(pool: torch.Tensor, head_dim: int) -> int:
+    """The page size of a pool (checked against head_dim)."""
+    if head_dim not in KV4_HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {KV4_HEAD_DIMS}, got {head_dim}")
+    _need(pool, torch.uint8, "pool", 3)
+    ps, rest = divmod(pool.shape[2], head_dim + 8)
+    if rest or ps not in KV4_PAGE_SIZES:
+        raise ValueError(f"pool blocks of {pool.shape[2]} bytes are no pages of head_dim {head_dim}")
+    return ps
+
+
+def _kv4_rows(t: torch.Tensor, name: str) -> None:
+    """Rows [n, heads, head_dim] on the GPU, any strides with contiguous head_dim."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in _KV4_DTYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [rows, heads, head_dim], got shape {tuple(t.shape)}")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name} must be contiguous along head_dim")
+
+
+def kv4_plan(lens, new_rows, block_table, free_pages, used, page_size, rows, lens_out=None,
+             used_out=None) -> KV4Plan:
+    """Block tables and slot maps of one step, built on the GPU from request lengths.
+
+    lens, new_rows: int64 [B], the positions each request holds and the rows
+    that join it now (B <= 4096). block_table: int32 [B, W], written in place
+    (new entries only). free_pages: int32 [F] in the order they are handed out,
+    used: int64 [1], how many of them are taken. rows: the row capacity of this
+    step (padding included). A request whose rows do not fit `rows`, whose pages
+    do not fit W, or for which the free pages do not last (counted in order)
+    keeps its length and gets slots -1. lens_out / used_out may be lens / used
+    themselves (a step captured in a CUDA graph then advances them)."""
+    _need(lens, torch.int64, "lens", 1)
+    _need(new_rows, torch.int64, "new_rows", 1)
+    _need(block_table, torch.int32, "block_table", 2)
+    _need(free_pages, torch.int32, "free_pages", 1)
+    _need(used, torch.int64, "used")
+    B, W = block_table.shape
+    rows = int(rows)
+    if lens.numel() != B or new_rows.numel() != B:
+        raise ValueError(f"lens and new_rows must have one element per table row ({B})")
+    if used.numel() != 1:
+        raise ValueError("used must have one element")
+    if rows < 0:
+        raise ValueError("rows must not be negative")
+    dev = lens.device
+    ensure_device(dev)
+    buf = torch.empty(2 * B + 2 + 2 * rows, dtype=torch.int64, device=dev)
+    cu, lo, uo, slots, positions = buf.split((B + 1, B, 1, rows, rows))
+    if lens_out is not None:
+        _need(lens_out, torch.int64, "lens_out", 1)
+        if lens_out.numel() != B:
+            raise ValueError(f"lens_out must have {B} elements")
+        lo = lens_out
+    if used_out is not None:
+        _need(used_out, torch.int64, "used_out")
+        if used_out.numel() != 1:
+            raise ValueError("used_out must have one element")
+        uo = used_out
+    _same_device(dev, new_rows, block_table, free_pages, used, lo, uo)
+    with _on(dev):
+        _lib.check(_lib.load().qz_kv4_plan(
+            lens.data_ptr(), new_rows.data_ptr(), B, block_table.data_ptr(), W,
+            free_pages.data_ptr(), free_pages.numel(), used.data_ptr(), int(page_size), rows,
+            cu.data_ptr(), lo.data_ptr(), uo.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+            _stream_ptr(dev)))
+    return KV4Plan(cu, lo, uo, slots, positions)
+
+
+def kv4_append(k, v, pool, slots) -> None:
+    """Quantise rows k, v [n, n_kv, hd] (float32, bfloat16 or float16; hd
+    contiguous, other strides free) to 4 bits and store row r at slots[r]
+    (int64 [n]; a slot outside the pool stores nothing). Each row of a kv head
+    keeps its own bf16 step and zero; a row with a non-finite value reads back
+    as NaN. A slot must not appear twice in one call."""
+    _kv4_rows(k, "k")
+    _kv4_rows(v, "v")
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k and v must have the same shape and dtype")
+    n, nkv, hd = k.shape
+    ps = _kv4_page_size(pool, hd)
+    if pool.shape[1] != nkv:
+        raise ValueError(f"pool has {pool.shape[1]} kv heads, k has {nkv}")
+    _need(slots, torch.int64, "slots", 1)
+    if slots.numel() != n:
+        raise ValueError(f"slots must have one element per row ({n})")
+    dev = pool.device
+    ensure_device(dev)
+    _same_device(dev, k, v, slots)
+    with _on(dev):
+        _lib.check(_lib.load().qz_kv4_append(
+            k.data_ptr(), v.data_ptr(), _KV4_DTYPES[k.dtype], k.stride(0), k.stride(1),
+            v.stride(0), v.stride(1), n, nkv, hd, pool.data_ptr(), pool.shape[0], ps,
+            slots.data_ptr(), _stream_ptr(dev)))
+
+
+def kv4_gather(pool, slots, head_dim, out=None):
+    """(k, v) fp32 [n, n_kv, head_dim]: the values at slots (int64 [n]); zeros
+    for a slot outside the pool. out: a pair of contiguous tensors to write."""
+    ps = _kv4_page_size(pool, int(head_dim))
+    _need(slots, torch.int64, "slots", 1)
+    dev = pool.device
+    ensure_device(dev)
+    n, nkv = slots.numel(), pool.shape[1]
+    if out is None:
+        k, v = torch.empty((2, n, nkv, head_dim), dtype=torch.float32, device=dev).unbind(0)
+    else:
+        k, v = out
+        for t, name in ((k, "out[0]"), (v, "out[1]")):
+            _need(t, torch.float32, name, 3)
+            if tuple(t.shape) != (n, nkv, head_dim):
+                raise ValueError(f"{name} must be [{n}, {nkv}, {head_dim}], got {tuple(t.shape)}")
+    _same_device(dev, slots, k, v)
+    with _on(dev):
+        _lib.check(_lib.load().qz_kv4_gather(
+            pool.data_ptr(), pool.shape[0], ps, nkv, int(head_dim), slots.data_ptr(), n,
+            k.data_ptr(), v.data_ptr(), _stream_ptr(dev)))
+    return k, v
+
+
+def kv4_attention_workspace(device, n_heads: int, n_kv: int, head_dim: int, max_rows: int = 1
+                            ) -> torch.Tensor:
+    """A new zeroed workspace of kv4_attention for calls with up to max_rows rows
+    per request. The calls leave it ready for the next one; calls that may
+    overlap on the GPU (other streams, graphs replayed side by side) must not
+    share one."""
+    idx = ensure_device(device)
+    return torch.zeros(_kv4_ws_bytes(idx, n_heads, n_kv, head_dim, max_rows), dtype=torch.uint8,
+                       device=torch.device("cuda", idx))
+
+
+def _kv4_ws_bytes(idx: int, nq: int, nkv: int, hd: int, max_rows: int) -> int:
+    key = (idx, nq, nkv, hd, max_rows)
+    need = _kv4_ws_need.get(key)
+    if need is None:
+        b = ctypes.c_int64(0)
+        with _on(torch.device("cuda", idx)):
+            _lib.check(_lib.load().qz_kv4_attention_workspace_bytes(nq, nkv, hd, max_rows,
+                                                                    ctypes.byref(b)))
+        if len(_kv4_ws_need) > 4096:
+            _kv4_ws_need.clear()
+        need = _kv4_ws_need[key] = b.value
+    return need
+
+
+def _kv4_default_ws(dev: torch.device, stream: int, need: int) -> torch.Tensor:
+    """The workspace of a call that brings none: one per device and stream. A call
+    under stream capture gets its own, so that two graphs (or a graph and eager
+    calls) never share one."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(need, dtype=torch.uint8, device=dev)
+    ws = _kv4_ws.get((dev.index, stream))
+    if ws is None or ws.numel() < need:
+        ws = _kv4_ws[dev.index, stream] = torch.zeros(need, dtype=torch.uint8, device=dev)
+    return ws
+
+
+def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=None, out=None,
+                  workspace=None):
+    """softmax(scale * q K^T) V of query rows over the paged 4-bit cache.
+
+    q: [n, n_heads, hd] (float32, bfloat16 or float16; hd contiguous). Rows
+    cu_rows[b] .. cu_rows[b + 1] - 1 are the last rows of request b, whose
+    lens[b] positions (int64 [B], this step's included) lie in the pages
+    block_table[b] (int32 [B, W]); each sees the positions up to its own, and
+    one that sees none gives zeros. cu_rows (int64 [B + 1]) None: row b is
+    request b's. max_rows: the most rows a request has (a host number; rows of
+    a request with more are not computed). scale: hd ** -0.5 unless given.
+    Returns out (q's dtype); rows of no request are left as they were. out may
+    be q itself."""
+    _kv4_rows(q, "q")
+    n, nq, hd = q.shape
+    ps = _kv4_page_size(pool, hd)
+    nkv = pool.shape[1]
+    _need(block_table, torch.int32, "block_table", 2)
+    _need(lens, torch.int64, "lens", 1)
+    B, W = block_table.shape
+    if lens.numel() != B:
+        raise ValueError(f"lens must have one element per table row ({B})")
+    max_rows = int(max_rows)
+    if cu_rows is not None:
+        _need(cu_rows, torch.int64, "cu_rows", 1)
+        if cu_rows.numel() != B + 1:
+            raise ValueError(f"cu_rows must have {B + 1} elements")
+    if nq % nkv:
+        raise ValueError(f"{nq} query heads are no multiple of {nkv} kv heads")
+    scale = hd ** -0.5 if scale is None else float(scale)
+    dev = pool.device
+    ensure_device(dev)
+    if out is None:
+        out = torch.empty((n, nq, hd), dtype=q.dtype, device=dev)
+    else:
+        _kv4_rows(out, "out")
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must have q's shape and dtype")
+        sr, sh = out.stride(0), out.stride(1)
+        if not ((nq == 1 or sh >= hd) and (n == 1 or sr >= (nq - 1) * sh + hd)
+                or (n == 1 or sr >= hd) and (nq == 1 or sh >= (n - 1) * sr + hd)):
+            raise ValueError("out's rows and heads must not overlap")
+    _same_device(dev, q, block_table, lens, cu_rows, out, workspace)
+    with _on(dev):
+        st = _stream_ptr(dev)
+        need = _kv4_ws_bytes(dev.index, nq, nkv, hd, max_rows)
+        ws = workspace if workspace is not None else _kv4_default_ws(dev, st, need)
+        _lib.check(_lib.load().qz_kv4_attention(
+            q.data_ptr(), _KV4_DTYPES[q.dtype], q.stride(0), q.stride(1), out.data_ptr(),
+            out.stride(0), out.stride(1), pool.data_ptr(), pool.shape[0], ps,
+            block_table.data_ptr(), W, lens.data_ptr(), _ptr(cu_rows), B, n, max_rows, nq, nkv,
+            hd, scale, ws.data_ptr(), ws.numel(), st))
+    return out

@@ -1,0 +1,523 @@
+"""The paged 4-bit KV cache on the GPU against plain 64-bit statements (tests/_kv4.py).
+
+What is integer (plans, codes, parameters) has to be equal; read-back values
+are one fp32 rounding of z + c * s. Attention's bound: q is split into two fp16
+values (2^-23 of the row's largest), the scores accumulate hd / 16 * 2 times in
+fp32 with truncation (2^-23 each) over unsigned codes, whose sums are at most
+about four times sum |q k|; so a score is off by at most
+4 A (hd / 16 + 8) 2^-23 with A = scale * sum |q k|, a weight by that relatively
+plus 2^-21 of exponent and split, and a result by twice it times max |v| (the
+normalisation has the same error), plus the rounding to the output's type.
+"""
+
+import math
+import random
+
+import pytest
+
+from tests import _kv4 as P
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _dev():
+    from quartz_b200 import device as qd
+    return qd, torch.device("cuda", 0)
+
+
+def _i64(x, dev):
+    return torch.tensor(x, dtype=torch.int64, device=dev)
+
+
+# ---------------------------------------------------------------------------
+# plan
+# ---------------------------------------------------------------------------
+
+def _run_plan(lens, joins, table, free, used, page, rows, in_place=False):
+    qd, dev = _dev()
+    tl, tj = _i64(lens, dev), _i64(joins, dev)
+    tt = torch.tensor(table, dtype=torch.int32, device=dev)
+    tf = torch.tensor(free, dtype=torch.int32, device=dev)
+    tu = _i64([used], dev)
+    p = qd.kv4_plan(tl, tj, tt, tf, tu, page, rows, lens_out=tl if in_place else None,
+                    used_out=tu if in_place else None)
+    if in_place:
+        assert p.lens is tl and p.used is tu
+    else:
+        assert tl.tolist() == list(lens) and tu.tolist() == [used]
+    return dict(cu_rows=p.cu_rows.tolist(), lens=p.lens.tolist(), used=p.used.tolist(),
+                slots=p.slots.tolist(), positions=p.positions.tolist(), table=tt.tolist())
+
+
+@pytest.mark.parametrize("B,page,most", [(1, 16, 1), (7, 16, 40), (64, 32, 1), (300, 64, 9),
+                                         (1025, 256, 3), (4096, 16, 2), (40, 128, 700)])
+@pytest.mark.parametrize("short", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_plan(B, page, most, short, in_place):
+    rng = random.Random(B * 7 + page + short)
+    lens = [rng.choice([0, 1, page - 1, page, page + 1, rng.randrange(5 * page)]) for _ in range(B)]
+    joins = [rng.choice([0, 1, most, rng.randrange(most + 1)]) for _ in range(B)]
+    width = max(-(-(h + n) // page) for h, n in zip(lens, joins)) or 1
+    if short:
+        width = max(1, width - 1)          # some requests outgrow the table
+    need = sum(-(-(h + n) // page) - -(-h // page) for h, n in zip(lens, joins))
+    free = rng.sample(range(10 * (need + 9)), need + 3)
+    used = 2
+    if short:
+        free = free[:2 + need // 2]
+    table = [[rng.randrange(1000) for _ in range(width)] for _ in range(B)]
+    rows = sum(joins) + (0 if short else 5)
+    got = _run_plan(lens, joins, table, free, used, page, rows, in_place)
+    want = P.plan(lens, joins, table, free, used, page, rows)
+    assert got == want
+
+
+@pytest.mark.parametrize("case", [
+    dict(lens=[3, 5], joins=[4, 4], rows=6),                 # the second request's rows do not fit
+    dict(lens=[3, 5, 2], joins=[4, 9, 1], rows=6),           # ... nor those of requests behind it
+    dict(lens=[-1, 5], joins=[1, 1], rows=4),                # negative length
+    dict(lens=[3, 5], joins=[-7, 1], rows=4),                # negative row count
+    dict(lens=[48, 0], joins=[1, 48], rows=64),              # the table's width
+    dict(lens=[1 << 40, 0], joins=[1, 1], rows=4),           # a length no table holds
+    dict(lens=[16, 16], joins=[0, 0], rows=0),               # nothing joins
+    dict(lens=[0, 0], joins=[1, 1], rows=2, used=-1),        # a cursor outside the list
+    dict(lens=[0, 16], joins=[1, 0], rows=2, used=99),
+    dict(lens=[0, 1], joins=[1, 1], rows=2, free=[]),        # no free pages; the second needs none
+])
+def test_plan_refuses(case):
+    case = dict(dict(free=[9, 8, 7, 6], used=0), **case)
+    table = [[100 + 10 * b + j for j in range(3)] for b in range(len(case["lens"]))]
+    args = (case["lens"], case["joins"], table, case["free"], case["used"], 16, case["rows"])
+    assert _run_plan(*args) == P.plan(*args)
+
+
+# ---------------------------------------------------------------------------
+# append and gather
+# ---------------------------------------------------------------------------
+
+def _rows(n, nkv, hd, dtype, g, dev, layout="plain"):
+    """k, v [n, nkv, hd] in one of several memory layouts."""
+    def fill():
+        x = torch.randn(n, nkv, hd, generator=g, device=dev)
+        return (x * torch.exp(torch.randn(n, nkv, 1, generator=g, device=dev)) +
+                torch.randn(n, nkv, 1, generator=g, device=dev)).to(dtype)
+    k, v = fill(), fill()
+    if layout == "slices":              # parts of projection rows
+        wide = torch.zeros(n, 4 * nkv, hd, dtype=dtype, device=dev)
+        wide[:, 2 * nkv:3 * nkv], wide[:, 3 * nkv:] = k, v
+        return wide[:, 2 * nkv:3 * nkv], wide[:, 3 * nkv:]
+    if layout == "odd":                 # rows that start off any 16-byte boundary
+        wide = torch.zeros(2, n, nkv, hd + 1, dtype=dtype, device=dev)
+        wide[0, ..., 1:], wide[1, ..., 1:] = k, v
+        return wide[0, ..., 1:], wide[1, ..., 1:]
+    if layout == "heads":               # heads outermost
+        return (k.transpose(0, 1).contiguous().transpose(0, 1),
+                v.transpose(0, 1).contiguous().transpose(0, 1))
+    return k, v
+
+
+def _check_append(k, v, page, pages, slots, fill=0xA5):
+    """Append, compare every byte of the pool, then read back."""
+    qd, dev = _dev()
+    hd, nkv = k.shape[2], k.shape[1]
+    pool = P.empty_pool(pages, nkv, hd, page, fill, dev)
+    want = pool.clone()
+    qd.kv4_append(k, v, pool, slots)
+    P.store(want, hd, slots, k, v)
+    half = page * hd // 2
+    # parameters of NaN rows: any NaN
+    wp, gp = (x[..., 2 * half:].contiguous().view(torch.bfloat16) for x in (want, pool))
+    assert torch.equal(torch.isnan(wp), torch.isnan(gp))
+    assert torch.equal(torch.nan_to_num(wp), torch.nan_to_num(gp))
+    assert torch.equal(want[..., :2 * half], pool[..., :2 * half])
+    gk, gv = qd.kv4_gather(pool, slots, hd)
+    keep = ((slots >= 0) & (slots < pages * page))[:, None, None]
+    for got, x in ((gk, k), (gv, v)):
+        ref = torch.where(keep, P.values(x), 0.0)
+        assert torch.equal(torch.isnan(ref), torch.isnan(got))
+        # z + c * s rounded once to fp32
+        assert torch.equal(torch.nan_to_num(ref).float(), torch.nan_to_num(got))
+    return pool
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,nkv,page,layout", [
+    (1, 1, 16, "plain"), (3, 8, 16, "slices"), (33, 3, 32, "odd"), (257, 2, 64, "heads"),
+    (1000, 5, 128, "slices"), (70, 1, 256, "plain")])
+def test_append_and_gather(dtype, hd, n, nkv, page, layout):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(n + hd)
+    k, v = _rows(n, nkv, hd, DTYPES[dtype], g, dev, layout)
+    pages = n // page + 2
+    slots = torch.randperm(pages * page, generator=g, device=dev)[:n].clone()
+    if n > 2:
+        slots[1] = -1
+        slots[2] = pages * page           # one behind the pool
+    _check_append(k, v, page, pages, slots)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_append_border_values(hd):
+    """Rows at the quantiser's edges: constants, zeros, ties between codes, one
+    outlier, subnormal and huge ranges, and non-finite values in each place."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(5)
+    base = torch.randn(hd, generator=g, device=dev)
+    ties = (torch.arange(hd, device=dev) % 31).float() * 0.5          # z = 0, s = 1: halves tie
+    ladder = torch.full((hd,), -8.0, device=dev)
+    ladder[1:] = (torch.arange(hd - 1, device=dev) % 31) * 0.25 - 8.0
+    rows = [torch.zeros(hd, device=dev), torch.full((hd,), 3.3, device=dev), ties, -ties, ladder,
+            base * 1e-38, base * 1e-42, base * 1e-30, base * 1e38, base * 3e37, base + 1e6,
+            base * 1e-3 + 100.0, torch.full((hd,), -1e-45, device=dev)]
+    spike = base * 1e-3
+    spike[hd // 2] = 1e4
+    rows.append(spike)
+    for bad in (math.nan, math.inf, -math.inf):
+        for at in (0, 15, hd - 1):
+            r = base.clone()
+            r[at] = bad
+            rows.append(r)
+    both = base.clone()
+    both[0], both[1] = 3.3e38, -3.3e38                                 # a range beyond fp32
+    rows.append(both)
+    # values one step to either side of the middle between two codes
+    s = torch.tensor(0.37, device=dev).bfloat16().float()
+    mids = (torch.arange(hd, device=dev) % 15 + 0.5) * s
+    mids[0], mids[1] = 0.0, 15 * s
+    for step in (0, 1, -1):
+        m = mids.clone()
+        m[2:] = torch.nextafter(m[2:], torch.full_like(m[2:], math.inf * step if step else 0)) if step else m[2:]
+        rows.append(m)
+    x = torch.stack(rows)
+    k = x[:, None].contiguous()
+    v = x.flip(0)[:, None].contiguous()
+    pages = -(-len(rows) // 16) + 1
+    _check_append(k, v, 16, pages, torch.arange(len(rows), device=dev))
+
+
+def test_append_to_a_pool_beyond_32_bits():
+    """Slots whose bytes lie past 4 GB."""
+    qd, dev = _dev()
+    if torch.cuda.mem_get_info(0)[0] < 8 << 30:
+        pytest.skip("needs 8 GB of device memory")
+    nkv, hd, page = 8, 128, 256
+    block = nkv * page * (hd + 8)
+    pages = (5 << 30) // block
+    pool = torch.zeros(pages, nkv, page * (hd + 8), dtype=torch.uint8, device=dev)
+    g = torch.Generator(device=dev).manual_seed(1)
+    k, v = _rows(40, nkv, hd, torch.float32, g, dev)
+    slots = torch.arange(40, device=dev) + pages * page - 40
+    qd.kv4_append(k, v, pool, slots)
+    gk, gv = qd.kv4_gather(pool, slots, hd)
+    assert torch.equal(gk, P.values(k).float()) and torch.equal(gv, P.values(v).float())
+    assert not pool[:pages - 1].any()
+    # and attention over the same pages
+    table = torch.full((1, 1), pages - 1, dtype=torch.int32, device=dev)
+    small = pool[pages - 1:].clone()
+    q = torch.randn(1, nkv, hd, generator=g, device=dev)
+    # the 40 rows are the page's last, so the context is the whole page
+    out = qd.kv4_attention(q, pool, table, _i64([page], dev))
+    ref = qd.kv4_attention(q, small, torch.zeros_like(table), _i64([page], dev))
+    assert torch.equal(out, ref)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+def _context(lens, nkv, hd, page, g, dev, extra=2, width=None, k_scale=1.0, v_scale=1.0):
+    """A pool with random rows for every position of every request, pages in a
+    shuffled order; whatever no request holds is filled with NaN parameters."""
+    count = [-(-max(0, t) // page) for t in lens]
+    width = width or max(1, max(count))
+    pages = sum(count) + extra
+    order = torch.randperm(pages, generator=g, device=dev).to(torch.int32)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32, device=dev)
+    pool = P.empty_pool(pages, nkv, hd, page, 0xFF, dev)      # bf16 0xFFFF: NaN
+    at = 0
+    for b, t in enumerate(lens):
+        own = order[at:at + count[b]]
+        at += count[b]
+        table[b, :min(width, count[b])] = own[:width]
+        if t <= 0:
+            continue
+        pos = torch.arange(t, device=dev)
+        slots = own[pos // page].long() * page + pos % page
+        k = torch.randn(t, nkv, hd, generator=g, device=dev) * k_scale
+        v = torch.randn(t, nkv, hd, generator=g, device=dev) * v_scale
+        P.store(pool, hd, slots, k, v)
+    return pool, table
+
+
+def _check_attention(q, pool, table, lens, cu, scale=None, max_rows=1, out=None, **kw):
+    qd, dev = _dev()
+    hd = q.shape[2]
+    s = hd ** -0.5 if scale is None else scale
+    if out is None:
+        out = torch.full_like(q, 0.25, memory_format=torch.contiguous_format)
+    ref, size = P.attention(q, pool, table, lens, cu if cu is not None else list(range(len(lens) + 1)),
+                            s, out, max_rows)
+    got = qd.kv4_attention(q, pool, table, _i64(lens, dev),
+                           cu_rows=None if cu is None else _i64(cu, dev), max_rows=max_rows,
+                           scale=scale, out=out, **kw)
+    assert got is out
+    assert torch.equal(torch.isnan(ref), torch.isnan(got.double()))
+    vmax = torch.nan_to_num(torch.stack(P.load(pool, hd))[1], nan=0.0).abs().max().item() or 1.0
+    bound = vmax * (2 * 4 * size * (hd / 16 + 8) * 2.0 ** -23 + 2.0 ** -19)
+    bound = bound[..., None] + ref.abs() * torch.finfo(q.dtype).eps / 2
+    err = torch.nan_to_num((got.double() - ref).abs(), nan=0.0)
+    worst = (err - torch.nan_to_num(bound, nan=math.inf)).max().item()
+    assert worst <= 0, (worst, err.max().item())
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,nkv", [(1, 1), (4, 2), (8, 2), (6, 2), (10, 2), (8, 1), (16, 1), (20, 1)])
+def test_decode_heads(dtype, hd, nq, nkv):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(nq * 10 + nkv)
+    lens = [37, 1, 130]
+    pool, table = _context(lens, nkv, hd, 16, g, dev)
+    q = torch.randn(len(lens), nq, hd, generator=g, device=dev).to(DTYPES[dtype])
+    _check_attention(q, pool, table, lens, None)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("lens", [[0], [1], [2], [15], [16], [17], [63], [64], [65], [127, 0, 129],
+                                  [5000], [0, 0, 0], [1, 2000, 3, 0, 700, 16], list(range(70))])
+def test_decode_lengths(page, lens):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(page + len(lens))
+    pool, table = _context(lens, 2, 64, page, g, dev)
+    q = torch.randn(len(lens) + 2, 6, 64, generator=g, device=dev)      # two rows of no request
+    _check_attention(q, pool, table, lens, None)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_long(hd):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(hd)
+    lens = [70001, 3]
+    pool, table = _context(lens, 1, hd, 64, g, dev)
+    q = torch.randn(2, 4, hd, generator=g, device=dev) * 2
+    _check_attention(q, pool, table, lens, None)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 2, 128), (3, 1, 64), (8, 1, 128)])
+@pytest.mark.parametrize("rows,lens", [
+    ([2], [2]), ([3], [100]), ([1, 4, 0, 2], [50, 4, 9, 81]), ([5, 1], [3, 1]),   # more rows than positions
+    ([33, 1, 70], [33, 200, 150]), ([130], [300]), ([0, 0], [4, 5])])
+def test_rows(dtype, nq, nkv, hd, rows, lens):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(sum(rows))
+    pool, table = _context(lens, nkv, hd, 16, g, dev)
+    cu = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    q = torch.randn(cu[-1] + 3, nq, hd, generator=g, device=dev).to(DTYPES[dtype])
+    _check_attention(q, pool, table, lens, cu, max_rows=max(1, max(rows)))
+
+
+def test_rows_beyond_max_rows_are_left():
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(2)
+    pool, table = _context([20, 30], 2, 64, 16, g, dev)
+    q = torch.randn(5, 4, 64, generator=g, device=dev)
+    got = _check_attention(q, pool, table, [20, 30], [0, 4, 5], max_rows=3)
+    assert (got[:4] == 0.25).all()
+
+
+def test_lengths_beyond_the_table_and_bad_pages():
+    """Positions past the table are not seen; entries outside the pool are not
+    read (their positions count as unseen), also when all of a request's are bad."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(3)
+    lens = [100, 100, 40, 100000]
+    pool, table = _context([100, 100, 40, 96], 2, 64, 16, g, dev, width=6)
+    table[1, 2] = pool.shape[0]
+    table[1, 4] = -5
+    table[2] = 1 << 30
+    q = torch.randn(4, 4, 64, generator=g, device=dev)
+    got = _check_attention(q, pool, table, lens, None)
+    assert (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("k_scale,v_scale", [(1e-3, 1e-6), (1e-20, 1e20), (1.0, 1e-36), (8.0, 1.0),
+                                             (1e-8, 1e30)])
+def test_value_ranges(k_scale, v_scale):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(4)
+    lens = [90, 33]
+    pool, table = _context(lens, 2, 64, 16, g, dev, k_scale=k_scale, v_scale=v_scale)
+    q = torch.randn(2, 4, 64, generator=g, device=dev) * min(1e6, 1.0 / k_scale)
+    _check_attention(q, pool, table, lens, None)
+
+
+def test_steps_of_very_different_size():
+    """V rows from 1e-25 to 1e25 in one context, in rising and falling order: the
+    weights' exponent has to follow."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(6)
+    for flip in (False, True):
+        t, hd = 200, 64
+        pool, table = _context([t], 1, hd, 16, g, dev)
+        ex = torch.linspace(-25, 25, t, device=dev)
+        v = torch.randn(t, 1, hd, generator=g, device=dev) * torch.pow(10.0, ex.flip(0) if flip else ex)[:, None, None]
+        k = torch.randn(t, 1, hd, generator=g, device=dev)
+        pos = torch.arange(t, device=dev)
+        P.store(pool, hd, table[0][pos // 16].long() * 16 + pos % 16, k, v)
+        _check_attention(torch.randn(1, 4, hd, generator=g, device=dev), pool, table, [t], None)
+
+
+def test_sharp_and_equal_scores():
+    """Scores that grow along the context by hundreds, fall by hundreds, and are all equal."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(7)
+    t, hd = 300, 64
+    for slope in (1.0, -1.0, 0.0):
+        pool, table = _context([t], 1, hd, 16, g, dev)
+        ramp = slope * torch.arange(t, device=dev).float()[:, None, None]
+        k = ramp.expand(t, 1, hd).contiguous()
+        v = torch.randn(t, 1, hd, generator=g, device=dev)
+        pos = torch.arange(t, device=dev)
+        P.store(pool, hd, table[0][pos // 16].long() * 16 + pos % 16, k, v)
+        q = torch.ones(1, 2, hd, device=dev)
+        q[0, 1] = 0.0                                   # a query of zeros: the mean of V
+        _check_attention(q, pool, table, [t], None)
+
+
+def test_non_finite_rows_stay_where_they_are_seen():
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(8)
+    hd, lens = 64, [40, 40, 40, 40]
+    pool, table = _context(lens, 2, hd, 16, g, dev)
+    k = torch.randn(3, 2, hd, generator=g, device=dev)
+    v = torch.randn(3, 2, hd, generator=g, device=dev)
+    k[0, 0, 3] = math.nan                               # request 0, kv head 0: K
+    v[1, 1, 5] = math.inf                               # request 1, kv head 1: V
+    k[2], v[2] = math.nan, math.nan                     # request 2, past its length
+    slot = lambda b, p: int(table[b, p // 16]) * 16 + p % 16  # noqa: E731
+    qd.kv4_append(k, v, pool, _i64([slot(0, 7), slot(1, 39), slot(2, 39)], dev))
+    q = torch.randn(4, 4, hd, generator=g, device=dev)
+    q[3, 1, 0] = math.inf
+    lens = [40, 40, 39, 40]
+    got = _check_attention(q[:3], pool, table[:3], lens[:3], None)
+    nan = torch.isnan(got).all(-1)
+    assert nan.tolist() == [[True, True, False, False], [False, False, True, True], [False] * 4]
+    got = qd.kv4_attention(q, pool, table, _i64(lens, dev))
+    assert torch.isnan(got[3, 1]).all() and torch.isfinite(got[3, [0, 2, 3]]).all()
+
+
+@pytest.mark.parametrize("layout", ["slices", "odd", "heads"])
+def test_strided_queries_and_outputs(layout):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(9)
+    lens = [70, 9, 0]
+    pool, table = _context(lens, 2, 128, 32, g, dev)
+    q, out = _rows(3, 4, 128, torch.float32, g, dev, layout)
+    out.fill_(0.25)
+    got = _check_attention(q, pool, table, lens, None, out=out)
+    # in place
+    want = got.clone()
+    again = qd.kv4_attention(q, pool, table, _i64(lens, dev), out=q)
+    assert again is q and torch.equal(q, want)
+    # one query row for all requests (stride 0)
+    one = torch.randn(1, 4, 128, generator=g, device=dev)
+    _check_attention(one.expand(3, 4, 128), pool, table, lens, None)
+
+
+def test_same_bits_every_time():
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(10)
+    lens = [3000, 1, 900, 64] * 8
+    pool, table = _context(lens, 2, 128, 16, g, dev)
+    q = torch.randn(len(lens), 8, 128, generator=g, device=dev)
+    first = qd.kv4_attention(q, pool, table, _i64(lens, dev))
+    for _ in range(5):
+        assert torch.equal(first, qd.kv4_attention(q, pool, table, _i64(lens, dev)))
+
+
+def test_other_streams_and_graphs_side_by_side():
+    """Two captured graphs and an eager stream run the same context at once; each
+    has its own workspace."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(11)
+    lens = [4000, 77, 2500]
+    pool, table = _context(lens, 2, 64, 16, g, dev)
+    tl = _i64(lens, dev)
+    qs = [torch.randn(3, 8, 64, generator=g, device=dev) for _ in range(3)]
+    want = [qd.kv4_attention(q, pool, table, tl) for q in qs]
+    outs = [torch.zeros_like(q) for q in qs]
+    side = torch.cuda.Stream()
+    graphs = []
+    for q, o in zip(qs[:2], outs[:2]):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            for _ in range(4):
+                qd.kv4_attention(q, pool, table, tl, out=o)
+        graphs.append(gr)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(10):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        with torch.cuda.stream(streams[2]):
+            qd.kv4_attention(qs[2], pool, table, tl, out=outs[2])
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
+def test_plan_append_attend_together():
+    """A batch of uneven requests grown step by step from a captured graph: plan
+    (in place), append, attend; compared with fp64 attention over all rows."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(12)
+    nq, nkv, hd, page, B, W = 6, 2, 64, 16, 5, 8
+    pages = 40
+    pool = qd.kv4_pool(pages, nkv, hd, page, dev)
+    table = torch.full((B, W), -1, dtype=torch.int32, device=dev)
+    free = torch.randperm(pages, generator=g, device=dev).to(torch.int32)
+    used, lens = _i64([0], dev), _i64([0] * B, dev)
+    rows_new = [20, 1, 0, 33, 16]
+    joins = _i64(rows_new, dev)
+    # prompts
+    n = sum(rows_new) + 2
+    q = torch.randn(n, nq, hd, generator=g, device=dev)
+    k, v = (torch.randn(n, nkv, hd, generator=g, device=dev) for _ in range(2))
+    p = qd.kv4_plan(lens, joins, table, free, used, page, n, lens_out=lens, used_out=used)
+    qd.kv4_append(k, v, pool, p.slots)
+    _check_attention(q, pool, table, rows_new, p.cu_rows.tolist(), max_rows=33)
+    # steps of one row each, from a graph
+    joins = _i64([1] * B, dev)
+    q, k, v = (torch.empty(B, h, hd, device=dev) for h in (nq, nkv, nkv))
+    out = torch.zeros_like(q)
+
+    def step():
+        p = qd.kv4_plan(lens, joins, table, free, used, page, B, lens_out=lens, used_out=used)
+        qd.kv4_append(k, v, pool, p.slots)
+        qd.kv4_attention(q, pool, table, lens, cu_rows=p.cu_rows, out=out)
+
+    keep = [x.clone() for x in (lens, used, table, pool)]
+    step()
+    for x, y in zip((lens, used, table, pool), keep):
+        x.copy_(y)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        step()
+    held = list(rows_new)
+    for _ in range(20):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g, device=dev))
+        gr.replay()
+        held = [h + 1 for h in held]
+        assert lens.tolist() == held
+        ref, size = P.attention(q, pool, table, held, list(range(B + 1)), hd ** -0.5, out)
+        assert (out.double() - ref).abs().max() < 1e-4
+    assert used.item() == sum(-(-h // page) for h in held)
