@@ -456,6 +456,7 @@ struct AttnArgs {
 };
 
 // CTAs per SM that the register file holds without spills.
+constexpr int kAttnMaxPerSm = 4;
 __host__ __device__ constexpr int attn_per_sm(int hd, int nb) {
   return nb == 1 ? (hd == 64 ? 4 : 3) : (hd == 64 ? 3 : 2);
 }

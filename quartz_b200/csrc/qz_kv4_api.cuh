@@ -3,6 +3,7 @@
 #pragma once
 
 #include "qz_kv4.cuh"
+#include "qz_kv4_tc.cuh"
 
 namespace {
 
@@ -87,7 +88,9 @@ struct Kv4AttnLayout {
 Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int nb, int hd) {
   Kv4AttnLayout l;
   l.grid = d.sms * qz::kv4::attn_per_sm(hd, nb);
-  l.part_off = qz::cdiv(int64_t(l.grid) * 4, 256) * 256;
+  // the tickets' place is the same for every variant, so that one workspace
+  // serves calls of different shapes in turn
+  l.part_off = qz::cdiv(int64_t(d.sms) * qz::kv4::kAttnMaxPerSm * 4, 256) * 256;
   l.total = l.part_off + int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4;
   return l;
 }
@@ -103,6 +106,21 @@ int launch_kv4_attn_t(int hd, int nb, const qz::kv4::AttnArgs& a, int grid, cuda
   if (hd == 64)
     return nb == 1 ? launch_kv4_attn<T, 64, 1>(a, grid, st) : launch_kv4_attn<T, 64, 2>(a, grid, st);
   return nb == 1 ? launch_kv4_attn<T, 128, 1>(a, grid, st) : launch_kv4_attn<T, 128, 2>(a, grid, st);
+}
+
+// Requests with more rows than this (and heads that fit a tile) take the
+// tensor-core kernel's 128-row tiles, the others the split kernel.
+constexpr int kTcMinQueries = 32;
+int64_t split_rows(int group) {
+  return group > qz::kv4::kTcRows ? 0x7FFFFFFF : std::max(1, kTcMinQueries / group);
+}
+
+template <class T, int HD>
+int launch_kv4_tc(const qz::kv4::TcArgs& a, int64_t grid, cudaStream_t st) {
+  constexpr int smem = qz::kv4::tc_smem<HD>();
+  QZ_CUDA(allow_smem(qz::kv4::attn_tc_kernel<T, HD>, smem));
+  return launch_kv4(qz::kv4::attn_tc_kernel<T, HD>, static_cast<int>(grid), qz::kv4::kTcThreads,
+                    smem, st, a);
 }
 
 }  // namespace
@@ -240,9 +258,30 @@ int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_h
   a.shift = page_shift(page_size);
   a.scale = scale * 1.44269504088896341f;
   a.vec = rows_aligned(q, q_row_stride, q_head_stride, dtype);
-  a.rows_lo = 0;
-  a.rows_hi = static_cast<int>(std::min<int64_t>(max_rows, 0x7FFFFFFF));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t few = split_rows(group);
+  if (max_rows > few) {
+    qz::kv4::TcArgs t{a, 0};
+    t.out_vec = rows_aligned(out, out_row_stride, out_head_stride, dtype);
+    t.a.rows_lo = static_cast<int>(few);
+    t.a.rows_hi = static_cast<int>(std::min<int64_t>(max_rows, 0x7FFFFFFF));
+    const int64_t per = qz::kv4::kTcRows / group;
+    const int64_t grid = (n / per + std::min<int64_t>(B, n / (few + 1))) * nkv;
+    if (grid > 0x7FFFFFFFll) return fail(QZ_ERR_INVALID, "qz_kv4_attention: too many rows");
+    if (grid > 0) {
+      int rc;
+      if (dtype == qz::kv4::kF32)
+        rc = hd == 64 ? launch_kv4_tc<float, 64>(t, grid, st) : launch_kv4_tc<float, 128>(t, grid, st);
+      else if (dtype == qz::kv4::kBF16)
+        rc = hd == 64 ? launch_kv4_tc<__nv_bfloat16, 64>(t, grid, st)
+                      : launch_kv4_tc<__nv_bfloat16, 128>(t, grid, st);
+      else
+        rc = hd == 64 ? launch_kv4_tc<__half, 64>(t, grid, st) : launch_kv4_tc<__half, 128>(t, grid, st);
+      if (rc) return rc;
+    }
+  }
+  a.rows_lo = 0;
+  a.rows_hi = static_cast<int>(std::min<int64_t>(max_rows, few));
   switch (dtype) {
     case qz::kv4::kF32: return launch_kv4_attn_t<float>(hd, nb, a, L.grid, st);
     case qz::kv4::kBF16: return launch_kv4_attn_t<__nv_bfloat16>(hd, nb, a, L.grid, st);

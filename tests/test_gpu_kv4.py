@@ -7,7 +7,11 @@ fp32 with truncation (2^-23 each) over unsigned codes, whose sums are at most
 about four times sum |q k|; so a score is off by at most
 4 A (hd / 16 + 8) 2^-23 with A = scale * sum |q k|, a weight by that relatively
 plus 2^-21 of exponent and split, and a result by twice it times max |v| (the
-normalisation has the same error), plus the rounding to the output's type.
+normalisation has the same error), plus the rounding to the output's type. For
+many rows of a 16-bit type the weights are single fp16 values: each is off by at
+most 2^-11 of itself, and multiplies a value of at most 16 steps of its row, so
+the result by at most 2^-11 * 16 s <= 2^-11 * 2.2 max |v| (16 / 15 of the row's
+range, which is at most 2 max |v|) more.
 """
 
 import math
@@ -269,6 +273,8 @@ def _check_attention(q, pool, table, lens, cu, scale=None, max_rows=1, out=None,
     assert torch.equal(torch.isnan(ref), torch.isnan(got.double()))
     vmax = torch.nan_to_num(torch.stack(P.load(pool, hd))[1], nan=0.0).abs().max().item() or 1.0
     bound = vmax * (2 * 4 * size * (hd / 16 + 8) * 2.0 ** -23 + 2.0 ** -19)
+    if q.dtype != torch.float32 and max_rows > 1:
+        bound = bound + vmax * 2.2 * 2.0 ** -11
     bound = bound[..., None] + ref.abs() * torch.finfo(q.dtype).eps / 2
     err = torch.nan_to_num((got.double() - ref).abs(), nan=0.0)
     worst = (err - torch.nan_to_num(bound, nan=math.inf)).max().item()
@@ -321,6 +327,112 @@ def test_rows(dtype, nq, nkv, hd, rows, lens):
     cu = [sum(rows[:i]) for i in range(len(rows) + 1)]
     q = torch.randn(cu[-1] + 3, nq, hd, generator=g, device=dev).to(DTYPES[dtype])
     _check_attention(q, pool, table, lens, cu, max_rows=max(1, max(rows)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,nkv,page", [(2, 2, 16), (4, 2, 256), (3, 1, 32), (5, 1, 16), (8, 1, 64),
+                                         (16, 1, 16), (48, 1, 16), (130, 1, 16)])
+@pytest.mark.parametrize("rows,lens", [
+    ([129], [129]), ([40, 0, 65, 1], [40, 7, 400, 300]), ([200, 34], [150, 1200])])
+def test_prompts(dtype, hd, nq, nkv, page, rows, lens):
+    """Whole prompts, chunks on top of a context, more rows than positions, decoding
+    and idle requests among them; groups that do not divide a tile."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(sum(rows) + nq)
+    pool, table = _context(lens, nkv, hd, page, g, dev)
+    cu = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    q = torch.randn(cu[-1] + 3, nq, hd, generator=g, device=dev).to(DTYPES[dtype])
+    _check_attention(q, pool, table, lens, cu, max_rows=max(rows))
+    qd.check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_edges(hd):
+    """Bad pages, a table that ends early, NaN and infinite rows, steps of very
+    different size, sharp scores, strided rows, in a prompt."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(21)
+    rows, t = 100, 300
+    cu = [0, rows]
+
+    def fresh(**kw):
+        pool, table = _context([t], 2, hd, 16, g, dev, **kw)
+        return pool, table, torch.randn(rows, 4, hd, generator=g, device=dev)
+
+    pool, table, q = fresh()
+    table[0, 3], table[0, 9], table[0, 18] = -1, pool.shape[0], 1 << 30
+    _check_attention(q, pool, table, [t], cu, max_rows=rows)
+    table[:] = -7
+    assert (_check_attention(q, pool, table, [t], cu, max_rows=rows) == 0).all()
+    pool, table, q = fresh(width=10)
+    _check_attention(q, pool, table, [t], cu, max_rows=rows)
+    # a NaN key at 250 and an infinite value at 290 of kv head 1
+    pool, table, q = fresh()
+    k, v = torch.randn(2, 2, 2, hd, generator=g, device=dev)
+    k[0, 1, 0], v[1, 1, 0] = math.nan, math.inf
+    slots = _i64([int(table[0, p // 16]) * 16 + p % 16 for p in (250, 290)], dev)
+    qd.kv4_append(k, v, pool, slots)
+    got = _check_attention(q, pool, table, [t], cu, max_rows=rows)
+    assert torch.isnan(got).any(-1).sum() == 2 * 50
+    # one query row with an infinity spoils itself only
+    pool, table, q = fresh()
+    q[37, 2, 5] = math.inf
+    got = qd.kv4_attention(q, pool, table, _i64([t], dev), cu_rows=_i64(cu, dev), max_rows=rows)
+    assert torch.isnan(got).any(-1).nonzero().tolist() == [[37, 2]]
+    # steps from 1e-25 to 1e25 (rising, falling), scores that rise or fall by hundreds
+    pos = torch.arange(t, device=dev)
+    for flip in (False, True):
+        pool, table, q = fresh()
+        ex = torch.linspace(-25, 25, t, device=dev)
+        ex = ex.flip(0) if flip else ex
+        k = torch.randn(t, 2, hd, generator=g, device=dev)
+        v = torch.randn(t, 2, hd, generator=g, device=dev) * torch.pow(10.0, ex)[:, None, None]
+        P.store(pool, hd, table[0][pos // 16].long() * 16 + pos % 16, k, v)
+        _check_attention(q, pool, table, [t], cu, max_rows=rows)
+        ramp = (-1.0 if flip else 1.0) * pos.float()[:, None, None]
+        v = torch.randn(t, 2, hd, generator=g, device=dev)
+        P.store(pool, hd, table[0][pos // 16].long() * 16 + pos % 16, ramp.expand(t, 2, hd), v)
+        q = torch.ones(rows, 4, hd, device=dev)
+        q[:, 1] = 0.0
+        _check_attention(q, pool, table, [t], cu, max_rows=rows)
+    for layout in ("slices", "odd", "heads"):
+        pool, table, _ = fresh()
+        q, out = _rows(rows, 4, hd, torch.float32, g, dev, layout)
+        out.fill_(0.25)
+        got = _check_attention(q, pool, table, [t], cu, max_rows=rows, out=out)
+        want = got.clone()
+        assert torch.equal(qd.kv4_attention(q, pool, table, _i64([t], dev), cu_rows=_i64(cu, dev),
+                                            max_rows=rows, out=q), want)
+    qd.check_status()
+
+
+def test_long_prompt_same_bits_and_graph():
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(22)
+    lens, rows = [900, 1500, 40], [900, 300, 1]
+    pool, table = _context(lens, 2, 128, 32, g, dev)
+    cu = _i64([0, 900, 1200, 1201], dev)
+    q = torch.randn(1201, 8, 128, generator=g, device=dev)
+    tl = _i64(lens, dev)
+    first = qd.kv4_attention(q, pool, table, tl, cu_rows=cu, max_rows=900)
+    out = torch.zeros_like(q)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        qd.kv4_attention(q, pool, table, tl, cu_rows=cu, max_rows=900, out=out)
+    for _ in range(3):
+        out.zero_()
+        gr.replay()
+        assert torch.equal(out, first)
+    # each request alone, and each row as a decode step, agree within rounding
+    for b, (r0, n) in enumerate(((0, 900), (900, 300), (1200, 1))):
+        alone = qd.kv4_attention(q[r0:r0 + n], pool, table[b:b + 1], tl[b:b + 1],
+                                 cu_rows=_i64([0, n], dev), max_rows=n)
+        assert torch.equal(alone, first[r0:r0 + n])
+        for i in (0, n // 2, n - 1):
+            one = qd.kv4_attention(q[r0 + i:r0 + i + 1], pool, table[b:b + 1], tl[b:b + 1] - n + i + 1)
+            assert (one - first[r0 + i]).abs().max() < 2e-5
+    qd.check_status()
 
 
 def test_rows_beyond_max_rows_are_left():
@@ -521,3 +633,22 @@ def test_plan_append_attend_together():
         ref, size = P.attention(q, pool, table, held, list(range(B + 1)), hd ** -0.5, out)
         assert (out.double() - ref).abs().max() < 1e-4
     assert used.item() == sum(-(-h // page) for h in held)
+
+
+def test_one_workspace_for_calls_of_different_shapes():
+    """A workspace large enough for all serves any of them in turn: what one
+    variant leaves in it does not reach the next."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(23)
+    shapes = [(2, 1, 64, 1), (16, 2, 128, 1), (8, 1, 64, 4), (8, 1, 128, 4), (4, 1, 128, 1)]
+    big = max(qd.kv4_attention_workspace(dev, nq, nkv, hd, rows).numel() for nq, nkv, hd, rows in shapes)
+    ws = torch.zeros(big, dtype=torch.uint8, device=dev)
+    made = []
+    for nq, nkv, hd, rows in shapes:
+        lens = [1500, 300, 77]
+        pool, table = _context(lens, nkv, hd, 16, g, dev)
+        cu = [0, rows, 2 * rows, 3 * rows]
+        made.append((torch.randn(3 * rows, nq, hd, generator=g, device=dev), pool, table, lens, cu, rows))
+    for _ in range(3):
+        for q, pool, table, lens, cu, rows in made:
+            _check_attention(q, pool, table, lens, cu, max_rows=rows, workspace=ws)
