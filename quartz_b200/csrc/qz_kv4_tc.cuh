@@ -16,15 +16,20 @@
 // producers store anything. W overwrites S in place (a thread's own columns).
 // TMEM columns: Q limbs 0..127, O 128..255, S/W double-buffered 256..511.
 //
-// 16 warps, one CTA per SM:
-//   0-7   softmax; thread = (row, half of the tile's columns), warps w and w + 4
-//         share rows and agree on a new maximum through one barrier reduction
-//   8-14  producers: bulk copies bring the packed pages of a tile to shared
-//         memory kTcRaw tiles ahead (issued by warp 8, one lane per page and
-//         part); all seven turn them into fp16 tiles in the swizzled layout the
-//         MMA reads, and (s, z) of each position into fp32
-//   15    one thread issues the MMAs: S(t + 1) before O(t), so that the next
-//         scores are ready when the softmax of this tile ends
+// 24 warps, one CTA per SM:
+//   0-15  softmax. A row of a tile has two threads, one for each 64 positions;
+//         groups of four warps take (even tiles, first half), (odd, first),
+//         (even, second), (odd, second), so each scheduler has four warps in
+//         different phases to hide latency behind. A row's maximum is agreed
+//         between its two threads and passed on from tile to tile through
+//         shared memory, before the weights are formed.
+//   16-19 converters: packed codes -> fp16 tiles in the swizzled layout the MMA
+//         reads
+//   20    parameters: (s, z) of each position -> fp32 arrays
+//   21    loader: one bulk copy per page brings a tile's packed blocks to shared
+//         memory, kTcRaw tiles ahead
+//   22    issues the MMAs: S(t + 1) before O(t), so that the next scores are
+//         ready when the softmax of this tile ends
 // K and V tiles of a position row hold their dimensions in nibble order
 // (0 4 1 5 2 6 3 7 of each word); Q is stored in the same order, and the
 // epilogue puts O's columns back.
@@ -36,11 +41,15 @@
 namespace qz {
 namespace kv4 {
 
-constexpr int kTcThreads = 16 * 32;
-constexpr int kTcProducers = 7 * 32;
+constexpr int kTcThreads = 24 * 32;
+constexpr int kTcSoftmax = 16 * 32;
+constexpr int kTcConverters = 4 * 32;
 constexpr int kTcRows = 128;    // (row, head) pairs per item
 constexpr int kTcKeys = 128;    // positions per tile
-constexpr int kTcRing = 4;      // parameter stages
+// Parameter stages. Tile j's are written once its packed tile has landed, so
+// after tile j - kTcRaw was converted, so after O(j - kTcRaw - 2) was issued:
+// the softmax is at most kTcRaw + 1 tiles behind.
+constexpr int kTcRing = 8;
 constexpr int kTcRaw = 3;       // stages of packed tiles
 constexpr uint32_t kColQ = 0, kColO = 128, kColS = 256;
 
@@ -61,15 +70,17 @@ __host__ __device__ constexpr int tc_raw_bytes() { return kTcKeys * (HD + 8); }
 struct TcShared {
   float sk[kTcRing][kTcKeys], zk[kTcRing][kTcKeys];   // K's step and zero
   float sv[kTcRing][kTcKeys], zc[kTcRing][kTcKeys];   // V's step * 2^(9 - ev), zero + 8 step
-  uint32_t valid[kTcRing][4];   // positions that exist, one bit each
+  alignas(16) uint32_t valid[kTcRing][4];   // positions that exist, one bit each
   float down[kTcRing];          // 2^(ev before - ev): O's factor when V's exponent grows
   float w_down[kTcRing];        // 2^(ev - 9)
-  float xa[2][kTcRows], xb[2][kTcRows];   // exchange between the two halves of a row
-  float dmax[2][4];
+  float top[2][2][kTcRows];     // [tile & 1][half]: maximum of a row's half tile
+  float max[2][kTcRows];        // [tile & 1]: a row's maximum so far
+  float ex[3][4][kTcRows];      // exchange between a row's four threads
+  uint32_t odd[kTcRing];        // a V parameter of the tile is not finite
   int64_t scan[128];
-  int64_t item[2];              // request, tile within it
+  int item[6];                  // request, first row, rows, first row of q, len - rows, positions seen
   uint64_t k_full[2], v_full[2], s_full[2], p_full[2], v_empty[2], par_full[kTcRing], q_ready, drain;
-  uint64_t raw_full[kTcRaw], raw_empty[kTcRaw];
+  uint64_t raw_full[kTcRaw], raw_empty[kTcRaw], t_full[2][4], m_full[2][4];
   uint32_t raw_groups[kTcRaw];  // which 16-position groups of a packed tile exist
   uint32_t tmem;
 };
@@ -186,54 +197,202 @@ __device__ __forceinline__ uint4 v_pairs(uint32_t w) {
   return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
+// Registers per thread of a warpgroup (all four warps call it). The shares of
+// the six warpgroups, 4 * 88 + 72 + 56, are the launch's 6 * 80.
+template <int N>
+__device__ __forceinline__ void regs_more() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_less() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0u;
+}
+
+// mbar_wait by a whole warp: true if every lane saw the phase complete.
+__device__ __forceinline__ bool warp_wait(const uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity));
+}
+
+// What a thread has summed of its row, relative to 2^m.
+struct RowState {
+  float m;         // maximum
+  f2_t l, zs;      // sum of p, sum of p (z_v + 8 s_v)
+};
+
+// x = score + mu of 64 positions, in TMEM in place of S; returns their maximum. MASK: positions that do not exist (bits of
+// `valid`) or lie at `lim` or behind it, counted from the first, become -inf.
+template <bool MASK>
+__device__ __forceinline__ float tc_scores(uint32_t taddr, const float* sk, const float* zk, f2_t F2,
+                                           f2_t Q2, f2_t mu2, const uint32_t* valid, int lim) {
+  float t0 = -INFINITY, t1 = -INFINITY;
+  uint32_t v[2][16];
+  tc::tmem_ld16(taddr, v[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tc::tmem_wait_ld();
+    if (c < 3) tc::tmem_ld16(taddr + 16 * (c + 1), v[(c + 1) & 1]);
+    uint32_t(&u)[16] = v[c & 1];
+    const uint32_t bits = MASK ? valid[c >> 1] >> (16 * (c & 1)) : 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 s = reinterpret_cast<const float4*>(sk)[4 * c + k];
+      const float4 z = reinterpret_cast<const float4*>(zk)[4 * c + k];
+      float2 a = f2_unpack(f2_fma(f2_mul(f2_pack(u[4 * k], u[4 * k + 1]), F2), f2_set(s.x, s.y),
+                                  f2_fma(f2_set(z.x, z.y), Q2, mu2)));
+      float2 b = f2_unpack(f2_fma(f2_mul(f2_pack(u[4 * k + 2], u[4 * k + 3]), F2), f2_set(s.z, s.w),
+                                  f2_fma(f2_set(z.z, z.w), Q2, mu2)));
+      if constexpr (MASK) {
+        const int left = lim - 16 * c - 4 * k;
+        const uint32_t four = bits >> (4 * k);
+        a.x = (four & 1u) && left > 0 ? a.x : -INFINITY;
+        a.y = (four & 2u) && left > 1 ? a.y : -INFINITY;
+        b.x = (four & 4u) && left > 2 ? b.x : -INFINITY;
+        b.y = (four & 8u) && left > 3 ? b.y : -INFINITY;
+      }
+      t0 = fmaxf(t0, fmaxf(a.x, a.y));
+      t1 = fmaxf(t1, fmaxf(b.x, b.y));
+      u[4 * k] = __float_as_uint(a.x);
+      u[4 * k + 1] = __float_as_uint(a.y);
+      u[4 * k + 2] = __float_as_uint(b.x);
+      u[4 * k + 3] = __float_as_uint(b.y);
+    }
+    tmem_st8(taddr + 16 * c, u);
+    tmem_st8(taddr + 16 * c + 8, u + 8);
+  }
+  tmem_wait_st();
+  return fmaxf(t0, t1);
+}
+
+// n columns of this row times f plus d.
+template <int n>
+__device__ __forceinline__ void tc_rescale(uint32_t taddr, float f, float d) {
+#pragma unroll 1
+  for (int c = 0; c < n; c += 16) {
+    uint32_t o[16];
+    tc::tmem_ld16(taddr + c, o);
+    tc::tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(o[k]), f, d));
+    tmem_st8(taddr + c, o);
+    tmem_st8(taddr + c + 8, o + 8);
+  }
+  tmem_wait_st();
+}
+
+// Weights of 64 positions into TMEM, in place of x (limbs of 16 positions side by
+// side). SELECT: parameters of hidden positions may be NaN, so they are selected
+// away; otherwise p = 0 makes their products vanish.
+template <int L, bool SELECT>
+__device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, const float* zc,
+                                           RowState& st) {
+  uint32_t v[2][16];
+  tc::tmem_ld16(taddr, v[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tc::tmem_wait_ld();
+    if (c < 3) tc::tmem_ld16(taddr + 16 * (c + 1), v[(c + 1) & 1]);
+    const uint32_t(&x)[16] = v[c & 1];
+    uint32_t w[8 * L];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float4 s = reinterpret_cast<const float4*>(sv)[4 * c + q];
+      float4 z = reinterpret_cast<const float4*>(zc)[4 * c + q];
+      if constexpr (SELECT) {
+        constexpr uint32_t kHidden = 0xFF800000u;   // -inf
+        if (x[4 * q] == kHidden) s.x = z.x = 0.f;
+        if (x[4 * q + 1] == kHidden) s.y = z.y = 0.f;
+        if (x[4 * q + 2] == kHidden) s.z = z.z = 0.f;
+        if (x[4 * q + 3] == kHidden) s.w = z.w = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f2_t p = f2_set(ex2(__uint_as_float(x[4 * q + 2 * e])),
+                              ex2(__uint_as_float(x[4 * q + 2 * e + 1])));
+        st.l = f2_add(st.l, p);
+        st.zs = f2_fma(p, e ? f2_set(z.z, z.w) : f2_set(z.x, z.y), st.zs);
+        const f2_t y2 = f2_mul(p, e ? f2_set(s.z, s.w) : f2_set(s.x, s.y));
+        const float2 y = f2_unpack(y2);
+        const __half2 hi = __floats2half2_rn(y.x, y.y);
+        w[2 * q + e] = *reinterpret_cast<const uint32_t*>(&hi);
+        if constexpr (L == 2) {
+          const float2 back = __half22float2(hi);
+          const float2 d = f2_unpack(f2_sub(y2, f2_set(back.x, back.y)));
+          const __half2 lo = __floats2half2_rn(d.x, d.y);
+          w[8 + 2 * q + e] = *reinterpret_cast<const uint32_t*>(&lo);
+        }
+      }
+    }
+#pragma unroll
+    for (int l = 0; l < L; ++l) tmem_st8(taddr + c * (8 * L) + 8 * l, w + 8 * l);
+  }
+}
+
 template <class T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs args) {
   constexpr int L = sizeof(T) == 4 ? 2 : 1;      // fp16 limbs of q and of the weights
   constexpr int TB = tc_tile_bytes<HD>();
+  constexpr int RB = tc_raw_bytes<HD>();
   constexpr int BLK = kTcKeys * 128;             // bytes of 64 dimensions of a tile
   constexpr float kNegInf = -INFINITY;
   const AttnArgs& a = args.a;
   extern __shared__ __align__(128) uint8_t tc_raw[];
-  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) &
-                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* raws = tiles + 4 * TB;
-  TcShared& sh = *reinterpret_cast<TcShared*>(raws + kTcRaw * tc_raw_bytes<HD>());
+  // pointer arithmetic, not integer rounding, keeps these shared-memory accesses
+  uint8_t* tiles = tc_raw + ((1024u - (smem_u32(tc_raw) & 1023u)) & 1023u);
+  uint8_t* raws = tiles + 4 * TB;                // K stages, V stages, packed stages
+  TcShared& sh = *reinterpret_cast<TcShared*>(raws + kTcRaw * RB);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_wait();
   // ---- which item: tiles of `per` query rows of every handled request ---------
   const int per = kTcRows / a.group;
+  const int cap = static_cast<int>(a.width << a.shift);
+  const int chunk = (a.B + 127) / 128;
+  auto tiles_of = [&](int64_t b) -> int {        // n <= 2^30 rows
+    int64_t r0;
+    return (static_cast<int>(rows_of(a, b, &r0)) + per - 1) / per;
+  };
   if (tid < 128) {
-    const int chunk = (a.B + 127) / 128;
     int64_t mine = 0;
     for (int k = 0; k < chunk; ++k) {
       const int64_t b = static_cast<int64_t>(tid) * chunk + k;
-      int64_t r0;
-      if (b < a.B) mine += (rows_of(a, b, &r0) + per - 1) / per;
+      if (b < a.B) mine += tiles_of(b);
     }
     sh.scan[tid] = mine;
   }
   if (tid == 0) {
     sh.item[0] = -1;
     for (int s = 0; s < 2; ++s) {
-      mbar_init(smem_u32(&sh.k_full[s]), kTcProducers);
-      mbar_init(smem_u32(&sh.v_full[s]), kTcProducers);
+      mbar_init(smem_u32(&sh.k_full[s]), kTcConverters);
+      mbar_init(smem_u32(&sh.v_full[s]), kTcConverters);
       mbar_init(smem_u32(&sh.s_full[s]), 1);
       mbar_init(smem_u32(&sh.p_full[s]), 256);
+      for (int w = 0; w < 4; ++w) {
+        mbar_init(smem_u32(&sh.t_full[s][w]), 2);
+        mbar_init(smem_u32(&sh.m_full[s][w]), 1);
+      }
       mbar_init(smem_u32(&sh.v_empty[s]), 1);
     }
-    for (int s = 0; s < kTcRing; ++s) mbar_init(smem_u32(&sh.par_full[s]), kTcProducers);
+    for (int s = 0; s < kTcRing; ++s) mbar_init(smem_u32(&sh.par_full[s]), 32);
     for (int s = 0; s < kTcRaw; ++s) {
       mbar_init(smem_u32(&sh.raw_full[s]), 1);
-      mbar_init(smem_u32(&sh.raw_empty[s]), kTcProducers);
+      mbar_init(smem_u32(&sh.raw_empty[s]), kTcConverters + 32);
     }
-    mbar_init(smem_u32(&sh.q_ready), 256);
+    mbar_init(smem_u32(&sh.q_ready), kTcSoftmax);
     mbar_init(smem_u32(&sh.drain), 1);
     fence_mbar_init();
   }
   __syncthreads();
   if (tid < 128) {
-    const int chunk = (a.B + 127) / 128;
     int64_t before = 0, total = 0;
     for (int k = 0; k * chunk < a.B; ++k) {
       const int64_t v = sh.scan[k];
@@ -243,20 +402,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     // a request's later tiles see more: they start first
     const int64_t t = total - 1 - blockIdx.x / a.nkv;
     if (t >= 0 && t >= before && t < before + sh.scan[tid]) {
-      int64_t b = static_cast<int64_t>(tid) * chunk, at = before, r0;
-      for (int64_t n = (rows_of(a, b, &r0) + per - 1) / per; t >= at + n;
-           n = (rows_of(a, b, &r0) + per - 1) / per) {
+      int64_t b = static_cast<int64_t>(tid) * chunk, at = before;
+      for (int n = tiles_of(b); t >= at + n; n = tiles_of(b)) {
         at += n;
         ++b;
       }
-      sh.item[0] = b;
-      sh.item[1] = t - at;
+      int64_t r0;
+      const int64_t n = rows_of(a, b, &r0), row0 = (t - at) * per, lim = int64_t(1) << 30;
+      const int64_t off = a.lens[b] - n, last = (row0 + per < n ? row0 + per : n) + off;
+      sh.item[0] = static_cast<int>(b);
+      sh.item[1] = static_cast<int>(row0);
+      sh.item[2] = static_cast<int>(n);
+      sh.item[3] = static_cast<int>(r0);
+      // rows and positions are at most 2^30, so more than that changes no limit
+      sh.item[4] = static_cast<int>(off > lim ? lim : (off < -lim ? -lim : off));
+      sh.item[5] = static_cast<int>(last < 0 ? 0 : (last > cap ? cap : last));
     }
   }
   __syncthreads();
-  const int64_t b = sh.item[0];
-  if (b < 0) return;                       // the grid is an upper bound
-  if (warp == 15) {
+  if (sh.item[0] < 0) return;              // the grid is an upper bound
+  if (warp == 22) {
     tc::tmem_alloc(smem_u32(&sh.tmem), 512);
     tc::tmem_relinquish();
   }
@@ -264,285 +429,387 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = sh.tmem;
-
   const int h = blockIdx.x % a.nkv;
-  int64_t r0;
-  const int64_t n = rows_of(a, b, &r0);
-  const int64_t row0 = sh.item[1] * per;                       // first row of the item
-  const int64_t len = a.lens[b], cap = a.width << a.shift;
-  auto limit = [&](int64_t row) -> int {                       // positions [0, limit) are seen
-    const int64_t l = len - n + row + 1;
-    return static_cast<int>(l < 0 ? 0 : (l > cap ? cap : l));
-  };
-  const int seen = limit(row0 + per < n ? row0 + per - 1 : n - 1);
-  const int nt = (seen + kTcKeys - 1) / kTcKeys;
+  const int seen = sh.item[5], nt = (seen + kTcKeys - 1) / kTcKeys;
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ======================= softmax =======================================
-    const int r = tid & 127, half = tid >> 7, pair = 1 + (warp & 3);
-    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-    const int64_t row = row0 + r / a.group;
-    const int head = h * a.group + r % a.group;
+    regs_more<88>();
+    // row r of the item; quarter: which TMEM lanes; odd / half: which tiles and positions
+    const int r = tid & 127, quarter = warp & 3, odd = (warp >> 2) & 1, half = warp >> 3;
+    const int part = warp >> 2;               // this thread's share of the row's dimensions
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    // r / group for r < 128: the error of the rounded-up reciprocal, 128 / 65536,
+    // is below 1 / group
+    const uint32_t inv_group = (65535u + a.group) / a.group;
+    const int rg = static_cast<int>((r * inv_group) >> 16);
+    const int row0 = sh.item[1], n = sh.item[2];
+    const int64_t r0 = sh.item[3];
+    const int row = row0 + rg, head = h * a.group + (r - rg * a.group);
     const bool real = r < per * a.group && row < n;
-    const int lim = real ? limit(row) : 0;
+    const int sees = sh.item[4] + row + 1;          // positions [0, lim) are seen
+    const int lim = !real || sees < 0 ? 0 : (sees > cap ? cap : sees);
+    constexpr int DP = HD / 4;                      // dimensions per thread
 
-    // ---- q: this thread's half of the row, as fp16 limbs in TMEM --------------
+    // ---- q: this thread's share of the row, as fp16 limbs in TMEM --------------
     float F, Qs;
     {
-      float x[HD / 2];
-      if (real) {
-        const T* p = static_cast<const T*>(a.q) + (r0 + row) * a.q_rs + head * a.q_hs + half * (HD / 2);
-        load_row(p, a.vec, x);
+      float x[DP];
+      if (a.vec) {
+        // through the second K and V stages (the converters leave them alone
+        // until q_ready): whole rows per warp, 16-byte chunk c of row r at c ^ (r & 7)
+        constexpr int CH = HD * static_cast<int>(sizeof(T)) / 16;
+        auto at = [&](int rr, int c) -> uint4* {
+          return reinterpret_cast<uint4*>(tiles + (rr < 64 ? TB : 3 * TB) + (rr & 63) * (CH * 16) +
+                                          ((c ^ (rr & 7)) << 4));
+        };
+#pragma unroll
+        for (int i = 0; i < CH / 4; ++i) {
+          const int idx = i * kTcSoftmax + tid, rr = idx / CH, c = idx % CH;
+          const int g = static_cast<int>((rr * inv_group) >> 16);
+          uint4 u = make_uint4(0u, 0u, 0u, 0u);
+          if (rr < per * a.group && row0 + g < n)
+            u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (r0 + row0 + g) * a.q_rs +
+                                                     (h * a.group + (rr - g * a.group)) * a.q_hs) + c);
+          *at(rr, c) = u;
+        }
+        named_bar_sync(6, kTcSoftmax);
+        constexpr int pv = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < CH / 4; ++j) {
+          const uint4 u = *at(r, part * (CH / 4) + j);
+          const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+          for (int k = 0; k < pv; ++k) x[j * pv + k] = to_f(e[k]);
+        }
+      } else if (real) {
+        load_row(static_cast<const T*>(a.q) + (r0 + row) * a.q_rs + head * a.q_hs + part * DP, false,
+                 x);
       } else {
 #pragma unroll
-        for (int j = 0; j < HD / 2; ++j) x[j] = 0.f;
+        for (int j = 0; j < DP; ++j) x[j] = 0.f;
       }
-      float mx = 0.f, sum = 0.f;
+      float m4[4] = {0.f, 0.f, 0.f, 0.f}, s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < HD / 2; ++j) {
-        mx = fmaxf(mx, fabsf(x[j]));
-        sum += x[j];
+      for (int j = 0; j < DP; ++j) {
+        m4[j & 3] = fmaxf(m4[j & 3], fabsf(x[j]));
+        s4[j & 3] += x[j];
       }
-      sh.xa[half][r] = mx;
-      sh.xb[half][r] = sum;
-      named_bar_sync(pair, 64);
-      mx = fmaxf(mx, sh.xa[half ^ 1][r]);
-      sum = sh.xb[0][r] + sh.xb[1][r];
+      float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      sh.ex[0][part][r] = mx;
+      sh.ex[1][part][r] = sum;
+      named_bar_sync(1 + quarter, 128);
+      mx = fmaxf(fmaxf(sh.ex[0][0][r], sh.ex[0][1][r]), fmaxf(sh.ex[0][2][r], sh.ex[0][3][r]));
+      sum = (sh.ex[1][0][r] + sh.ex[1][1][r]) + (sh.ex[1][2][r] + sh.ex[1][3][r]);
       int e = static_cast<int>((__float_as_uint(mx) >> 23) & 255u) - 127;
       e = e < -113 ? -113 : (e > 117 ? 117 : e);
       const float up = pow2i(14 - e);
       F = pow2i(10 + e) * a.scale;
       Qs = sum * a.scale;
-      const __half r16 = __ushort_as_half(0x2C00);   // 1 / 16
+      // pairs (0 4) (1 5) (2 6) (3 7) of each eight; odd nibbles stand as 16 c
+      const f2_t up2 = f2_set(up, up), up16 = f2_set(up * 0.0625f, up * 0.0625f);
 #pragma unroll
-      for (int m = 0; m < HD / 16; m += 2) {
+      for (int m = 0; m < DP / 8; m += 2) {
         uint32_t w[L][8];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t s[8];                             // (hi, lo) of eight dimensions
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            s[j] = split_h2(x[8 * (m + k) + j] * up);
-            if (j & 1) {                             // odd nibbles stand as 16 c
-              const __half2 t = __hmul2(*reinterpret_cast<const __half2*>(&s[j]), __half2half2(r16));
-              s[j] = *reinterpret_cast<const uint32_t*>(&t);
-            }
-          }
-#pragma unroll
-          for (int l = 0; l < L; ++l) {
-            const uint32_t sel = l ? 0x7632u : 0x5410u;
-            w[l][4 * k] = prmt(s[0], s[4], sel);
-            w[l][4 * k + 1] = prmt(s[1], s[5], sel);
-            w[l][4 * k + 2] = prmt(s[2], s[6], sel);
-            w[l][4 * k + 3] = prmt(s[3], s[7], sel);
+        for (int k = 0; k < 8; ++k) {
+          const int at = 8 * (m + (k >> 2)) + (k & 3);
+          const f2_t y2 = f2_mul(f2_set(x[at], x[at + 4]), k & 1 ? up16 : up2);
+          const float2 y = f2_unpack(y2);
+          const __half2 hi = __floats2half2_rn(y.x, y.y);
+          w[0][k] = *reinterpret_cast<const uint32_t*>(&hi);
+          if constexpr (L == 2) {
+            const float2 back = __half22float2(hi);
+            const float2 d = f2_unpack(f2_sub(y2, f2_set(back.x, back.y)));
+            const __half2 lo = __floats2half2_rn(d.x, d.y);
+            w[L - 1][k] = *reinterpret_cast<const uint32_t*>(&lo);
           }
         }
 #pragma unroll
         for (int l = 0; l < L; ++l)
-          tmem_st8(lane_addr + kColQ + l * (HD / 2) + half * (HD / 4) + 4 * m, w[l]);
+          tmem_st8(lane_addr + kColQ + l * (HD / 2) + part * (DP / 2) + 4 * m, w[l]);
       }
       tmem_wait_st();
       tc::tc_fence_before();
       mbar_arrive(smem_u32(&sh.q_ready));
-      named_bar_sync(pair, 64);   // xa is used again below
     }
 
     const f2_t F2 = f2_set(F, F), Q2 = f2_set(Qs, Qs);
-    float m = kNegInf;
-    f2_t l2 = f2_set(0.f, 0.f), zs2 = f2_set(0.f, 0.f);
+    RowState st{kNegInf, f2_set(0.f, 0.f), f2_set(0.f, 0.f)};
     bool failed = false;
-    for (int j = 0; j < nt; ++j) {
-      const int ring = j & (kTcRing - 1), buf = j & 1;
-      const int p0 = j * kTcKeys + half * 64;           // this thread's first position
+#pragma unroll 1
+    for (int j = odd; j < nt; j += 2) {
+      const int ring = j & (kTcRing - 1), p0 = j * kTcKeys + half * 64;
       bool ok = mbar_wait(smem_u32(&sh.par_full[ring]), (j / kTcRing) & 1) &&
-                mbar_wait(smem_u32(&sh.s_full[buf]), (j >> 1) & 1);
-      ok = __all_sync(0xffffffffu, ok);
+                mbar_wait(smem_u32(&sh.s_full[odd]), (j >> 1) & 1);
+      // the row's maximum up to tile j - 1
+      if (j > 0) ok = ok && mbar_wait(smem_u32(&sh.m_full[odd ^ 1][quarter]), ((j - 1) >> 1) & 1);
+      failed = !__all_sync(0xffffffffu, ok);
+      if (failed) break;
       tc::tc_fence_after();
-      float top = kNegInf;
-      const uint32_t va = sh.valid[ring][half * 2], vb = sh.valid[ring][half * 2 + 1];
-      const bool whole = (va & vb) == 0xFFFFFFFFu && __all_sync(0xffffffffu, lim >= p0 + 64);
-      // scores (base 2) of 16 positions; they are formed twice, for the maximum
-      // and for the weights, which costs three instructions per two positions
-      // and saves holding 64 of them
-      const float4* sk4 = reinterpret_cast<const float4*>(&sh.sk[ring][half * 64]);
-      const float4* zk4 = reinterpret_cast<const float4*>(&sh.zk[ring][half * 64]);
-      auto scores = [&](int c, f2_t (&x)[8]) {
-        uint32_t v[16];
-        tc::tmem_ld16(lane_addr + kColS + buf * 128 + half * 64 + 16 * c, v);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float4 s = sk4[4 * c + k], z = zk4[4 * c + k];
-          x[2 * k] = f2_fma(f2_mul(f2_pack(v[4 * k], v[4 * k + 1]), F2), f2_set(s.x, s.y),
-                            f2_mul(f2_set(z.x, z.y), Q2));
-          x[2 * k + 1] = f2_fma(f2_mul(f2_pack(v[4 * k + 2], v[4 * k + 3]), F2),
-                                f2_set(s.z, s.w), f2_mul(f2_set(z.z, z.w), Q2));
-        }
-        if (!whole) {
-          const uint32_t bits = (c < 2 ? va : vb) >> (16 * (c & 1));
-          const int left = lim - p0 - 16 * c;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float2 t = f2_unpack(x[k]);
-            x[k] = f2_set((bits >> (2 * k)) & 1u && 2 * k < left ? t.x : kNegInf,
-                          (bits >> (2 * k)) & 2u && 2 * k + 1 < left ? t.y : kNegInf);
-          }
-        }
-      };
-      if (ok) {
-#pragma unroll 2
-        for (int c = 0; c < 4; ++c) {
-          f2_t x[8];
-          scores(c, x);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float2 t = f2_unpack(x[k]);
-            top = fmaxf(top, fmaxf(t.x, t.y));
-          }
-        }
+      const float before = j > 0 ? sh.max[odd ^ 1][r] : kNegInf;
+      const uint32_t cols = lane_addr + kColS + odd * 128 + half * 64;
+      const float mu = before == kNegInf ? 0.f : -before;
+      const uint2 vb = *reinterpret_cast<const uint2*>(&sh.valid[ring][2 * half]);
+      const bool whole = (vb.x & vb.y) == 0xFFFFFFFFu && __all_sync(0xffffffffu, lim >= p0 + 64);
+      const f2_t mu2 = f2_set(mu, mu);
+      const float* sk = sh.sk[ring] + half * 64;
+      const float* zk = sh.zk[ring] + half * 64;
+      float top = whole ? tc_scores<false>(cols, sk, zk, F2, Q2, mu2, nullptr, 0)
+                        : tc_scores<true>(cols, sk, zk, F2, Q2, mu2, &sh.valid[ring][2 * half], lim - p0);
+      // both halves' maximum; the four arrays it takes are free again once O(j) is issued
+      sh.top[odd][half][r] = top;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.t_full[odd][quarter]));
+      failed = !warp_wait(&sh.t_full[odd][quarter], (j >> 1) & 1);
+      if (failed) break;
+      top = fmaxf(top, sh.top[odd][half ^ 1][r]);
+      // a maximum that rose by more than 2^4 is renewed (x stands relative to -mu)
+      float now = before;
+      if (top > (before == kNegInf ? kNegInf : 4.f)) now = fmaxf(before, top - mu);
+      if (half == 0) {
+        sh.max[odd][r] = now;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.m_full[odd][quarter]));
       }
       const float down = sh.down[ring];
-      if (bar_any(pair, 64, !ok || top > m + 4.f || down != 1.f)) {
-        // a new maximum for the pair's rows (or a new exponent of V's steps)
-        sh.xa[half][r] = top;
-        if (bar_any(pair, 64, !ok)) {
-          failed = true;
-          break;
-        }
-        const float mn = fmaxf(m, fmaxf(top, sh.xa[half ^ 1][r]));
-        const float al = m == kNegInf ? 1.f : ex2(m - mn);
-        m = mn;
-        l2 = f2_mul(l2, f2_set(al, al));
-        zs2 = f2_mul(zs2, f2_set(al, al));
+      if (__any_sync(0xffffffffu, now != before || down != 1.f)) {
+        tc_rescale<64>(cols, 1.f, now == kNegInf ? 0.f : -mu - now);
         if (j > 0) {
-          bool done = mbar_wait(smem_u32(&sh.v_empty[(j - 1) & 1]), ((j - 1) >> 1) & 1);
-          done = __all_sync(0xffffffffu, done);
+          // O holds tiles 0 .. j - 1 relative to `before`, V's steps to the old exponent
+          const bool done = warp_wait(&sh.v_empty[odd ^ 1], ((j - 1) >> 1) & 1);
           if (!done && lane == 0) report_error(ERR_WAIT_FULL, 0x401u);
           tc::tc_fence_after();
-          const float f = al * down;
-#pragma unroll
-          for (int c = 0; c < HD / 2; c += 16) {
-            uint32_t o[16];
-            const uint32_t at = lane_addr + kColO + half * (HD / 2) + c;
-            tc::tmem_ld16(at, o);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st8(at, o);
-            tmem_st8(at + 8, o + 8);
-          }
-          tmem_wait_st();
+          tc_rescale<HD / 2>(lane_addr + kColO + half * (HD / 2),
+                             (before == kNegInf ? 1.f : ex2(before - now)) * down, 0.f);
         }
-        named_bar_sync(pair, 64);   // xa is free again
       }
-      // weights, over this thread's own columns of S
-      const float mu = m == kNegInf ? 0.f : -m;
-      const f2_t mu2 = f2_set(mu, mu);
-      const float4* sv4 = reinterpret_cast<const float4*>(&sh.sv[ring][half * 64]);
-      const float4* zc4 = reinterpret_cast<const float4*>(&sh.zc[ring][half * 64]);
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {       // 16 positions: one K step of the MMA
-        f2_t x[8];
-        scores(c, x);
-        uint32_t w[8 * L];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float4 s = sv4[4 * c + q], z = zc4[4 * c + q];
-          if (!whole) {
-            // selected, not multiplied, away: a hidden position may hold anything
-            const float2 a0 = f2_unpack(x[2 * q]), a1 = f2_unpack(x[2 * q + 1]);
-            if (a0.x == kNegInf) s.x = z.x = 0.f;
-            if (a0.y == kNegInf) s.y = z.y = 0.f;
-            if (a1.x == kNegInf) s.z = z.z = 0.f;
-            if (a1.y == kNegInf) s.w = z.w = 0.f;
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 t = f2_unpack(f2_add(x[2 * q + e], mu2));
-            const f2_t p = f2_set(ex2(t.x), ex2(t.y));
-            l2 = f2_add(l2, p);
-            zs2 = f2_fma(p, e ? f2_set(z.z, z.w) : f2_set(z.x, z.y), zs2);
-            const float2 y = f2_unpack(f2_mul(p, e ? f2_set(s.z, s.w) : f2_set(s.x, s.y)));
-            const __half2 hi = __floats2half2_rn(y.x, y.y);
-            w[2 * q + e] = *reinterpret_cast<const uint32_t*>(&hi);
-            if constexpr (L == 2) {
-              const float2 back = __half22float2(hi);
-              const __half2 lo = __floats2half2_rn(y.x - back.x, y.y - back.y);
-              w[8 + 2 * q + e] = *reinterpret_cast<const uint32_t*>(&lo);
-            }
-          }
-        }
-        const uint32_t at = lane_addr + kColS + buf * 128 + half * 64 + c * (8 * L);
-#pragma unroll
-        for (int l = 0; l < L; ++l) tmem_st8(at + 8 * l, w + 8 * l);
+      if (__any_sync(0xffffffffu, now != st.m)) {        // this thread's own sums
+        const float al = st.m == kNegInf ? 1.f : ex2(st.m - now);
+        st.m = now;
+        st.l = f2_mul(st.l, f2_set(al, al));
+        st.zs = f2_mul(st.zs, f2_set(al, al));
       }
+      // weights, over this thread's columns of S
+      const float* sv = sh.sv[ring] + half * 64;
+      const float* zc = sh.zc[ring] + half * 64;
+      if (sh.odd[ring])
+        tc_weights<L, true>(cols, sv, zc, st);
+      else
+        tc_weights<L, false>(cols, sv, zc, st);
       tmem_wait_st();
       tc::tc_fence_before();
-      mbar_arrive(smem_u32(&sh.p_full[buf]));
+      mbar_arrive(smem_u32(&sh.p_full[odd]));
     }
     if (failed && lane == 0) report_error(ERR_WAIT_FULL, 0x400u);
-    // ---- epilogue ---------------------------------------------------------------
-    const float2 lt = f2_unpack(l2), zt = f2_unpack(zs2);
-    sh.xa[half][r] = lt.x + lt.y;
-    sh.xb[half][r] = zt.x + zt.y;
-    named_bar_sync(pair, 64);
-    const float l = sh.xa[0][r] + sh.xa[1][r], zs = sh.xb[0][r] + sh.xb[1][r];
+    // ---- epilogue: the four threads' sums, relative to the last maximum ------------
+    const float2 lt = f2_unpack(st.l), zt = f2_unpack(st.zs);
+    sh.ex[0][part][r] = st.m;
+    sh.ex[1][part][r] = lt.x + lt.y;
+    sh.ex[2][part][r] = zt.x + zt.y;
+    named_bar_sync(1 + quarter, 128);
+    // (odd tiles' sums have the maximum of theirs: parts 1 and 3)
+    const float mf = fmaxf(sh.ex[0][0][r], sh.ex[0][1][r]);
+    float l = 0.f, zs = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float m = sh.ex[0][k][r], al = m == kNegInf ? 1.f : ex2(m - mf);
+      l = fmaf(sh.ex[1][k][r], al, l);
+      zs = fmaf(sh.ex[2][k][r], al, zs);
+    }
     bool ok = !failed;
     if (nt > 0 && ok) ok = mbar_wait(smem_u32(&sh.v_empty[(nt - 1) & 1]), ((nt - 1) >> 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok && lane == 0) report_error(ERR_WAIT_FULL, 0x402u);
     tc::tc_fence_after();
     const float wd = nt > 0 ? sh.w_down[(nt - 1) & (kTcRing - 1)] : 0.f;
-    T* o = static_cast<T*>(a.out) + (r0 + row) * a.o_rs + head * a.o_hs + half * (HD / 2);
+    constexpr int CH = HD * static_cast<int>(sizeof(T)) / 16, pv = 16 / sizeof(T);
     if (ok) {
+      // The tiles are free now: rows of 16-byte chunks (chunk c of row r at
+      // c ^ (r & 7)) go through them, so that a warp stores whole rows.
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-      for (int c = 0; c < HD / 2; c += 32) {
-        uint32_t u[32];
+      for (int c = 0; c < DP; c += 16) {
+        uint32_t u[16];
         if (nt > 0) {
-          tmem_ld32(lane_addr + kColO + half * (HD / 2) + c, u);
+          tc::tmem_ld16(lane_addr + kColO + part * DP + c, u);
           tc::tmem_wait_ld();
         }
-        T y[32];
+        T y[16];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
+        for (int k = 0; k < 16; ++k) {
           // column 8 w + k holds dimension 8 w + (k / 2) + (k odd ? 4 : 0)
           const int d = (k & ~7) + ((k & 7) >> 1) + ((k & 1) << 2);
-          const float t = nt > 0 ? fmaf(__uint_as_float(u[k]), wd, zs) : 0.f;
-          y[d] = from_f<T>(l == 0.f ? 0.f : t / l);
+          y[d] = from_f<T>(nt > 0 ? fmaf(__uint_as_float(u[k]), wd, zs) * inv : 0.f);
         }
-        if (real) {
-          if (args.out_vec) {
-            constexpr int pv = 16 / sizeof(T);
+        if (args.out_vec) {
 #pragma unroll
-            for (int k = 0; k < 32 / pv; ++k)
-              reinterpret_cast<uint4*>(o + c)[k] = *reinterpret_cast<const uint4*>(y + k * pv);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[c + k] = y[k];
+          for (int k = 0; k < 16 / pv; ++k) {
+            const int ch = (part * DP + c) / pv + k;
+            *reinterpret_cast<uint4*>(tiles + r * (CH * 16) + ((ch ^ (r & 7)) << 4)) =
+                *reinterpret_cast<const uint4*>(y + k * pv);
           }
+        } else if (real) {
+          T* o = static_cast<T*>(a.out) + (r0 + row) * a.o_rs + head * a.o_hs + part * DP + c;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = y[k];
         }
       }
     }
-  } else if (warp < 15) {
-    // ======================= producers =====================================
-    const int dt = tid - 256;
-    constexpr int LPR = HD / 32;                 // 16-byte chunks per code row
-    constexpr int NC = 128 * LPR;                // ... per tile
-    constexpr int RB = tc_raw_bytes<HD>();
+    // every softmax warp comes here, whatever happened
+    if (!bar_any(6, kTcSoftmax, !ok) && args.out_vec) {
+#pragma unroll 4
+      for (int i = 0; i < CH / 4; ++i) {
+        const int idx = i * kTcSoftmax + tid, rr = idx / CH, c = idx % CH;
+        const int g = static_cast<int>((rr * inv_group) >> 16);
+        if (rr < per * a.group && row0 + g < n)
+          *(reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (r0 + row0 + g) * a.o_rs +
+                                     (h * a.group + (rr - g * a.group)) * a.o_hs) + c) =
+              *reinterpret_cast<const uint4*>(tiles + rr * (CH * 16) + ((c ^ (rr & 7)) << 4));
+      }
+    }
+  } else if (warp < 20) {
+    // ======================= converters ====================================
+    regs_less<72>();
+    // 16-byte chunks of code rows, LPR per row; a thread has the same chunk of
+    // every RPI-th row, so its addresses are fixed. The eight threads of one
+    // store phase hold two rows (hd 128) and four chunks of each; taking the
+    // last two chunks' words in the order 2 3 0 1 keeps their sixteen-byte
+    // columns apart.
+    const int dt = tid - kTcSoftmax;
+    constexpr int LPR = HD / 32, RPI = kTcConverters / LPR, NI = kTcKeys / RPI;
+    const int s7 = a.shift < 7 ? a.shift : 7, cnt = 1 << s7;   // positions per packed block
+    const int rr = dt / LPR, ci = dt % LPR;
+    const bool swap = LPR == 4 && (ci & 2);
+    uint32_t src[NI], dst[4];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int p = rr + i * RPI;
+      src[i] = (p >> s7) * (cnt * (HD + 8)) + (p & (cnt - 1)) * (HD / 2) + ci * 16;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = ci * 4 + (swap ? k ^ 2 : k);       // word of the row
+      dst[k] = (c >> 3) * BLK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+    }
+    auto put = [&](uint8_t* tile, const uint8_t* codes, uint32_t groups, auto pairs) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        uint4 c4 = *reinterpret_cast<const uint4*>(codes + src[i]);
+        if (!((groups >> ((rr + i * RPI) >> 4)) & 1u)) c4 = make_uint4(0u, 0u, 0u, 0u);   // never copied
+        const uint32_t w[4] = {swap ? c4.z : c4.x, swap ? c4.w : c4.y, swap ? c4.x : c4.z,
+                               swap ? c4.y : c4.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint4*>(tile + dst[k] + i * (RPI * 128)) = pairs(w[k]);
+      }
+      fence_async_smem();
+    };
+    if (nt > 1 && !mbar_wait(smem_u32(&sh.q_ready), 0)) report_error(ERR_WAIT_FULL, 0x415u);
+#pragma unroll 1
+    for (int j = 0; j < nt; ++j) {
+      const int buf = j & 1, st = j % kTcRaw;
+      if (!mbar_wait(smem_u32(&sh.raw_full[st]), (j / kTcRaw) & 1)) {
+        report_error(ERR_WAIT_FULL, 0x413u);
+        break;
+      }
+      const uint8_t* raw = raws + st * RB;
+      const uint32_t groups = sh.raw_groups[st];
+      // K's stage is free once S(j - 2) is done, V's once O(j - 2) is
+      if (j >= 2 && !mbar_wait(smem_u32(&sh.s_full[buf]), ((j >> 1) - 1) & 1)) {
+        report_error(ERR_WAIT_EMPTY, 0x410u);
+        break;
+      }
+      put(tiles + buf * TB, raw, groups, [](uint32_t w) { return k_pairs(w); });
+      mbar_arrive(smem_u32(&sh.k_full[buf]));
+      if (j >= 2 && !mbar_wait(smem_u32(&sh.v_empty[buf]), ((j >> 1) - 1) & 1)) {
+        report_error(ERR_WAIT_EMPTY, 0x411u);
+        break;
+      }
+      put(tiles + (2 + buf) * TB, raw + cnt * (HD / 2), groups, [](uint32_t w) { return v_pairs(w); });
+      mbar_arrive(smem_u32(&sh.v_full[buf]));
+      mbar_arrive(smem_u32(&sh.raw_empty[st]));
+    }
+  } else {
+  regs_less<56>();
+  if (warp == 20) {
+    // ======================= parameters ====================================
+    // weights are p * s_v * 2^(9 - ev), ev the largest exponent of s_v so far
+    const int s7 = a.shift < 7 ? a.shift : 7, cnt = 1 << s7;
+    int ev = -100;
+#pragma unroll 1
+    for (int j = 0; j < nt; ++j) {
+      const int ring = j & (kTcRing - 1), st = j % kTcRaw;
+      if (!warp_wait(&sh.raw_full[st], (j / kTcRaw) & 1)) {
+        if (lane == 0) report_error(ERR_WAIT_FULL, 0x416u);
+        break;
+      }
+      const uint32_t groups = sh.raw_groups[st];
+      uint32_t kp[4], vp[4];
+      float mx = 0.f;
+      bool odd = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int p = lane + 32 * k;
+        const bool here = j * kTcKeys + p < seen && ((groups >> (p >> 4)) & 1u);
+        kp[k] = vp[k] = 0u;                    // positions that do not exist: s = z = 0
+        if (here) {
+          const uint8_t* q = raws + st * RB + (p >> s7) * (cnt * (HD + 8)) + cnt * HD + (p & (cnt - 1)) * 4;
+          kp[k] = *reinterpret_cast<const uint32_t*>(q);
+          vp[k] = *reinterpret_cast<const uint32_t*>(q + cnt * 4);
+        }
+        const uint32_t bits = __ballot_sync(0xffffffffu, here);
+        if (lane == 0) sh.valid[ring][k] = bits;
+        mx = fmaxf(mx, par_s(vp[k]));
+        odd = odd || !isfinite(par_s(vp[k])) || !isfinite(par_z(vp[k]));
+      }
+      mbar_arrive(smem_u32(&sh.raw_empty[st]));
+      int e = static_cast<int>((__reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23) & 255u) - 127;
+      e = e > 127 ? 127 : e;
+      const int ev_old = ev;
+      ev = e > ev ? e : ev;
+      const float up = pow2i(9 - ev);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int p = lane + 32 * k;
+        const float sv = par_s(vp[k]);
+        sh.sk[ring][p] = par_s(kp[k]);
+        sh.zk[ring][p] = par_z(kp[k]);
+        sh.sv[ring][p] = sv * up;
+        sh.zc[ring][p] = fmaf(8.f, sv, par_z(vp[k]));
+      }
+      odd = __any_sync(0xffffffffu, odd);
+      if (lane == 0) {
+        sh.odd[ring] = odd ? 1u : 0u;
+        sh.down[ring] = j == 0 ? 1.f : (ev_old - ev < -126 ? 0.f : pow2i(ev_old - ev));
+        sh.w_down[ring] = pow2i(ev - 9);
+      }
+      mbar_arrive(smem_u32(&sh.par_full[ring]));
+    }
+  } else if (warp == 21) {
+    // ======================= loader ========================================
+    // lane = page of the tile (its whole block), or, for pages of more than a
+    // tile, one of the four parts of 128 of its positions
     const int64_t ps = int64_t(1) << a.shift;
-    const int32_t* tab = a.table + b * a.width;
-    // ---- the copies of one tile: lane = (page of the tile, part of its block) --
-    const int cnt = a.shift < 7 ? 1 << a.shift : kTcKeys;        // positions per copy
-    const int pg = lane >> 2, part = lane & 3;
+    const int32_t* tab = a.table + static_cast<int64_t>(sh.item[0]) * a.width;
+    const bool parts = a.shift > 7;
+    const int cnt = parts ? kTcKeys : 1 << a.shift, copies = parts ? 4 : kTcKeys >> a.shift;
+    const int pg = parts ? 0 : lane;
+    const uint32_t bytes = parts ? (lane < 2 ? kTcKeys * (HD / 2) : kTcKeys * 4) : cnt * (HD + 8);
     auto page_of = [&](int j) -> int {
       const int p = j * kTcKeys + pg * cnt;
-      return pg * cnt < kTcKeys && p < seen ? __ldg(tab + (p >> a.shift)) : -1;
+      return lane < copies && p < seen ? __ldg(tab + (p >> a.shift)) : -1;
     };
-    int page = -1;
-    auto issue = [&](int j) {      // warp 8; `page` is page_of(j)
+    int page = page_of(0), j = 0;
+#pragma unroll 1
+    for (; j < nt; ++j) {
       const int st = j % kTcRaw;
+      if (j >= kTcRaw && !warp_wait(&sh.raw_empty[st], ((j / kTcRaw) - 1) & 1)) {
+        if (lane == 0) report_error(ERR_WAIT_EMPTY, 0x412u);
+        break;
+      }
       const bool have = page >= 0 && page < a.pages;
-      const uint32_t bytes = cnt * (part < 2 ? HD / 2 : 4);
       const uint32_t total = __reduce_add_sync(0xffffffffu, have ? bytes : 0u);
       const uint32_t groups = __reduce_or_sync(
           0xffffffffu, have ? ((1u << (cnt >> 4)) - 1u) << (pg * (cnt >> 4)) : 0u);
@@ -553,173 +820,84 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
       __syncwarp();
       if (have) {
-        const int64_t off = (j * kTcKeys + pg * cnt) & (ps - 1);
-        const uint8_t* src = a.pool + (static_cast<int64_t>(page) * a.nkv + h) * (ps * (HD + 8));
-        src += part < 2 ? part * (ps * (HD / 2)) + off * (HD / 2) : ps * HD + (part - 2) * (ps * 4) + off * 4;
-        const uint32_t dst = smem_u32(raws + st * RB) +
-                             (part < 2 ? part * (kTcKeys * (HD / 2)) + pg * cnt * (HD / 2)
-                                       : kTcKeys * HD + (part - 2) * (kTcKeys * 4) + pg * cnt * 4);
-        bulk_copy(dst, src, bytes, bar);
+        const uint8_t* from = a.pool + (static_cast<int64_t>(page) * a.nkv + h) * (ps * (HD + 8));
+        uint32_t to = smem_u32(raws + st * RB);
+        if (parts) {
+          const int64_t off = (j * kTcKeys) & (ps - 1);
+          from += lane < 2 ? lane * (ps * (HD / 2)) + off * (HD / 2)
+                           : ps * HD + (lane - 2) * (ps * 4) + off * 4;
+          to += lane < 2 ? lane * (kTcKeys * (HD / 2)) : kTcKeys * HD + (lane - 2) * (kTcKeys * 4);
+        } else {
+          to += pg * bytes;
+        }
+        bulk_copy(to, from, bytes, bar);
       }
       page = page_of(j + 1);
-    };
-    // Codes of the tile -> fp16. The eight threads of one store phase hold two
-    // rows (hd 128) and four chunks of each; taking the last two chunks' words
-    // in the order 2 3 0 1 keeps their sixteen-byte columns apart.
-    auto put = [&](uint8_t* tile, const uint8_t* codes, uint32_t groups, bool is_v) {
-#pragma unroll 2
-      for (int t = dt; t < NC; t += kTcProducers) {
-        const int row = t / LPR, ci = t % LPR;
-        uint4 c4 = *reinterpret_cast<const uint4*>(codes + t * 16);
-        if (!((groups >> (row >> 4)) & 1u)) c4 = make_uint4(0u, 0u, 0u, 0u);   // never copied
-        const bool swap = LPR == 4 && (ci & 2);
-        const uint32_t w[4] = {swap ? c4.z : c4.x, swap ? c4.w : c4.y, swap ? c4.x : c4.z,
-                               swap ? c4.y : c4.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int c = ci * 4 + (swap ? k ^ 2 : k);       // word of the row
-          const uint4 u = is_v ? v_pairs(w[k]) : k_pairs(w[k]);
-          *reinterpret_cast<uint4*>(tile + (c >> 3) * BLK + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = u;
-        }
-      }
-    };
-    bool fail = false;
-    int ev = -100, issued = 0, landed = 0;
-    if (warp == 8) {
-      page = page_of(0);
-      for (; issued < kTcRaw - 1 && issued < nt; ++issued) issue(issued);
     }
-    for (int j = 0; j < nt; ++j) {
-      const int ring = j & (kTcRing - 1), buf = j & 1, st = j % kTcRaw;
-      if (warp == 8 && issued < nt && !fail) {
-        // the stage of tile j - 1, read by every producer before it arrived there
-        if (j > 0 && !mbar_wait(smem_u32(&sh.raw_empty[(j - 1) % kTcRaw]), ((j - 1) / kTcRaw) & 1)) {
-          report_error(ERR_WAIT_EMPTY, 0x412u);
-          fail = true;
-        }
-        fail = __any_sync(0xffffffffu, fail);
-        if (!fail) issue(issued++);
-      }
-      if (!fail && !mbar_wait(smem_u32(&sh.raw_full[st]), (j / kTcRaw) & 1)) {
-        report_error(ERR_WAIT_FULL, 0x413u);
-        fail = true;
-      }
-      if (!fail) landed = j + 1;
-      const uint8_t* raw = raws + st * RB;
-      const uint32_t groups = sh.raw_groups[st];
-      // parameters, one position a thread; weights are p * s_v * 2^(9 - ev), ev
-      // the largest exponent so far
-      const bool mine = dt < kTcKeys;            // whole warps
-      const bool here = mine && j * kTcKeys + dt < seen && ((groups >> (dt >> 4)) & 1u);
-      uint32_t kpar = 0u, vpar = 0u;             // positions that do not exist: s = z = 0
-      if (here) {
-        kpar = *reinterpret_cast<const uint32_t*>(raw + kTcKeys * HD + dt * 4);
-        vpar = *reinterpret_cast<const uint32_t*>(raw + kTcKeys * (HD + 4) + dt * 4);
-      }
-      const float sv = par_s(vpar);
-      if (mine) {
-        float t = fmaxf(sv, 0.f);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-        const uint32_t bits = __ballot_sync(0xffffffffu, here);
-        if (lane == 0) {
-          sh.dmax[j & 1][warp - 8] = t;
-          sh.valid[ring][warp - 8] = bits;
-        }
-      }
-      if (bar_any(5, kTcProducers, fail)) {
-        fail = true;
+    // no copy stays in flight into memory that is given up
+    for (int t = j > kTcRaw ? j - kTcRaw : 0; t < j; ++t)
+      if (!warp_wait(&sh.raw_full[t % kTcRaw], (t / kTcRaw) & 1)) {
+        if (lane == 0) report_error(ERR_DRAIN, 0x414u);
         break;
       }
-      const float mx = fmaxf(fmaxf(sh.dmax[j & 1][0], sh.dmax[j & 1][1]),
-                             fmaxf(sh.dmax[j & 1][2], sh.dmax[j & 1][3]));
-      int e = static_cast<int>((__float_as_uint(mx) >> 23) & 255u) - 127;
-      e = e > 127 ? 127 : e;
-      const int ev_old = ev;
-      ev = e > ev ? e : ev;
-      if (mine) {
-        sh.sk[ring][dt] = par_s(kpar);
-        sh.zk[ring][dt] = par_z(kpar);
-        sh.sv[ring][dt] = sv * pow2i(9 - ev);
-        sh.zc[ring][dt] = fmaf(8.f, sv, par_z(vpar));
-      }
-      if (dt == 0) {
-        sh.down[ring] = j == 0 || ev_old - ev < -126 ? (j == 0 ? 1.f : 0.f) : pow2i(ev_old - ev);
-        sh.w_down[ring] = pow2i(ev - 9);
-      }
-      mbar_arrive(smem_u32(&sh.par_full[ring]));
-      // K (its stage is free once S(j - 2) is done), then V (once O(j - 2) is)
-      if (j >= 2 && !mbar_wait(smem_u32(&sh.s_full[buf]), ((j >> 1) - 1) & 1)) {
-        report_error(ERR_WAIT_EMPTY, 0x410u);
-        fail = true;
-      }
-      if (!fail) {
-        put(tiles + buf * TB, raw, groups, false);
-        fence_async_smem();
-        mbar_arrive(smem_u32(&sh.k_full[buf]));
-      }
-      if (!fail && j >= 2 && !mbar_wait(smem_u32(&sh.v_empty[buf]), ((j >> 1) - 1) & 1)) {
-        report_error(ERR_WAIT_EMPTY, 0x411u);
-        fail = true;
-      }
-      if (!fail) {
-        put(tiles + (2 + buf) * TB, raw + kTcKeys * (HD / 2), groups, true);
-        fence_async_smem();
-        mbar_arrive(smem_u32(&sh.v_full[buf]));
-        mbar_arrive(smem_u32(&sh.raw_empty[st]));
-      }
-    }
-    // after a failed wait: no copy stays in flight into memory that is given up
-    for (int t = landed; t < issued; ++t)
-      if (!mbar_wait(smem_u32(&sh.raw_full[t % kTcRaw]), (t / kTcRaw) & 1)) {
-        report_error(ERR_DRAIN, 0x414u);
-        break;
-      }
-  } else if (lane == 0 && nt > 0) {
+  } else if (warp == 22 && nt > 0) {
     // ======================= MMA issuer ====================================
     constexpr uint32_t id_s = idesc_f16(kTcKeys, false), id_o = idesc_f16(HD, true);
+    const bool leader = elect_one();
+    const uint64_t kdesc = tc::smem_desc_sw128(smem_u32(tiles));
+    const uint64_t vdesc = smem_desc_mn(smem_u32(tiles + 2 * TB), BLK);
     auto scores = [&](int j) {
-      const uint32_t kt = smem_u32(tiles + (j & 1) * TB), d = tmem + kColS + (j & 1) * 128;
+      const uint64_t kd = kdesc + (j & 1) * (TB >> 4);
+      const uint32_t d = tmem + kColS + (j & 1) * 128;
+      if (leader) {
 #pragma unroll
-      for (int s = 0; s < HD / 16; ++s)
+        for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
-        for (int l = 0; l < L; ++l)
-          mma_f16_ts(d, tmem + kColQ + l * (HD / 2) + s * 8,
-                     tc::smem_desc_sw128(kt + (s >> 2) * BLK + (s & 3) * 32), id_s, (s | l) != 0);
-      tc::tc_commit(smem_u32(&sh.s_full[j & 1]));
+          for (int l = 0; l < L; ++l)
+            mma_f16_ts(d, tmem + kColQ + l * (HD / 2) + s * 8,
+                       kd + (((s >> 2) * BLK + (s & 3) * 32) >> 4), id_s, (s | l) != 0);
+        tc::tc_commit(smem_u32(&sh.s_full[j & 1]));
+      }
+      __syncwarp();
     };
-    bool ok = mbar_wait(smem_u32(&sh.q_ready), 0) && mbar_wait(smem_u32(&sh.k_full[0]), 0);
+    bool ok = warp_wait(&sh.q_ready, 0) && warp_wait(&sh.k_full[0], 0);
     tc::tc_fence_after();
     if (ok) scores(0);
+#pragma unroll 1
     for (int j = 0; ok && j < nt; ++j) {
       if (j + 1 < nt) {
         // S(j + 1) goes where W(j - 1) was; the MMAs run in the order of issue
-        ok = mbar_wait(smem_u32(&sh.k_full[(j + 1) & 1]), ((j + 1) >> 1) & 1);
+        ok = warp_wait(&sh.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
         if (!ok) break;
         tc::tc_fence_after();
         scores(j + 1);
       }
-      ok = mbar_wait(smem_u32(&sh.v_full[j & 1]), (j >> 1) & 1) &&
-           mbar_wait(smem_u32(&sh.p_full[j & 1]), (j >> 1) & 1);
+      ok = warp_wait(&sh.v_full[j & 1], (j >> 1) & 1) && warp_wait(&sh.p_full[j & 1], (j >> 1) & 1);
       if (!ok) break;
       tc::tc_fence_after();
-      const uint32_t vt = smem_u32(tiles + (2 + (j & 1)) * TB), w = tmem + kColS + (j & 1) * 128;
+      const uint64_t vd = vdesc + (j & 1) * (TB >> 4);
+      const uint32_t w = tmem + kColS + (j & 1) * 128;
+      if (leader) {
 #pragma unroll
-      for (int s = 0; s < kTcKeys / 16; ++s)
+        for (int s = 0; s < kTcKeys / 16; ++s)
 #pragma unroll
-        for (int l = 0; l < L; ++l)
-          mma_f16_ts(tmem + kColO, w + (s >> 2) * 64 + (s & 3) * (8 * L) + 8 * l,
-                     smem_desc_mn(vt + s * 2048, BLK), id_o, (j | s | l) != 0);
-      tc::tc_commit(smem_u32(&sh.v_empty[j & 1]));
+          for (int l = 0; l < L; ++l)
+            mma_f16_ts(tmem + kColO, w + (s >> 2) * 64 + (s & 3) * (8 * L) + 8 * l,
+                       vd + ((s * 2048) >> 4), id_o, (j | s | l) != 0);
+        tc::tc_commit(smem_u32(&sh.v_empty[j & 1]));
+      }
+      __syncwarp();
     }
-    if (!ok) report_error(ERR_WAIT_FULL, 0x420u);
+    if (!ok && lane == 0) report_error(ERR_WAIT_FULL, 0x420u);
     // TMEM and shared memory are given up only after every issued MMA has finished
-    tc::tc_commit(smem_u32(&sh.drain));
-    if (!mbar_wait(smem_u32(&sh.drain), 0)) report_error(ERR_DRAIN, 0x421u);
+    if (leader) tc::tc_commit(smem_u32(&sh.drain));
+    __syncwarp();
+    if (!warp_wait(&sh.drain, 0) && lane == 0) report_error(ERR_DRAIN, 0x421u);
+  }
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 15) {
+  if (warp == 22) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
