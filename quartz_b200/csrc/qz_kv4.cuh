@@ -413,30 +413,38 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const GatherArgs
 // HBM speed and the tensor pipe is not the bound, so mma.sync serves here (a
 // tcgen05 tile of 128 rows would be 94 % padding).
 //
-// Fragments come straight from the packed pages: a lane's share of a K row is
-// 16 (hd 64: 8) consecutive bytes. The order of dimensions inside an MMA's K
+// Each warp streams its own 32 positions at a time: bulk copies bring the packed
+// blocks of one stage into shared memory, kAttnDepth - 1 stages ahead of the
+// math, so no registers hold data in flight. A lane's share of a K row is 16
+// (hd 64: 8) consecutive bytes. The order of dimensions inside an MMA's K
 // axis is free as long as q has the same one, so nibbles 0 and 4 of a word
 // (w & 0x000F000F) form one fp16 pair: the bits c are the subnormal c * 2^-24,
 // exact. Nibbles 1 and 5 lie four bits higher, as 16 c * 2^-24; q's values for
 // them are divided by 16. For V, pairs run along positions: one PRMT joins the
 // halves of two positions' words; 0x6400 | d is 1024 + d, and one HADD2 (HFMA2
 // for the nibbles four bits higher) leaves d - 8. Centring V keeps the running
-// sum as small as its result; the MMA's accumulation truncates.
+// sum as small as its result; the MMA's accumulation truncates. Row r of the
+// eight positions an MMA fragment pairs up is position r / 2 + 4 (r & 1), so
+// that the V rows a quarter-warp reads are neighbours (fewer bank conflicts).
 //
-// Work is cut into steps of 64 positions over all (request, kv head, block of
+// Work is cut into steps of 128 positions over all (request, kv head, block of
 // queries), shared out evenly over a fixed grid whatever the lengths, which
 // only the device knows (graph replay). A CTA's share may begin or end within an item; those partials
 // (max, sum, accumulator) go to the workspace and the last of an item's CTAs
 // to arrive merges them in CTA order, so results do not depend on timing.
 //
 // The running maximum is only renewed when a score passes it by 2^4 (weights
-// stay below 2^4 relative to it): one vote per tile instead of a reduction.
+// stay below 2^4 relative to it): one vote per stage instead of a reduction.
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kAttnTile = 16;
-constexpr int kAttnStep = kAttnWarps * kAttnTile;
+constexpr int kAttnStage = 32;    // positions per warp and stage
+constexpr int kAttnDepth = 3;     // stages of a warp
+constexpr int kAttnStep = kAttnWarps * kAttnStage;
 constexpr int kAttnMaxB = 4096;
+// What an item costs beside its positions (its query fragments, the merge), in
+// steps: the shares of short and long contexts take about as long.
+constexpr int kAttnItemUnits = 1;
 
 struct AttnArgs {
   const void* q;
@@ -455,19 +463,26 @@ struct AttnArgs {
   int rows_lo, rows_hi;             // requests with rows_lo < rows <= rows_hi are handled
 };
 
-// CTAs per SM that the register file holds without spills.
-constexpr int kAttnMaxPerSm = 4;
+// CTAs per SM that the register file and shared memory hold.
+constexpr int kAttnMaxPerSm = 5;
 __host__ __device__ constexpr int attn_per_sm(int hd, int nb) {
-  return nb == 1 ? (hd == 64 ? 4 : 3) : (hd == 64 ? 3 : 2);
+  return nb == 1 ? (hd == 64 ? 5 : 4) : (hd == 64 ? 4 : 2);
 }
 template <int HD, int NB>
 __host__ __device__ constexpr int attn_queries() { return 4 * NB; }
 template <int HD, int NB>
 __host__ __device__ constexpr int attn_part_floats() { return 4 * NB * (HD + 2); }
+template <int HD>
+__host__ __device__ constexpr int attn_stage_bytes() { return kAttnStage * (HD + 8); }
+constexpr int kAttnHead = kAttnThreads * 8 + 64 + kAttnWarps * kAttnDepth * 8;
+// The warps' rings; their results take the same place afterwards.
 template <int HD, int NB>
 __host__ __device__ constexpr int attn_smem() {
-  return kAttnThreads * 8 + 64 + kAttnWarps * attn_part_floats<HD, NB>() * 4;
+  constexpr int ring = kAttnWarps * kAttnDepth * attn_stage_bytes<HD>();
+  constexpr int merge = kAttnWarps * attn_part_floats<HD, NB>() * 4;
+  return 2048 + (ring > merge ? ring : merge);
 }
+static_assert(kAttnHead <= 2048, "the rings start 2 KB in");
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -520,51 +535,28 @@ __device__ __forceinline__ void centred4(uint32_t x, uint32_t (&h)[4]) {
 }
 
 template <int W>
-__device__ __forceinline__ void ld_stream(const uint8_t* p, uint32_t (&v)[W]) {
+__device__ __forceinline__ void lds(uint32_t addr, uint32_t (&v)[W]) {
   if constexpr (W == 4)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
   else if constexpr (W == 2)
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
-                 : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr));
   else
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(addr));
 }
 
-// A lane's share of a 16-position tile.
-template <int HD>
-struct Tile {
-  uint32_t k[2][HD / 32];   // K codes of positions g, g + 8
-  uint32_t v[4][HD / 64];   // V codes of positions 2i, 2i + 1, 2i + 8, 2i + 9
-  uint32_t kp[2], vp[2];    // (s, z) of positions g, g + 8
-  bool ok;                  // the table entry is a page of the pool
+// 1-D bulk copy global -> this CTA's shared memory (no cluster multicast).
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
 
-  __device__ __forceinline__ void load(const AttnArgs& a, int h, int page, int pos, int g, int i) {
-    ok = page >= 0 && page < a.pages;
-    if (!ok) return;
-    const int64_t ps = int64_t(1) << a.shift;
-    const int off = pos & static_cast<int>(ps - 1);
-    const uint8_t* blk = a.pool + (static_cast<int64_t>(page) * a.nkv + h) * (ps * (HD + 8));
-    const uint8_t* kc = blk + (off + g) * (HD / 2) + i * (HD / 8);
-    ld_stream(kc, k[0]);
-    ld_stream(kc + 8 * (HD / 2), k[1]);
-    const uint8_t* vc = blk + ps * (HD / 2) + (off + 2 * i) * (HD / 2) + g * (HD / 16);
-    ld_stream(vc, v[0]);
-    ld_stream(vc + HD / 2, v[1]);
-    ld_stream(vc + 8 * (HD / 2), v[2]);
-    ld_stream(vc + 9 * (HD / 2), v[3]);
-    const uint8_t* par = blk + ps * HD + (off + g) * 4;
-    uint32_t w[1];
-    ld_stream(par, w);
-    kp[0] = w[0];
-    ld_stream(par + 32, w);
-    kp[1] = w[0];
-    ld_stream(par + ps * 4, w);
-    vp[0] = w[0];
-    ld_stream(par + ps * 4 + 32, w);
-    vp[1] = w[0];
-  }
-};
+__device__ __forceinline__ void fence_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 
 __device__ __forceinline__ int64_t rows_of(const AttnArgs& a, int64_t b, int64_t* first) {
   int64_t r0 = b, r1 = b + 1;
@@ -587,6 +579,15 @@ __device__ __forceinline__ int64_t steps_of(const AttnArgs& a, int64_t len) {
   return s > 0 ? s : 1;   // an empty context still has its (zero) rows to write
 }
 
+// floor(x / y) for 0 <= x < 2^52 with inv = 1 / y: the product is off by less
+// than one, which the remainder shows.
+__device__ __forceinline__ int64_t div_floor(int64_t x, int64_t y, double inv) {
+  int64_t q = static_cast<int64_t>(static_cast<double>(x) * inv);
+  const int64_t r = x - q * y;
+  q += r >= y ? 1 : (r < 0 ? -1 : 0);
+  return q;
+}
+
 template <class T, int HD, int NB>
 __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel(const AttnArgs a) {
   constexpr int Q = attn_queries<HD, NB>();   // queries (row, head) of an item
@@ -594,22 +595,51 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
   constexpr int KW = HD / 32;                 // K words of a lane and row
   constexpr int VW = HD / 64;                 // V words of a lane and position
   constexpr float kNegInf = -INFINITY;
-  extern __shared__ __align__(16) uint8_t attn_sh[];
+  constexpr int SB = attn_stage_bytes<HD>();
+  extern __shared__ __align__(128) uint8_t attn_sh[];
   int64_t* s_scan = reinterpret_cast<int64_t*>(attn_sh);                        // [threads]
   int64_t* s_at = reinterpret_cast<int64_t*>(attn_sh + kAttnThreads * 8);       // {b, its first unit}
   int* s_last = reinterpret_cast<int*>(s_at + 2);
-  float* s_o = reinterpret_cast<float*>(attn_sh + kAttnThreads * 8 + 64);       // [warps][Q][HD]
+  float* s_o = reinterpret_cast<float*>(attn_sh + 2048);                        // [warps][Q][HD]
   float* s_ml = s_o + kAttnWarps * Q * HD;                                      // [warps][Q][2]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
+  const uint32_t bars = smem_u32(attn_sh + kAttnThreads * 8 + 64) + warp * (kAttnDepth * 8);
+  const uint32_t ring = smem_u32(attn_sh + 2048) + warp * (kAttnDepth * SB);
+  if (lane == 0) {
+    for (int k = 0; k < kAttnDepth; ++k) mbar_init(bars + 8 * k, 1);
+    fence_mbar_init();
+  }
+  // A stage is one block of 32 positions, or (pages of 16) two of 16. Copies: a
+  // whole block each, or the four parts of 32 positions of a larger page.
+  const bool small = a.shift == 4, parts = a.shift > 5;
+  const int copies = parts ? 4 : (small ? 2 : 1);
+  const uint32_t bytes = parts ? (lane < 2 ? kAttnStage * (HD / 2) : kAttnStage * 4)
+                               : (small ? SB / 2 : SB);
+  const uint32_t to = parts ? (lane < 2 ? lane * (kAttnStage * (HD / 2))
+                                        : kAttnStage * HD + (lane - 2) * (kAttnStage * 4))
+                            : lane * (SB / 2);
+  const int64_t ps = int64_t(1) << a.shift;
+  // this lane's offsets within a stage: K row and parameters of its first score
+  // row, V row of its first position; from 16 positions to the next
+  const int blk = small ? 16 : 32, tau = (g >> 1) + 4 * (g & 1);
+  const uint32_t k_at = tau * (HD / 2) + i * (HD / 8);
+  const uint32_t v_at = blk * (HD / 2) + i * (HD / 2) + g * (HD / 16);
+  const uint32_t p_at = blk * HD + tau * 4;
+  const uint32_t k_next = small ? SB / 2 : 16 * (HD / 2), p_next = small ? SB / 2 : 64;
+  int st = 0;            // the ring position of the next stage to be used
+  uint32_t phase = 0;    // its parity
 
   pdl_wait();
   // ---- this CTA's share [u0, u1) of all units --------------------------------
+  // An item (request, kv head, block of queries) is kAttnItemUnits units for its
+  // fixed costs and one for each step of its positions.
   const int per_thread = (a.B + kAttnThreads - 1) / kAttnThreads;
   auto units = [&](int64_t b) -> int64_t {
     int64_t r0;
     const int64_t n = rows_of(a, b, &r0);
     if (n == 0) return 0;
-    return a.nkv * ((n * a.group + Q - 1) / Q) * steps_of<NB>(a, a.lens[b]);
+    return a.nkv * static_cast<int64_t>((static_cast<unsigned>(n * a.group) + Q - 1) / Q) *
+           (steps_of<NB>(a, a.lens[b]) + kAttnItemUnits);
   };
   int64_t mine = 0;
   for (int k = 0; k < per_thread; ++k) {
@@ -628,7 +658,11 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
   const int64_t C = U < gridDim.x ? U : gridDim.x;
   const int64_t c = blockIdx.x;
   if (c >= C) return;
-  const int64_t u0 = c * U / C, u1 = (c + 1) * U / C;
+  const double inv_c = 1.0 / static_cast<double>(C), inv_u = 1.0 / static_cast<double>(U);
+  // CTA k's share begins at k U / C; unit x belongs to CTA ((x + 1) C - 1) / U
+  auto begin_of = [&](int64_t k) -> int64_t { return div_floor(k * U, C, inv_c); };
+  auto cta_of = [&](int64_t x) -> int64_t { return div_floor((x + 1) * C - 1, U, inv_u); };
+  const int64_t u0 = begin_of(c), u1 = begin_of(c + 1);
   if (u0 >= before && u0 < before + mine) {
     int64_t b = static_cast<int64_t>(tid) * per_thread, at = before;
     for (int64_t n = units(b); u0 >= at + n; n = units(b)) {
@@ -640,47 +674,55 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
   }
   __syncthreads();
   int64_t b = s_at[0], ub = s_at[1];
+  const int cap = static_cast<int>(a.width << a.shift);
 
   for (int64_t u = u0; u < u1;) {
     int64_t r0;
-    const int64_t n = rows_of(a, b, &r0);
+    const int n = static_cast<int>(rows_of(a, b, &r0));
     const int64_t len = n ? a.lens[b] : 0;
-    const int64_t steps = steps_of<NB>(a, len);
-    const int64_t nqb = (n * a.group + Q - 1) / Q;
-    const int64_t all = a.nkv * nqb * steps;
+    const int64_t size = steps_of<NB>(a, len) + kAttnItemUnits;   // units of an item
+    const int nqueries = n * a.group;
+    const int nqb = (nqueries + Q - 1) / Q;
+    const int64_t all = a.nkv * nqb * size;
     if (u >= ub + all) {
       ub += all;
       ++b;
       continue;
     }
-    const int64_t item = (u - ub) / steps, i0 = ub + item * steps;
-    const int64_t s0 = u - i0, s1 = steps < s0 + (u1 - u) ? steps : s0 + (u1 - u);
-    const int h = static_cast<int>(item / nqb);
-    const int64_t q0 = (item - h * nqb) * Q;   // first query of the item
-    const int64_t nqueries = n * a.group;
+    const int64_t rel = u - ub;
+    const int64_t item = rel >> 31 ? rel / size
+                                   : static_cast<int64_t>(static_cast<unsigned>(rel) / static_cast<unsigned>(size));
+    const int64_t i0 = ub + item * size, i1 = i0 + size < u1 ? i0 + size : u1;
+    // steps [s0, s1) of the item
+    const int s0 = u - i0 < kAttnItemUnits ? 0 : static_cast<int>(u - i0) - kAttnItemUnits;
+    const int s1 = static_cast<int>(i1 - i0) - kAttnItemUnits;
+    u = i1;
+    if (s1 <= s0) continue;                  // (the item's steps are the next CTA's)
+    const int h = static_cast<int>(static_cast<unsigned>(item) / static_cast<unsigned>(nqb));
+    const int q0 = (static_cast<int>(item) - h * nqb) * Q;   // first query of the item
 
-    // positions [0, lim) that a query sees
-    const int64_t cap = a.width << a.shift;
-    auto limit = [&](int64_t qi) -> int {
+    // positions [0, lim) that a query sees; rows and positions are at most 2^30
+    const int64_t far = int64_t(1) << 30, off64 = len - n;
+    const int off = static_cast<int>(off64 > far ? far : (off64 < -far ? -far : off64));
+    auto limit = [&](int qi) -> int {
       if (qi >= nqueries) return 0;
-      const int64_t l = len - n + qi / a.group + 1;
-      return static_cast<int>(l < 0 ? 0 : (l > cap ? cap : l));
+      const int l = off + static_cast<int>(static_cast<unsigned>(qi) / static_cast<unsigned>(a.group)) + 1;
+      return l < 0 ? 0 : (l > cap ? cap : l);
     };
     int lim[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) lim[nb] = limit(q0 + nb * 4 + i);
-    const int64_t last_q = q0 + Q < nqueries ? q0 + Q - 1 : nqueries - 1;
-    const int seen = limit(last_q);   // the last query of the block sees most
+    const int seen = limit(q0 + Q < nqueries ? q0 + Q - 1 : nqueries - 1);   // the last query of the block sees most
 
     // ---- q: two fp16 columns per query, scaled by a power of two --------------
     uint32_t qf[NB][KS][2];
     float F[NB], Qs[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int64_t qi = q0 + nb * 4 + (g >> 1);
+      const int qi = q0 + nb * 4 + (g >> 1);
       float x[HD / 4];
       if (qi < nqueries) {
-        const int64_t r = qi / a.group;
+        const int r = static_cast<int>(static_cast<unsigned>(qi) / static_cast<unsigned>(a.group));
         const T* p = static_cast<const T*>(a.q) + (r0 + r) * a.q_rs +
                      (h * a.group + (qi - r * a.group)) * a.q_hs + i * (HD / 4);
         load_row(p, a.vec, x);
@@ -707,19 +749,19 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
       const float f = pow2i(10 + e) * a.scale, qs = sum * a.scale;
       F[nb] = __shfl_sync(0xffffffffu, f, 8 * i);
       Qs[nb] = __shfl_sync(0xffffffffu, qs, 8 * i);
-      auto limb = [&](float v) -> __half {
-        const uint32_t w = split_h2(v * up);
-        return __ushort_as_half(static_cast<unsigned short>(g & 1 ? w >> 16 : w & 0xFFFFu));
-      };
-      const __half r16 = __ushort_as_half(0x2C00);   // 1 / 16
+      // pairs (0 4) (1 5) (2 6) (3 7) of each eight; odd nibbles stand as 16 c
 #pragma unroll
-      for (int m = 0; m < KW; ++m) {
-        const float* e8 = x + 8 * m;
-        qf[nb][2 * m][0] = pack_h2(limb(e8[0]), limb(e8[4]));
-        qf[nb][2 * m][1] = pack_h2(__hmul(limb(e8[1]), r16), __hmul(limb(e8[5]), r16));
-        qf[nb][2 * m + 1][0] = pack_h2(limb(e8[2]), limb(e8[6]));
-        qf[nb][2 * m + 1][1] = pack_h2(__hmul(limb(e8[3]), r16), __hmul(limb(e8[7]), r16));
-      }
+      for (int m = 0; m < KW; ++m)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float s = k & 1 ? up * 0.0625f : up;
+          const float y0 = x[8 * m + k] * s, y1 = x[8 * m + k + 4] * s;
+          const __half2 hi = __floats2half2_rn(y0, y1);
+          const float2 back = __half22float2(hi);
+          const __half2 lo = __floats2half2_rn(y0 - back.x, y1 - back.y);
+          const __half2 v = g & 1 ? lo : hi;
+          qf[nb][2 * m + (k >> 1)][k & 1] = *reinterpret_cast<const uint32_t*>(&v);
+        }
     }
 
     float acc[NB][KS][4], m[NB], l[NB], zs[NB];
@@ -735,24 +777,69 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
     int ev = -100;                       // weights are p * s * 2^(9 - ev)
     float s_lim = pow2i(ev + 1), w_up = pow2i(9 - ev);
 
-    // ---- tiles of this warp ----------------------------------------------------
+    // ---- stages of this warp ---------------------------------------------------
     const int32_t* tab = a.table + b * a.width;
-    const int64_t t_end64 = (s1 * kAttnStep < seen ? s1 * kAttnStep : seen);
-    const int t_end = static_cast<int>(t_end64);
-    int pos = static_cast<int>(s0 * kAttnStep) + warp * kAttnTile;
-    auto page_at = [&](int p) -> int { return p < t_end ? __ldg(tab + (p >> a.shift)) : -1; };
-    Tile<HD> cur, nxt;
-    cur.ok = nxt.ok = false;
-    if (pos < t_end) cur.load(a, h, page_at(pos), pos, g, i);
-    int page_next = page_at(pos + kAttnStep);
-    for (; pos < t_end; pos += kAttnStep) {
-      nxt.ok = false;
-      if (pos + kAttnStep < t_end) {
-        nxt.load(a, h, page_next, pos + kAttnStep, g, i);
-        page_next = page_at(pos + 2 * kAttnStep);
+    const int t_end = s1 * kAttnStep < seen ? s1 * kAttnStep : seen;
+    int pos = s0 * kAttnStep + warp * kAttnStage;
+    int ahead = pos;                       // first position of the next stage to be copied
+    auto page_at = [&](int p) -> int {
+      p += small ? lane * 16 : 0;
+      return lane < copies && p < t_end ? __ldg(tab + (p >> a.shift)) : -1;
+    };
+    int page = page_at(ahead);
+    // bit (stage's 16-position half) of ring position k: that half was copied
+    uint32_t there = 0;
+    auto issue = [&](int k) {
+      const bool have = page >= 0 && page < a.pages;
+      const uint32_t vote = __ballot_sync(0xffffffffu, have);
+      const uint32_t halves = small ? vote & 3u : (vote & 1u) * 3u;
+      there = (there & ~(3u << (2 * k))) | (halves << (2 * k));
+      const uint32_t bar = bars + 8 * k;
+      if (lane == 0) mbar_arrive_expect_tx(bar, small ? __popc(vote) * (SB / 2) : (vote ? SB : 0));
+      __syncwarp();
+      if (have) {
+        const uint8_t* from = a.pool + (static_cast<int64_t>(page) * a.nkv + h) * (ps * (HD + 8));
+        if (parts) {
+          const int64_t off = ahead & (ps - 1);
+          from += lane < 2 ? lane * (ps * (HD / 2)) + off * (HD / 2)
+                           : ps * HD + (lane - 2) * (ps * 4) + off * 4;
+        }
+        bulk_copy(ring + k * SB + to, from, bytes, bar);
       }
-      if (cur.ok) {
-        // scores
+      ahead += kAttnStep;
+      page = page_at(ahead);
+    };
+    {
+      int k = st;
+      for (int j = 0; j < kAttnDepth - 1 && ahead < t_end; ++j) {
+        issue(k);
+        k = k + 1 == kAttnDepth ? 0 : k + 1;
+      }
+    }
+    for (; pos < t_end; pos += kAttnStep) {
+      if (ahead < t_end) issue(st == 0 ? kAttnDepth - 1 : st - 1);   // the stage used last
+      const bool landed = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, phase));
+      if (!landed) {   // reported; the copy gets as long again before its place is used
+        if (lane == 0) report_error(ERR_WAIT_FULL, 0x430u);
+        mbar_wait(bars + 8 * st, phase);
+      }
+      const uint32_t base = ring + st * SB, half_ok = landed ? there >> (2 * st) : 0u;
+      // scores of rows g, g + 8 of both halves
+      float x[2][2][NB];
+      bool vis[2][2][NB], renew = false;
+      uint32_t vp[2][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        uint32_t k0[KW], k1[KW], kp[2], one[1];
+        lds(base + k_at + t * k_next, k0);
+        lds(base + k_at + t * k_next + 8 * (HD / 2), k1);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          lds(base + p_at + t * p_next + 32 * r, one);
+          kp[r] = one[0];
+          lds(base + p_at + t * p_next + 32 * r + blk * 4, one);
+          vp[t][r] = one[0];
+        }
         float sc[NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -760,74 +847,80 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
           for (int j = 0; j < 4; ++j) sc[nb][j] = 0.f;
 #pragma unroll
         for (int w = 0; w < KW; ++w) {
-          const uint32_t x = cur.k[0][w], y = cur.k[1][w];
-          const uint32_t x8 = x >> 8, y8 = y >> 8;
+          const uint32_t c0 = k0[w], c1 = k1[w], d0 = c0 >> 8, d1 = c1 >> 8;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            mma_f16(sc[nb], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u,
+            mma_f16(sc[nb], c0 & 0x000F000Fu, c1 & 0x000F000Fu, c0 & 0x00F000F0u, c1 & 0x00F000F0u,
                     qf[nb][2 * w][0], qf[nb][2 * w][1]);
-            mma_f16(sc[nb], x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u,
-                    y8 & 0x00F000F0u, qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
+            mma_f16(sc[nb], d0 & 0x000F000Fu, d1 & 0x000F000Fu, d0 & 0x00F000F0u, d1 & 0x00F000F0u,
+                    qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
           }
         }
-        const float sk0 = par_s(cur.kp[0]), zk0 = par_z(cur.kp[0]);
-        const float sk1 = par_s(cur.kp[1]), zk1 = par_z(cur.kp[1]);
-        const float sv0 = par_s(cur.vp[0]), sv1 = par_s(cur.vp[1]);
-        const float zc0 = fmaf(8.f, sv0, par_z(cur.vp[0]));
-        const float zc1 = fmaf(8.f, sv1, par_z(cur.vp[1]));
-        float x0[NB], x1[NB];
-        bool v0[NB], v1[NB], renew = false;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float sk = par_s(kp[r]), zk = par_z(kp[r]);
+          const bool heavy = par_s(vp[t][r]) >= s_lim;
+          const int p = (half_ok >> t) & 1u ? pos + 16 * t + 8 * r + tau : 0x7FFFFFFF;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const bool v = p < lim[nb];
+            const float y = fmaf((sc[nb][2 * r] + sc[nb][2 * r + 1]) * F[nb], sk, zk * Qs[nb]);
+            x[t][r][nb] = v ? y : kNegInf;
+            vis[t][r][nb] = v;
+            renew = renew || x[t][r][nb] > m[nb] + 4.f || (v && heavy);
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, renew)) {
+        // new maximum per query and new exponent of V's steps
+        float sm = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              if (vis[t][r][nb]) sm = fmaxf(sm, par_s(vp[t][r]));
+        const int es = static_cast<int>((__reduce_max_sync(0xffffffffu, __float_as_uint(sm)) >> 23) & 255u) - 127;
+        const int ev_old = ev;
+        ev = es > ev ? (es > 127 ? 127 : es) : ev;
+        s_lim = ev >= 127 ? INFINITY : pow2i(ev + 1);
+        w_up = pow2i(9 - ev);
+        const float down = ev_old - ev < -126 ? 0.f : pow2i(ev_old - ev);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          v0[nb] = pos + g < lim[nb];
-          v1[nb] = pos + g + 8 < lim[nb];
-          x0[nb] = v0[nb] ? fmaf((sc[nb][0] + sc[nb][1]) * F[nb], sk0, zk0 * Qs[nb]) : kNegInf;
-          x1[nb] = v1[nb] ? fmaf((sc[nb][2] + sc[nb][3]) * F[nb], sk1, zk1 * Qs[nb]) : kNegInf;
-          renew = renew || x0[nb] > m[nb] + 4.f || x1[nb] > m[nb] + 4.f ||
-                  (v0[nb] && sv0 >= s_lim) || (v1[nb] && sv1 >= s_lim);
+          float t = fmaxf(fmaxf(x[0][0][nb], x[0][1][nb]), fmaxf(x[1][0][nb], x[1][1][nb]));
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+          const float mn = fmaxf(m[nb], t);
+          const float al = m[nb] == kNegInf ? 1.f : ex2(m[nb] - mn);
+          m[nb] = mn;
+          l[nb] *= al;
+          zs[nb] *= al;
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[nb][k][j] *= al * down;
         }
-        if (__any_sync(0xffffffffu, renew)) {
-          // new maximum per query and new exponent of V's steps
-          float sm = 0.f;
+      }
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (v0[nb]) sm = fmaxf(sm, sv0);
-            if (v1[nb]) sm = fmaxf(sm, sv1);
-          }
+      for (int t = 0; t < 2; ++t) {
+        uint32_t v[4][VW];
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, o));
-          const int es = static_cast<int>((__float_as_uint(sm) >> 23) & 255u) - 127;
-          const int ev_old = ev;
-          ev = es > ev ? es : ev;
-          s_lim = ev >= 127 ? INFINITY : pow2i(ev + 1);
-          w_up = pow2i(9 - ev);
-          const float down = ev_old - ev < -126 ? 0.f : pow2i(ev_old - ev);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float t = fmaxf(x0[nb], x1[nb]);
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-            const float mn = fmaxf(m[nb], t);
-            const float al = m[nb] == kNegInf ? 1.f : ex2(m[nb] - mn);
-            m[nb] = mn;
-            l[nb] *= al;
-            zs[nb] *= al;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[nb][k][j] *= al * down;
-          }
-        }
+        for (int r = 0; r < 4; ++r) lds(base + v_at + t * k_next + r * 4 * (HD / 2), v[r]);
         uint32_t wb[NB][2];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          // selected, not multiplied, away: a hidden position may hold anything
-          const float p0 = v0[nb] ? ex2(x0[nb] - m[nb]) : 0.f;
-          const float p1 = v1[nb] ? ex2(x1[nb] - m[nb]) : 0.f;
-          l[nb] += p0 + p1;
-          zs[nb] = fmaf(p0, v0[nb] ? zc0 : 0.f, fmaf(p1, v1[nb] ? zc1 : 0.f, zs[nb]));
-          wb[nb][0] = trans8x8(split_h2(v0[nb] ? p0 * (sv0 * w_up) : 0.f));
-          wb[nb][1] = trans8x8(split_h2(v1[nb] ? p1 * (sv1 * w_up) : 0.f));
+        for (int r = 0; r < 2; ++r) {
+          const float sv = par_s(vp[t][r]), zc = fmaf(8.f, sv, par_z(vp[t][r]));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            // selected, not multiplied, away: a hidden position may hold anything
+            const bool see = vis[t][r][nb];
+            const float p = see ? ex2(x[t][r][nb] - m[nb]) : 0.f;
+            l[nb] += p;
+            zs[nb] = fmaf(p, see ? zc : 0.f, zs[nb]);
+            wb[nb][r] = trans8x8(split_h2(see ? p * (sv * w_up) : 0.f));
+          }
         }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
@@ -835,8 +928,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
           for (int half = 0; half < 2; ++half) {
             const uint32_t sel = half ? 0x7632u : 0x5410u;
             uint32_t ha[4], hb[4];
-            centred4(prmt(cur.v[0][w], cur.v[1][w], sel), ha);
-            centred4(prmt(cur.v[2][w], cur.v[3][w], sel), hb);
+            centred4(prmt(v[0][w], v[1][w], sel), ha);
+            centred4(prmt(v[2][w], v[3][w], sel), hb);
 #pragma unroll
             for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -846,8 +939,11 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
           }
         }
       }
-      cur = nxt;
+      __syncwarp();                        // the stage may be copied over
+      st = st + 1 == kAttnDepth ? 0 : st + 1;
+      phase ^= st == 0 ? 1u : 0u;
     }
+    __syncthreads();   // the rings are done with: the results take their place
 
     // ---- the warps' partials, relative to each warp's maximum -----------------
     const float w_down = pow2i(ev - 9);
@@ -872,75 +968,97 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
     __syncthreads();
 
     // ---- merge: the warps, then (for a shared item) the CTAs -------------------
-    const int64_t c_first = ((i0 + 1) * C - 1) / U, c_last = ((i0 + steps) * C - 1) / U;
+    const int64_t c_first = cta_of(i0 + kAttnItemUnits), c_last = cta_of(i0 + size - 1);
     const int parts = static_cast<int>(c_last - c_first) + 1;
-    auto store = [&](int qq, int d, float o, float lsum) {
-      const int64_t qi = q0 + qq;
+    auto store = [&](int qq, int d, const float4& o, float lsum) {
+      const int qi = q0 + qq;
       if (qi >= nqueries) return;
-      const int64_t r = qi / a.group;
-      static_cast<T*>(a.out)[(r0 + r) * a.o_rs + (h * a.group + (qi - r * a.group)) * a.o_hs + d] =
-          from_f<T>(lsum == 0.f ? 0.f : o / lsum);
+      const int r = static_cast<int>(static_cast<unsigned>(qi) / static_cast<unsigned>(a.group));
+      T* p = static_cast<T*>(a.out) + (r0 + r) * a.o_rs + (h * a.group + (qi - r * a.group)) * a.o_hs + d;
+      const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
+      p[0] = from_f<T>(o.x * inv);
+      p[1] = from_f<T>(o.y * inv);
+      p[2] = from_f<T>(o.z * inv);
+      p[3] = from_f<T>(o.w * inv);
+    };
+    auto add = [](float4& o, float f, const float4& v) {
+      o.x = fmaf(f, v.x, o.x);
+      o.y = fmaf(f, v.y, o.y);
+      o.z = fmaf(f, v.z, o.z);
+      o.w = fmaf(f, v.w, o.w);
     };
     float* mypart = a.part + (c * 2 + (c == c_first && u0 < i0 ? 1 : 0)) * (Q * (HD + 2));
-    for (int e = tid; e < Q * HD; e += kAttnThreads) {
-      const int qq = e / HD, d = e - qq * HD;
+    for (int e = tid; e < Q * HD / 4; e += kAttnThreads) {
+      const int qq = e / (HD / 4), d = (e - qq * (HD / 4)) * 4;
       float M = kNegInf;
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, s_ml[(w * Q + qq) * 2]);
-      float o = 0.f, ls = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float ls = 0.f;
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) {
         const float mw = s_ml[(w * Q + qq) * 2];
         const float f = mw == kNegInf ? 0.f : ex2(mw - M);
-        o = fmaf(f, s_o[(w * Q + qq) * HD + d], o);
+        add(o, f, *reinterpret_cast<const float4*>(s_o + (w * Q + qq) * HD + d));
         ls = fmaf(f, s_ml[(w * Q + qq) * 2 + 1], ls);
       }
       if (parts == 1) {
         store(qq, d, o, ls);
       } else {
-        __stcg(mypart + qq * HD + d, o);
-        if (d == 0) {
-          __stcg(mypart + Q * HD + qq * 2, M);
-          __stcg(mypart + Q * HD + qq * 2 + 1, ls);
-        }
+        __stcg(reinterpret_cast<float4*>(mypart + qq * HD + d), o);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(mypart + Q * HD + qq * 2), make_float2(M, ls));
       }
     }
     if (parts > 1) {
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
+        __threadfence();                     // the CTA's partial before its ticket
         const unsigned old = atomicAdd(a.tickets + c_first, 1u);
         *s_last = old == static_cast<unsigned>(parts - 1);
+        __threadfence();
       }
       __syncthreads();
       if (*s_last) {
-        __threadfence();
         // an item begins in its first CTA's last segment (slot 1 unless that CTA begins with
         // it) and is the first segment (slot 0) of the others
-        const int64_t first_u0 = c_first * U / C;
-        auto part = [&](int k) -> const float* {
-          const int64_t slot = k == 0 && first_u0 < i0 ? 1 : 0;
-          return a.part + ((c_first + k) * 2 + slot) * (Q * (HD + 2));
-        };
-        for (int e = tid; e < Q * HD; e += kAttnThreads) {
-          const int qq = e / HD, d = e - qq * HD;
-          float M = kNegInf;
-          for (int k = 0; k < parts; ++k) M = fmaxf(M, __ldcg(part(k) + Q * HD + qq * 2));
-          float o = 0.f, ls = 0.f;
-          for (int k = 0; k < parts; ++k) {
-            const float* p = part(k);
-            const float mk = __ldcg(p + Q * HD + qq * 2);
-            const float f = mk == kNegInf ? 0.f : ex2(mk - M);
-            o = fmaf(f, __ldcg(p + qq * HD + d), o);
-            ls = fmaf(f, __ldcg(p + Q * HD + qq * 2 + 1), ls);
+        const float* base = a.part + c_first * 2 * (Q * (HD + 2));
+        const int skip = begin_of(c_first) < i0 ? Q * (HD + 2) : 0;
+        for (int e = tid; e < Q * HD / 4; e += kAttnThreads) {
+          const int qq = e / (HD / 4), d = (e - qq * (HD / 4)) * 4;
+          // the running maximum is renewed part by part, four parts in flight
+          float M = kNegInf, ls = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int k0 = 0; k0 < parts; k0 += 4) {
+            float2 ml[4];
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float* p = base + static_cast<int64_t>(k0 + k) * 2 * (Q * (HD + 2)) + (k0 + k == 0 ? skip : 0);
+              const bool have = k0 + k < parts;
+              ml[k] = have ? __ldcg(reinterpret_cast<const float2*>(p + Q * HD + qq * 2))
+                           : make_float2(kNegInf, 0.f);
+              v[k] = have ? __ldcg(reinterpret_cast<const float4*>(p + qq * HD + d))
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            const float mn = fmaxf(fmaxf(M, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+            const float al = M == kNegInf ? 1.f : ex2(M - mn);   // (sums of 0, or NaN, without a maximum)
+            M = mn;
+            ls *= al;
+            o = make_float4(o.x * al, o.y * al, o.z * al, o.w * al);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float f = ml[k].x == kNegInf ? 0.f : ex2(ml[k].x - M);
+              add(o, f, v[k]);
+              ls = fmaf(f, ml[k].y, ls);
+            }
           }
           store(qq, d, o, ls);
         }
         if (tid == 0) a.tickets[c_first] = 0u;   // ready for the next call
       }
     }
-    __syncthreads();   // shared memory is reused by the next segment
-    u += s1 - s0;
+    fence_async_smem();   // these reads and writes come before the next segment's copies
+    __syncthreads();
   }
 }
 

@@ -97,6 +97,7 @@ Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int nb, int hd) {
 
 template <class T, int HD, int NB>
 int launch_kv4_attn(const qz::kv4::AttnArgs& a, int grid, cudaStream_t st) {
+  QZ_CUDA(allow_smem(qz::kv4::attn_kernel<T, HD, NB>, qz::kv4::attn_smem<HD, NB>()));
   return launch_kv4(qz::kv4::attn_kernel<T, HD, NB>, grid, qz::kv4::kAttnThreads,
                     qz::kv4::attn_smem<HD, NB>(), st, a);
 }
@@ -222,7 +223,8 @@ int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_h
   if (dtype < 0 || dtype > 2) return fail(QZ_ERR_INVALID, "qz_kv4_attention: unknown dtype");
   if (B < 0 || B > qz::kv4::kAttnMaxB)
     return fail(QZ_ERR_INVALID, "qz_kv4_attention: requests must be 0 .. 4096");
-  if (n < 0 || n > (int64_t(1) << 30)) return fail(QZ_ERR_INVALID, "qz_kv4_attention: bad row count");
+  if (n < 0 || n > (int64_t(1) << 30) / (nq / nkv))
+    return fail(QZ_ERR_INVALID, "qz_kv4_attention: bad row count");
   if (width < 1 || width > (int64_t(1) << 30) / page_size)
     return fail(QZ_ERR_INVALID, "qz_kv4_attention: table width must be 1 .. 2^30 / page size");
   if (max_rows < 1 || (!cu_rows && max_rows != 1))

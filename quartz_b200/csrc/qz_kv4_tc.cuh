@@ -157,19 +157,6 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t lead) {
   return d;
 }
 
-// 1-D bulk copy global -> this CTA's shared memory (no cluster multicast).
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-
-__device__ __forceinline__ void fence_async_smem() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
 // Whether `q` holds for any of the `n` threads at named barrier `id`.
 __device__ __forceinline__ bool bar_any(int id, int n, bool q) {
   uint32_t r;
