@@ -415,7 +415,9 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const GatherArgs
 //
 // Each warp streams its own 32 positions at a time: bulk copies bring the packed
 // blocks of one stage into shared memory, kAttnDepth - 1 stages ahead of the
-// math, so no registers hold data in flight. A lane's share of a K row is 16
+// math, so no registers hold data in flight. (cp.async by all lanes: 4 to 6 %
+// slower for pages of 16 and 32, for its instructions; 5 % faster for larger
+// pages, which take four copies a stage here.) A lane's share of a K row is 16
 // (hd 64: 8) consecutive bytes. The order of dimensions inside an MMA's K
 // axis is free as long as q has the same one, so nibbles 0 and 4 of a word
 // (w & 0x000F000F) form one fp16 pair: the bits c are the subnormal c * 2^-24,
@@ -618,7 +620,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
   const uint32_t to = parts ? (lane < 2 ? lane * (kAttnStage * (HD / 2))
                                         : kAttnStage * HD + (lane - 2) * (kAttnStage * 4))
                             : lane * (SB / 2);
-  const int64_t ps = int64_t(1) << a.shift;
+  const int64_t ps = int64_t(1) << a.shift, page_bytes = a.nkv * (ps * (HD + 8));
   // this lane's offsets within a stage: K row and parameters of its first score
   // row, V row of its first position; from 16 positions to the next
   const int blk = small ? 16 : 32, tau = (g >> 1) + 4 * (g & 1);
@@ -689,9 +691,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
       ++b;
       continue;
     }
-    const int64_t rel = u - ub;
-    const int64_t item = rel >> 31 ? rel / size
-                                   : static_cast<int64_t>(static_cast<unsigned>(rel) / static_cast<unsigned>(size));
+    const int64_t in_b = u - ub;
+    const int64_t item = in_b >> 31 ? in_b / size
+                                    : static_cast<int64_t>(static_cast<unsigned>(in_b) / static_cast<unsigned>(size));
     const int64_t i0 = ub + item * size, i1 = i0 + size < u1 ? i0 + size : u1;
     // steps [s0, s1) of the item
     const int s0 = u - i0 < kAttnItemUnits ? 0 : static_cast<int>(u - i0) - kAttnItemUnits;
@@ -705,14 +707,17 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
     const int64_t far = int64_t(1) << 30, off64 = len - n;
     const int off = static_cast<int>(off64 > far ? far : (off64 < -far ? -far : off64));
     auto limit = [&](int qi) -> int {
-      if (qi >= nqueries) return 0;
       const int l = off + static_cast<int>(static_cast<unsigned>(qi) / static_cast<unsigned>(a.group)) + 1;
       return l < 0 ? 0 : (l > cap ? cap : l);
     };
     int lim[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) lim[nb] = limit(q0 + nb * 4 + i);
-    const int seen = limit(q0 + Q < nqueries ? q0 + Q - 1 : nqueries - 1);   // the last query of the block sees most
+    for (int nb = 0; nb < NB; ++nb) {
+      const int qi = q0 + nb * 4 + i;
+      lim[nb] = limit(qi < nqueries ? qi : nqueries - 1);   // (more queries than there are: q = 0)
+    }
+    const int all_see = limit(q0);                 // the first query sees least ...
+    const int seen = limit(q0 + Q < nqueries ? q0 + Q - 1 : nqueries - 1);   // ... and the last most
 
     // ---- q: two fp16 columns per query, scaled by a power of two --------------
     uint32_t qf[NB][KS][2];
@@ -764,11 +769,12 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
         }
     }
 
-    float acc[NB][KS][4], m[NB], l[NB], zs[NB];
+    // m: maximum; rel: what scores are taken relative to (0 until there is a maximum)
+    float acc[NB][KS][4], m[NB], rel[NB], l[NB], zs[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       m[nb] = kNegInf;
-      l[nb] = zs[nb] = 0.f;
+      rel[nb] = l[nb] = zs[nb] = 0.f;
 #pragma unroll
       for (int t = 0; t < KS; ++t)
 #pragma unroll
@@ -787,6 +793,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
       return lane < copies && p < t_end ? __ldg(tab + (p >> a.shift)) : -1;
     };
     int page = page_at(ahead);
+    const uint8_t* head = a.pool + static_cast<int64_t>(h) * (ps * (HD + 8));
+    if (parts) head += lane < 2 ? lane * (ps * (HD / 2)) : ps * HD + (lane - 2) * (ps * 4);
+    const uint32_t per_pos = parts ? (lane < 2 ? HD / 2 : 4) : 0;
     // bit (stage's 16-position half) of ring position k: that half was copied
     uint32_t there = 0;
     auto issue = [&](int k) {
@@ -798,12 +807,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
       if (lane == 0) mbar_arrive_expect_tx(bar, small ? __popc(vote) * (SB / 2) : (vote ? SB : 0));
       __syncwarp();
       if (have) {
-        const uint8_t* from = a.pool + (static_cast<int64_t>(page) * a.nkv + h) * (ps * (HD + 8));
-        if (parts) {
-          const int64_t off = ahead & (ps - 1);
-          from += lane < 2 ? lane * (ps * (HD / 2)) + off * (HD / 2)
-                           : ps * HD + (lane - 2) * (ps * 4) + off * 4;
-        }
+        const uint8_t* from = head + page * page_bytes + (ahead & (static_cast<int>(ps) - 1)) * per_pos;
         bulk_copy(ring + k * SB + to, from, bytes, bar);
       }
       ahead += kAttnStep;
@@ -823,11 +827,11 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
         if (lane == 0) report_error(ERR_WAIT_FULL, 0x430u);
         mbar_wait(bars + 8 * st, phase);
       }
-      const uint32_t base = ring + st * SB, half_ok = landed ? there >> (2 * st) : 0u;
-      // scores of rows g, g + 8 of both halves
+      const uint32_t base = ring + st * SB, half_ok = landed ? (there >> (2 * st)) & 3u : 0u;
+      const bool whole = half_ok == 3u && pos + kAttnStage <= all_see;
+      // scores of rows g, g + 8 of both halves, and their V parameters
       float x[2][2][NB];
-      bool vis[2][2][NB], renew = false;
-      uint32_t vp[2][2];
+      uint32_t vp[2][2][NB];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         uint32_t k0[KW], k1[KW], kp[2], one[1];
@@ -838,7 +842,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
           lds(base + p_at + t * p_next + 32 * r, one);
           kp[r] = one[0];
           lds(base + p_at + t * p_next + 32 * r + blk * 4, one);
-          vp[t][r] = one[0];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) vp[t][r][nb] = one[0];
         }
         float sc[NB][4];
 #pragma unroll
@@ -859,28 +864,37 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float sk = par_s(kp[r]), zk = par_z(kp[r]);
-          const bool heavy = par_s(vp[t][r]) >= s_lim;
-          const int p = (half_ok >> t) & 1u ? pos + 16 * t + 8 * r + tau : 0x7FFFFFFF;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const bool v = p < lim[nb];
-            const float y = fmaf((sc[nb][2 * r] + sc[nb][2 * r + 1]) * F[nb], sk, zk * Qs[nb]);
-            x[t][r][nb] = v ? y : kNegInf;
-            vis[t][r][nb] = v;
-            renew = renew || x[t][r][nb] > m[nb] + 4.f || (v && heavy);
-          }
+          for (int nb = 0; nb < NB; ++nb)
+            x[t][r][nb] = fmaf((sc[nb][2 * r] + sc[nb][2 * r + 1]) * F[nb], sk, zk * Qs[nb]);
         }
       }
-      if (__any_sync(0xffffffffu, renew)) {
-        // new maximum per query and new exponent of V's steps
-        float sm = 0.f;
+      if (!whole) {
+        // hidden positions, which may hold anything: no score, no V
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+          for (int r = 0; r < 2; ++r) {
+            const int p = (half_ok >> t) & 1u ? pos + 16 * t + 8 * r + tau : 0x7FFFFFFF;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
-              if (vis[t][r][nb]) sm = fmaxf(sm, par_s(vp[t][r]));
+              if (p >= lim[nb]) {
+                x[t][r][nb] = kNegInf;
+                vp[t][r][nb] = 0u;
+              }
+          }
+      }
+      float top[NB], sm = 0.f;
+      bool renew = false;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        top[nb] = fmaxf(fmaxf(x[0][0][nb], x[0][1][nb]), fmaxf(x[1][0][nb], x[1][1][nb]));
+        renew = renew || top[nb] > m[nb] + 4.f;
+        sm = fmaxf(fmaxf(sm, fmaxf(par_s(vp[0][0][nb]), par_s(vp[0][1][nb]))),
+                   fmaxf(par_s(vp[1][0][nb]), par_s(vp[1][1][nb])));
+      }
+      if (__any_sync(0xffffffffu, renew || sm >= s_lim)) {
+        // new maximum per query and new exponent of V's steps
         const int es = static_cast<int>((__reduce_max_sync(0xffffffffu, __float_as_uint(sm)) >> 23) & 255u) - 127;
         const int ev_old = ev;
         ev = es > ev ? (es > 127 ? 127 : es) : ev;
@@ -889,12 +903,13 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
         const float down = ev_old - ev < -126 ? 0.f : pow2i(ev_old - ev);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          float t = fmaxf(fmaxf(x[0][0][nb], x[0][1][nb]), fmaxf(x[1][0][nb], x[1][1][nb]));
+          float t = top[nb];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
           const float mn = fmaxf(m[nb], t);
           const float al = m[nb] == kNegInf ? 1.f : ex2(m[nb] - mn);
           m[nb] = mn;
+          rel[nb] = mn == kNegInf ? 0.f : mn;
           l[nb] *= al;
           zs[nb] *= al;
 #pragma unroll
@@ -910,17 +925,22 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
         for (int r = 0; r < 4; ++r) lds(base + v_at + t * k_next + r * 4 * (HD / 2), v[r]);
         uint32_t wb[NB][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float sv = par_s(vp[t][r]), zc = fmaf(8.f, sv, par_z(vp[t][r]));
+        for (int nb = 0; nb < NB; ++nb) {
+          float w[2];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            // selected, not multiplied, away: a hidden position may hold anything
-            const bool see = vis[t][r][nb];
-            const float p = see ? ex2(x[t][r][nb] - m[nb]) : 0.f;
+          for (int r = 0; r < 2; ++r) {
+            const float p = ex2(x[t][r][nb] - rel[nb]), sv = par_s(vp[t][r][nb]);
             l[nb] += p;
-            zs[nb] = fmaf(p, see ? zc : 0.f, zs[nb]);
-            wb[nb][r] = trans8x8(split_h2(see ? p * (sv * w_up) : 0.f));
+            zs[nb] = fmaf(p, fmaf(8.f, sv, par_z(vp[t][r][nb])), zs[nb]);
+            w[r] = p * (sv * w_up);
           }
+          // (hi, lo) of each row's weight side by side, then transposed
+          const __half2 hi = __floats2half2_rn(w[0], w[1]);
+          const float2 back = __half22float2(hi);
+          const __half2 lo = __floats2half2_rn(w[0] - back.x, w[1] - back.y);
+          const uint32_t h2 = *reinterpret_cast<const uint32_t*>(&hi), l2 = *reinterpret_cast<const uint32_t*>(&lo);
+          wb[nb][0] = trans8x8(prmt(h2, l2, 0x5410u));
+          wb[nb][1] = trans8x8(prmt(h2, l2, 0x7632u));
         }
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
@@ -1023,36 +1043,69 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
         // it) and is the first segment (slot 0) of the others
         const float* base = a.part + c_first * 2 * (Q * (HD + 2));
         const int skip = begin_of(c_first) < i0 ? Q * (HD + 2) : 0;
-        for (int e = tid; e < Q * HD / 4; e += kAttnThreads) {
+        // Threads take four dimensions; where that leaves threads over, groups of
+        // them take every G-th part and meet in shared memory. The running maximum
+        // is renewed every kFly parts, which are in flight together: one CTA reads
+        // all of a long context's parts, so it is latency that counts here.
+        constexpr int E = Q * HD / 4, G = E < kAttnThreads ? kAttnThreads / E : 1, kFly = 8;
+        for (int e0 = 0; e0 < E; e0 += kAttnThreads) {
+          const int e = e0 + tid % (E < kAttnThreads ? E : kAttnThreads), grp = tid / E % G;
           const int qq = e / (HD / 4), d = (e - qq * (HD / 4)) * 4;
-          // the running maximum is renewed part by part, four parts in flight
           float M = kNegInf, ls = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int k0 = 0; k0 < parts; k0 += 4) {
-            float2 ml[4];
-            float4 v[4];
+          for (int k0 = grp; k0 < parts; k0 += kFly * G) {
+            float2 ml[kFly];
+            float4 v[kFly];
+            float mn = M;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float* p = base + static_cast<int64_t>(k0 + k) * 2 * (Q * (HD + 2)) + (k0 + k == 0 ? skip : 0);
-              const bool have = k0 + k < parts;
+            for (int k = 0; k < kFly; ++k) {
+              const int part = k0 + k * G;
+              const float* p = base + static_cast<int64_t>(part) * 2 * (Q * (HD + 2)) + (part == 0 ? skip : 0);
+              const bool have = part < parts;
               ml[k] = have ? __ldcg(reinterpret_cast<const float2*>(p + Q * HD + qq * 2))
                            : make_float2(kNegInf, 0.f);
               v[k] = have ? __ldcg(reinterpret_cast<const float4*>(p + qq * HD + d))
                           : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            const float mn = fmaxf(fmaxf(M, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+#pragma unroll
+            for (int k = 0; k < kFly; ++k) mn = fmaxf(mn, ml[k].x);
             const float al = M == kNegInf ? 1.f : ex2(M - mn);   // (sums of 0, or NaN, without a maximum)
             M = mn;
             ls *= al;
             o = make_float4(o.x * al, o.y * al, o.z * al, o.w * al);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < kFly; ++k) {
               const float f = ml[k].x == kNegInf ? 0.f : ex2(ml[k].x - M);
               add(o, f, v[k]);
               ls = fmaf(f, ml[k].y, ls);
             }
           }
-          store(qq, d, o, ls);
+          if constexpr (G == 1) {
+            store(qq, d, o, ls);
+          } else {
+            float4* g_o = reinterpret_cast<float4*>(s_o);             // [G][E]
+            float2* g_ml = reinterpret_cast<float2*>(g_o + G * E);    // [G][E]
+            __syncthreads();
+            g_o[grp * E + e] = o;
+            g_ml[grp * E + e] = make_float2(M, ls);
+            __syncthreads();
+            if (grp == 0) {
+              float mn = M;
+#pragma unroll
+              for (int k = 1; k < G; ++k) mn = fmaxf(mn, g_ml[k * E + e].x);
+              const float al = M == kNegInf ? 1.f : ex2(M - mn);
+              ls *= al;
+              o = make_float4(o.x * al, o.y * al, o.z * al, o.w * al);
+#pragma unroll
+              for (int k = 1; k < G; ++k) {
+                const float2 t = g_ml[k * E + e];
+                const float f = t.x == kNegInf ? 0.f : ex2(t.x - mn);
+                add(o, f, g_o[k * E + e]);
+                ls = fmaf(f, t.y, ls);
+              }
+              store(qq, d, o, ls);
+            }
+          }
         }
         if (tid == 0) a.tickets[c_first] = 0u;   // ready for the next call
       }
