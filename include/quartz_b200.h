@@ -502,6 +502,19 @@ int qz_kv4_append(const void* k, const void* v, int dtype, int64_t k_row_stride,
 int qz_kv4_gather(const uint8_t* pool, int64_t pages, int64_t page_size, int nkv, int hd,
                   const int64_t* slots, int64_t n, float* k, float* v, void* stream);
 
+/*
+ * qz_qk_rope for rows of uneven requests over the paged cache, in one launch:
+ * projection rows qkv [M, (nq + 2 nkv) hd] -> q_out [M, nq hd] (optional per-head
+ * RMSNorm, half-split RoPE at positions[r]) and, normed, rotated and quantised
+ * as by qz_kv4_append, the k and v rows at slots[r]. A negative position counts
+ * as 0; a slot outside the pool stores nothing. (quartz/models/qwen3.py:31-41,
+ * quartz/rope.py:47-78.)
+ */
+int qz_qk_rope_kv4(const float* qkv, const float* q_norm_w, const float* k_norm_w,
+                   const float* inv_freq, float* q_out, int64_t M, int nq, int nkv, int hd,
+                   const int64_t* positions, uint8_t* pool, int64_t pages, int64_t page_size,
+                   const int64_t* slots, float eps, void* stream);
+
 /* Workspace bytes of qz_kv4_attention on the current device (256-byte aligned,
  * zeroed once before its first use and left ready for the next call; calls
  * sharing it must not overlap on the GPU). */

@@ -88,6 +88,8 @@ SIGNATURES = {
     "qz_kv4_append": ([_vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp, _i64, _i64,
                        _vp, _vp], _int),
     "qz_kv4_gather": ([_vp, _i64, _i64, _int, _int, _vp, _i64, _vp, _vp, _vp], _int),
+    "qz_qk_rope_kv4": ([_vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _vp, _vp, _i64, _i64, _vp,
+                        ctypes.c_float, _vp], _int),
     "qz_kv4_attention_workspace_bytes": ([_int, _int, _int, _i64, ctypes.POINTER(_i64)], _int),
     "qz_kv4_attention": ([_vp, _int, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp,
                           _vp, _i64, _i64, _i64, _int, _int, _int, ctypes.c_float, _vp,

@@ -260,28 +260,32 @@ __device__ __forceinline__ uint32_t row_params(float mn, float mx, float& s, flo
   return sb | (zb << 16);
 }
 
-// Codes of 16 values: clamp(round((x - z) / s), 0, 15) of the real quotient,
+// A value's code: clamp(round((x - z) / s), 0, 15) of the real quotient,
 // ties to even. t = (x - z) * (1 / s) in fp32 is within 3 * 2^-24 * |t| < 1e-5
 // of it, so only a t that close to the middle of two codes (1e-4 is taken) is
 // decided again in fp64, where x - z and the comparison lose nothing that
 // matters. Adding 1.5 * 2^23 rounds t to an integer in the low mantissa bits.
-__device__ __forceinline__ uint2 codes16(const float (&x)[16], float s, float z) {
+__device__ __forceinline__ uint32_t code_of(float x, float s, float z, float inv, bool tiny) {
+  float t = __fsub_rn(x, z) * inv;
+  t = fminf(fmaxf(t, 0.f), 15.f);
+  const float r = __fadd_rn(t, 12582912.0f);
+  uint32_t c = __float_as_uint(r) & 15u;
+  if (tiny || fabsf(t - __fsub_rn(r, 12582912.0f)) > 0.4999f) {
+    const double d = rint((static_cast<double>(x) - static_cast<double>(z)) / static_cast<double>(s));
+    c = d >= 15.0 ? 15u : (d > 0.0 ? static_cast<uint32_t>(d) : 0u);
+  }
+  return c;
+}
+
+// Codes of n <= 16 values, value j in bits 4 j ...; zero when s is.
+template <int n>
+__device__ __forceinline__ uint2 codes_of(const float (&x)[n], float s, float z) {
   if (!(s > 0.f)) return make_uint2(0u, 0u);
   const bool tiny = s < 1e-30f;   // 1 / s would overflow
   const float inv = tiny ? 0.f : 1.0f / s;
   uint32_t w[2] = {0u, 0u};
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    float t = __fsub_rn(x[j], z) * inv;
-    t = fminf(fmaxf(t, 0.f), 15.f);
-    const float r = __fadd_rn(t, 12582912.0f);
-    uint32_t c = __float_as_uint(r) & 15u;
-    if (tiny || fabsf(t - __fsub_rn(r, 12582912.0f)) > 0.4999f) {
-      const double d = rint((static_cast<double>(x[j]) - static_cast<double>(z)) / static_cast<double>(s));
-      c = d >= 15.0 ? 15u : (d > 0.0 ? static_cast<uint32_t>(d) : 0u);
-    }
-    w[j >> 3] |= c << (4 * (j & 7));
-  }
+  for (int j = 0; j < n; ++j) w[j >> 3] |= code_of(x[j], s, z, inv, tiny) << (4 * (j & 7));
   return make_uint2(w[0], w[1]);
 }
 
@@ -342,13 +346,105 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     if (!live) continue;
     float s, z;
     const uint32_t par = row_params(mn, mx, s, z);
-    const uint2 c = codes16(x, s, z);
+    const uint2 c = codes_of(x, s, z);
     const int64_t ps = int64_t(1) << a.shift, off = slot & (ps - 1);
     uint8_t* blk = a.pool + ((slot >> a.shift) * a.nkv + h) * (ps * (HD + 8));
     *reinterpret_cast<uint2*>(blk + (is_v ? ps * (HD / 2) : 0) + off * (HD / 2) + lane * 8) = c;
     if (lane == 0)
       *reinterpret_cast<uint32_t*>(blk + ps * HD + (is_v ? ps * 4 : 0) + off * 4) = par;
   }
+}
+
+// q/k norm, RoPE and append of projection rows in one pass
+struct RopeArgs {
+  const float* qkv;        // [M, (nq + 2 nkv) hd]
+  const float* qn_w;       // [hd] or null
+  const float* kn_w;
+  const float* inv_freq;   // [hd / 2]
+  float* q_out;            // [M, nq hd]
+  uint8_t* pool;
+  const int64_t* positions;
+  const int64_t* slots;
+  int64_t m, slots_max;
+  int nq, nkv, shift;
+  float eps;
+};
+
+constexpr int kRopeThreads = 128;
+
+// A warp per (row, head), HD / 32 dimensions a lane: q heads are normed, rotated
+// and written, k heads normed, rotated and quantised, v heads quantised, each
+// straight from the projection (the roped k never goes to memory). The pair of
+// dimension j under the half-split rotation, j +- HD / 2, lies 16 lanes away.
+// Latency-bound at decode sizes (16 rows of 48 heads: 0.4 MB).
+template <int HD>
+__global__ void __launch_bounds__(kRopeThreads) qk_rope_kv4_kernel(const RopeArgs a) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const int heads = a.nq + 2 * a.nkv;
+  pdl_wait();
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (kRopeThreads / 32) + (threadIdx.x >> 5);
+  if (id >= a.m * heads) return;
+  const int64_t row = id / heads;
+  const int head = static_cast<int>(id - row * heads);
+  const bool is_q = head < a.nq, is_v = head >= a.nq + a.nkv;
+  const float* src = a.qkv + (row * heads + head) * HD + lane * E;
+  float x[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) x[j] = src[j];
+  if (!is_v) {
+    const float* w = is_q ? a.qn_w : a.kn_w;
+    if (w) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[j] = x[j] * r * w[lane * E + j];
+    }
+    const int64_t pos = a.positions[row];
+    const float fpos = static_cast<float>(pos < 0 ? 0 : pos);
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float ang = fpos * a.inv_freq[(lane * E + j) & (HD / 2 - 1)];
+      const float c = cosf(ang), s = sinf(ang);
+      const float y = __shfl_xor_sync(0xffffffffu, x[j], 16);
+      x[j] = lane < 16 ? x[j] * c - y * s : x[j] * c + y * s;
+    }
+  }
+  if (is_q) {
+    float* dst = a.q_out + (row * a.nq + head) * HD + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; ++j) dst[j] = x[j];
+    return;
+  }
+  const int64_t slot = a.slots[row];
+  if (slot < 0 || slot >= a.slots_max) return;
+  float mn = x[0], mx = x[0];
+#pragma unroll
+  for (int j = 1; j < E; ++j) {
+    mn = min_nan(mn, x[j]);
+    mx = max_nan(mx, x[j]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  float s, z;
+  const uint32_t par = row_params(mn, mx, s, z);
+  const uint32_t c = codes_of(x, s, z).x;
+  const int h = head - a.nq - (is_v ? a.nkv : 0);
+  const int64_t ps = int64_t(1) << a.shift, off = slot & (ps - 1);
+  uint8_t* blk = a.pool + ((slot >> a.shift) * a.nkv + h) * (ps * (HD + 8));
+  uint8_t* at = blk + (is_v ? ps * (HD / 2) : 0) + off * (HD / 2) + lane * (E / 2);
+  if constexpr (E == 4)
+    *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(c);
+  else
+    *at = static_cast<uint8_t>(c);
+  if (lane == 0) *reinterpret_cast<uint32_t*>(blk + ps * HD + (is_v ? ps * 4 : 0) + off * 4) = par;
 }
 
 struct GatherArgs {

@@ -199,6 +199,30 @@ int qz_kv4_gather(const uint8_t* pool, int64_t pages, int64_t page_size, int nkv
                   : launch_kv4(qz::kv4::gather_kernel<128>, grid, qz::kv4::kGatherThreads, 0, st, a);
 }
 
+int qz_qk_rope_kv4(const float* qkv, const float* q_norm_w, const float* k_norm_w,
+                   const float* inv_freq, float* q_out, int64_t M, int nq, int nkv, int hd,
+                   const int64_t* positions, uint8_t* pool, int64_t pages, int64_t page_size,
+                   const int64_t* slots, float eps, void* stream) {
+  if (int rc = check_kv4_heads(nq, nkv, "qz_qk_rope_kv4")) return rc;
+  if (int rc = check_kv4_pool(pool, pages, page_size, nkv, hd, "qz_qk_rope_kv4")) return rc;
+  if (M < 0 || M > (int64_t(1) << 32) / (nq + 2 * nkv))
+    return fail(QZ_ERR_INVALID, "qz_qk_rope_kv4: bad row count");
+  if ((q_norm_w == nullptr) != (k_norm_w == nullptr))
+    return fail(QZ_ERR_INVALID, "qz_qk_rope_kv4: pass both norm weights or neither");
+  if (M == 0) return QZ_OK;
+  if (!qkv || !inv_freq || !q_out || !positions || !slots)
+    return fail(QZ_ERR_INVALID, "qz_qk_rope_kv4: null pointer");
+  DeviceInfo* d = nullptr;
+  if (int rc = device_info(&d)) return rc;
+  const qz::kv4::RopeArgs a{qkv, q_norm_w, k_norm_w, inv_freq, q_out, pool, positions, slots, M,
+                            pages * page_size, nq, nkv, page_shift(page_size), eps};
+  const int64_t warps = M * (nq + 2 * nkv);
+  const int grid = static_cast<int>(qz::cdiv(warps, qz::kv4::kRopeThreads / 32));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return hd == 64 ? launch_kv4(qz::kv4::qk_rope_kv4_kernel<64>, grid, qz::kv4::kRopeThreads, 0, st, a)
+                  : launch_kv4(qz::kv4::qk_rope_kv4_kernel<128>, grid, qz::kv4::kRopeThreads, 0, st, a);
+}
+
 int qz_kv4_attention_workspace_bytes(int nq, int nkv, int hd, int64_t max_rows, int64_t* bytes) {
   if (!bytes) return fail(QZ_ERR_INVALID, "qz_kv4_attention_workspace_bytes: null pointer");
   if (int rc = check_kv4_heads(nq, nkv, "qz_kv4_attention_workspace_bytes")) return rc;

@@ -112,37 +112,17 @@ def quartz_checkpoint(net) -> tuple[ModelSpec, dict, dict]:
     return spec, int8, norms
 
 
-class DecodeEngine:
-    """Device-resident all-int8 decoder for one sequence.
+class _Int8Weights:
+    """The device-resident int8 checkpoint an engine runs on, and its GEMMs.
+    Subclasses set spec, dev and lib first, and gemm_ws, xn, act and fold_norms
+    before they call _gemm_act."""
 
-    weights: name -> (q int8 [out, in], scale fp32 [out, ng]) for every Linear
-    and the embedding (names as quartz.model.leaf_names), name -> fp32 vector for
-    the RMSNorms (quartz.model.norm_weights). Iterables of (name, q, scale) are
-    accepted for the int8 tensors so a large checkpoint streams to the device.
-    """
-
-    def __init__(self, spec: ModelSpec, int8_weights: Mapping | Iterable, norms: Mapping,
-                 *, max_ctx: int, max_prefill: int = 512, device=None,
-                 persistent: bool = False, fold_norms: bool = True, batch: int = 1):
-        """batch: sequences decoded in lockstep (quartz's decode_logits on [B, 1]
-        ids, quartz/models/common.py:79-88): every step runs B rows through the
-        int8 GEMMs (M = B, quartz/kernels/int8.py:66-87, 106-107), the per-op
-        MLP (quartz/quantize.py:112-114) and a batched attention over B caches
-        sharing one position. batch > 1 decodes through generate_batch and has
-        no prefill (sequences start from a loaded cache)."""
-        self.spec = spec
-        self.batch = int(batch)
-        if self.batch < 1:
-            raise ValueError("batch must be >= 1")
-        if self.batch > 1:
-            persistent = False
-        self.dev = torch.device("cuda", qd.ensure_device(device))
-        dev = self.dev
-        self.lib = _lib.load()
-        self.max_ctx = int(max_ctx)
-        self.max_prefill = max(1, int(max_prefill))
-        S = spec
-        H, hd = S.hidden, S.head_dim
+    def _load_weights(self, int8_weights: Mapping | Iterable, norms: Mapping) -> None:
+        """name -> (q int8 [out, in], scale fp32 [out, ng]) for every Linear and the
+        embedding (or an iterable of (name, q, scale)), name -> fp32 vector for the
+        RMSNorms."""
+        dev, S = self.dev, self.spec
+        hd = S.head_dim
         self.layers = [_Layer() for _ in range(S.layers)]
         self.embed_q = self.embed_s = self.lm_q = self.lm_s = None
         leaves = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
@@ -202,6 +182,66 @@ class DecodeEngine:
         self.inv_freq = _dev_f32(rope_inv_freq(S), dev)
         self.attn_scale = float(hd ** -0.5)
         self.ng = self.layers[0].qkv_s.shape[1] if self.layers else 1
+
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.dev).cuda_stream
+
+    def _gemm_act(self, q, s, x: int, act: int, norm_w: int | None, y: int, M: int, N: int,
+                  K: int, residual: int | None, st: int) -> None:
+        """The int8 GEMM of M > 1 rows on an activation of x: its RMSNorm
+        (act QZ_ACT_RMSNORM, weight norm_w) or silu(g) * u of its [g | u] rows
+        (QZ_ACT_SILU_MUL). With fold_norms and a tensor-path shape the
+        activation is computed inside the GEMM's limb split (one kernel less);
+        otherwise qz_rmsnorm / qz_silu_mul write it first. Both give the same
+        values."""
+        lib, chk = self.lib, _lib.check
+        ws, wsb = self.gemm_ws.data_ptr(), self.gemm_ws.numel()
+        if self.fold_norms and s.shape[1] == 1 and K % 16 == 0:
+            chk(lib.qz_gemm_w8_act_ws(q.data_ptr(), s.data_ptr(), 1, x, act, norm_w,
+                                      self.spec.eps, y, M, N, K, residual, ws, wsb, st))
+            return
+        if act == _lib.QZ_ACT_RMSNORM:
+            chk(lib.qz_rmsnorm(x, norm_w, self.xn.data_ptr(), M, K, self.spec.eps, st))
+            src = self.xn.data_ptr()
+        else:
+            chk(lib.qz_silu_mul(x, self.act.data_ptr(), M, K, st))
+            src = self.act.data_ptr()
+        chk(lib.qz_gemm_w8_ws(q.data_ptr(), s.data_ptr(), s.shape[1], src, y, M, N, K, residual,
+                              ws, wsb, st))
+
+
+class DecodeEngine(_Int8Weights):
+    """Device-resident all-int8 decoder for one sequence.
+
+    weights: name -> (q int8 [out, in], scale fp32 [out, ng]) for every Linear
+    and the embedding (names as quartz.model.leaf_names), name -> fp32 vector for
+    the RMSNorms (quartz.model.norm_weights). Iterables of (name, q, scale) are
+    accepted for the int8 tensors so a large checkpoint streams to the device.
+    """
+
+    def __init__(self, spec: ModelSpec, int8_weights: Mapping | Iterable, norms: Mapping,
+                 *, max_ctx: int, max_prefill: int = 512, device=None,
+                 persistent: bool = False, fold_norms: bool = True, batch: int = 1):
+        """batch: sequences decoded in lockstep (quartz's decode_logits on [B, 1]
+        ids, quartz/models/common.py:79-88): every step runs B rows through the
+        int8 GEMMs (M = B, quartz/kernels/int8.py:66-87, 106-107), the per-op
+        MLP (quartz/quantize.py:112-114) and a batched attention over B caches
+        sharing one position. batch > 1 decodes through generate_batch and has
+        no prefill (sequences start from a loaded cache)."""
+        self.spec = spec
+        self.batch = int(batch)
+        if self.batch < 1:
+            raise ValueError("batch must be >= 1")
+        if self.batch > 1:
+            persistent = False
+        self.dev = torch.device("cuda", qd.ensure_device(device))
+        dev = self.dev
+        self.lib = _lib.load()
+        self.max_ctx = int(max_ctx)
+        self.max_prefill = max(1, int(max_prefill))
+        S = spec
+        H, hd = S.hidden, S.head_dim
+        self._load_weights(int8_weights, norms)
 
         # KV cache and activation buffers
         f32 = dict(dtype=torch.float32, device=dev)
@@ -327,9 +367,6 @@ class DecodeEngine:
         self.reset(T)
 
     # ------------------------------------------------------------- the token
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
     def _decode_ops(self, st: int) -> None:
         """One token at position *pos_dev: reads self.tok, writes self.tok and
         advances pos_dev. Every call is a libquartz_b200 launch on stream st."""
@@ -392,29 +429,6 @@ class DecodeEngine:
                                p(self.logits), S.vocab, H, None, st))
         chk(lib.qz_argmax(p(self.logits), 1, S.vocab, p(self.keys), p(self.tok), p(self.pos_dev),
                           1, st))
-
-    def _gemm_act(self, q, s, x: int, act: int, norm_w: int | None, y: int, M: int, N: int,
-                  K: int, residual: int | None, st: int) -> None:
-        """The int8 GEMM of M > 1 rows on an activation of x: its RMSNorm
-        (act QZ_ACT_RMSNORM, weight norm_w) or silu(g) * u of its [g | u] rows
-        (QZ_ACT_SILU_MUL). With fold_norms and a tensor-path shape the
-        activation is computed inside the GEMM's limb split (one kernel less);
-        otherwise qz_rmsnorm / qz_silu_mul write it first. Both give the same
-        values."""
-        lib, chk = self.lib, _lib.check
-        ws, wsb = self.gemm_ws.data_ptr(), self.gemm_ws.numel()
-        if self.fold_norms and s.shape[1] == 1 and K % 16 == 0:
-            chk(lib.qz_gemm_w8_act_ws(q.data_ptr(), s.data_ptr(), 1, x, act, norm_w,
-                                      self.spec.eps, y, M, N, K, residual, ws, wsb, st))
-            return
-        if act == _lib.QZ_ACT_RMSNORM:
-            chk(lib.qz_rmsnorm(x, norm_w, self.xn.data_ptr(), M, K, self.spec.eps, st))
-            src = self.xn.data_ptr()
-        else:
-            chk(lib.qz_silu_mul(x, self.act.data_ptr(), M, K, st))
-            src = self.act.data_ptr()
-        chk(lib.qz_gemm_w8_ws(q.data_ptr(), s.data_ptr(), s.shape[1], src, y, M, N, K, residual,
-                              ws, wsb, st))
 
     def _batch_layer_attn(self, li: int, L, st: int) -> None:
         """RMSNorm, q/k/v GEMM and the batched attention of layer li for the

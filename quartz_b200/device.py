@@ -28,6 +28,7 @@ over one pool of pages. ``quartz_b200.paged`` decodes with it.
                                                block tables, slots, positions
     kv4_append(k, v, pool, slots)              quantise and store rows
     kv4_gather(pool, slots, hd)  -> k, v       the values the rows stand for
+    qk_rope_kv4(qkv, ...)        -> q          q/k norm, RoPE and append in one launch
     kv4_attention(q, pool, table, lens, ...)   one row, a few rows or a prompt
 """
 
@@ -733,6 +734,46 @@ def kv4_gather(pool, slots, head_dim, out=None):
             pool.data_ptr(), pool.shape[0], ps, nkv, int(head_dim), slots.data_ptr(), n,
             k.data_ptr(), v.data_ptr(), _stream_ptr(dev)))
     return k, v
+
+
+def qk_rope_kv4(qkv, inv_freq, positions, pool, slots, n_heads, q_norm=None, k_norm=None,
+                eps=1e-6, q_out=None):
+    """Split projection rows qkv [M, (nq + 2 nkv) hd] (fp32) into q, normed and rotated at
+    positions [M] (returned as [M, nq, hd]), and the k and v rows, which are stored
+    in the paged cache at slots [M] as kv4_append would."""
+    hd = 2 * inv_freq.numel()
+    ps = _kv4_page_size(pool, hd)
+    nkv = pool.shape[1]
+    _need(qkv, torch.float32, "qkv", 2)
+    _need(inv_freq, torch.float32, "inv_freq", 1)
+    _need(positions, torch.int64, "positions", 1)
+    _need(slots, torch.int64, "slots", 1)
+    M = qkv.shape[0]
+    if qkv.shape[1] != (n_heads + 2 * nkv) * hd:
+        raise ValueError(f"qkv rows must have {(n_heads + 2 * nkv) * hd} elements")
+    if positions.numel() != M or slots.numel() != M:
+        raise ValueError(f"positions and slots must have one element per row ({M})")
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("pass both q_norm and k_norm or neither")
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is not None:
+            _need(t, torch.float32, name, 1)
+            if t.numel() != hd:
+                raise ValueError(f"{name} must have head_dim elements")
+    dev = pool.device
+    ensure_device(dev)
+    if q_out is None:
+        q_out = torch.empty((M, n_heads, hd), dtype=torch.float32, device=dev)
+    _need(q_out, torch.float32, "q_out")
+    if q_out.numel() != M * n_heads * hd:
+        raise ValueError("q_out must hold M * n_heads * head_dim elements")
+    _same_device(dev, qkv, inv_freq, positions, slots, q_norm, k_norm, q_out)
+    with _on(dev):
+        _lib.check(_lib.load().qz_qk_rope_kv4(
+            qkv.data_ptr(), _ptr(q_norm), _ptr(k_norm), inv_freq.data_ptr(), q_out.data_ptr(), M,
+            n_heads, nkv, hd, positions.data_ptr(), pool.data_ptr(), pool.shape[0], ps,
+            slots.data_ptr(), float(eps), _stream_ptr(dev)))
+    return q_out
 
 
 def kv4_attention_workspace(device, n_heads: int, n_kv: int, head_dim: int, max_rows: int = 1

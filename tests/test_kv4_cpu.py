@@ -29,6 +29,13 @@ def _append(**kw):
     return _lib().load().qz_kv4_append(*a.values())
 
 
+def _rope(**kw):
+    a = dict(qkv=P16, qn=None, kn=None, inv=P16, q_out=P16, M=4, nq=4, nkv=2, hd=64, pos=P16,
+             pool=P16, pages=9, page=16, slots=P16, eps=1e-6, stream=None)
+    a.update(kw)
+    return _lib().load().qz_qk_rope_kv4(*a.values())
+
+
 def _gather(**kw):
     a = dict(pool=P16, pages=9, page=16, nkv=2, hd=64, slots=P16, n=4, k=P16, v=P16, stream=None)
     a.update(kw)
@@ -55,6 +62,9 @@ def _attend(**kw):
     (_append, dict(pool=None), "pool"), (_append, dict(pool=P16 + 8), "pool"),
     (_append, dict(dtype=3), "dtype"), (_append, dict(n=-1), "row count"),
     (_append, dict(k=None), "null pointer"), (_append, dict(slots=None), "null pointer"),
+    (_rope, dict(nq=3), "multiple"), (_rope, dict(hd=32), "head_dim"), (_rope, dict(M=-1), "row count"),
+    (_rope, dict(qn=P16), "both norm weights"), (_rope, dict(pos=None), "null pointer"),
+    (_rope, dict(page=0), "page size"),
     (_gather, dict(hd=256), "head_dim"), (_gather, dict(k=P16 + 4), "16-byte"),
     (_gather, dict(v=None), "null pointer"), (_gather, dict(n=-1), "row count"),
     (_attend, dict(nq=5), "multiple"), (_attend, dict(nq=0), "multiple"),
