@@ -34,6 +34,19 @@ int launch_kv4(void (*fn)(A), int grid, int threads, int smem, cudaStream_t st, 
   return QZ_OK;
 }
 
+// The dynamic shared memory of `fn`, allowed once per device.
+template <class F>
+int allow_smem_once(F* fn, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  QZ_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = uint64_t(1) << (dev & 63);      // device_info() refuses devices beyond 64
+  if (!(done.load(std::memory_order_acquire) & bit)) {
+    QZ_CUDA(allow_smem(fn, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+  }
+  return QZ_OK;
+}
+
 // log2 of a page size the kernels take (16 .. 256, a power of two), else -1.
 int page_shift(int64_t page_size) {
   for (int s = 4; s <= 8; ++s)
@@ -70,7 +83,7 @@ bool rows_aligned(const void* p, int64_t rs, int64_t hs, int dtype) {
 template <class T>
 int launch_append(const DeviceInfo& d, int hd, const qz::kv4::AppendArgs& a, cudaStream_t st) {
   const int per_block = qz::kv4::kAppendThreads / (hd / 16);
-  const int64_t want = qz::cdiv(a.n * a.nkv * 2, per_block);
+  const int64_t want = qz::cdiv(a.n * a.nkv, per_block);
   const int grid = static_cast<int>(std::min<int64_t>(want, int64_t(d.sms) * 8));
   return hd == 64 ? launch_kv4(qz::kv4::append_kernel<T, 64>, grid, qz::kv4::kAppendThreads, 0, st, a)
                   : launch_kv4(qz::kv4::append_kernel<T, 128>, grid, qz::kv4::kAppendThreads, 0, st, a);
@@ -97,7 +110,9 @@ Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int nb, int hd) {
 
 template <class T, int HD, int NB>
 int launch_kv4_attn(const qz::kv4::AttnArgs& a, int grid, cudaStream_t st) {
-  QZ_CUDA(allow_smem(qz::kv4::attn_kernel<T, HD, NB>, qz::kv4::attn_smem<HD, NB>()));
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow_smem_once(qz::kv4::attn_kernel<T, HD, NB>, qz::kv4::attn_smem<HD, NB>(), done))
+    return rc;
   return launch_kv4(qz::kv4::attn_kernel<T, HD, NB>, grid, qz::kv4::kAttnThreads,
                     qz::kv4::attn_smem<HD, NB>(), st, a);
 }
@@ -119,7 +134,8 @@ int64_t split_rows(int group) {
 template <class T, int HD>
 int launch_kv4_tc(const qz::kv4::TcArgs& a, int64_t grid, cudaStream_t st) {
   constexpr int smem = qz::kv4::tc_smem<HD>();
-  QZ_CUDA(allow_smem(qz::kv4::attn_tc_kernel<T, HD>, smem));
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow_smem_once(qz::kv4::attn_tc_kernel<T, HD>, smem, done)) return rc;
   return launch_kv4(qz::kv4::attn_tc_kernel<T, HD>, static_cast<int>(grid), qz::kv4::kTcThreads,
                     smem, st, a);
 }
@@ -191,9 +207,9 @@ int qz_kv4_gather(const uint8_t* pool, int64_t pages, int64_t page_size, int nkv
   DeviceInfo* d = nullptr;
   if (int rc = device_info(&d)) return rc;
   const qz::kv4::GatherArgs a{pool, slots, k, v, n, pages * page_size, nkv, page_shift(page_size)};
-  const int per_block = qz::kv4::kGatherThreads / (hd / 4);
+  const int per_block = qz::kv4::kGatherThreads / (hd / 4) * qz::kv4::kGatherFly;
   const int grid = static_cast<int>(
-      std::min<int64_t>(qz::cdiv(n * nkv * 2, per_block), int64_t(d->sms) * 8));
+      std::min<int64_t>(qz::cdiv(n * nkv, per_block), int64_t(d->sms) * 8));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return hd == 64 ? launch_kv4(qz::kv4::gather_kernel<64>, grid, qz::kv4::kGatherThreads, 0, st, a)
                   : launch_kv4(qz::kv4::gather_kernel<128>, grid, qz::kv4::kGatherThreads, 0, st, a);

@@ -48,14 +48,23 @@ _mlp_ws: dict[int, torch.Tensor] = {}
 _gemm_ws: dict[int, torch.Tensor] = {}
 
 
+# The current stream's raw handle without building a torch.cuda.Stream object
+# (a few microseconds of host time in every call).
+_raw_stream_fn = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(dev: torch.device) -> int:
+    if _raw_stream_fn is not None and dev.index is not None:
+        return _raw_stream_fn(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 
 def ensure_device(dev: torch.device | int | None = None) -> int:
     """qz_init once per device (checks that it is an sm_100 GPU)."""
-    if dev is None and _ready_devices:
-        idx = torch.cuda.current_device()   # the per-call path: no availability probe
+    if _ready_devices:                      # the per-call path: no availability probe
+        idx = dev.index if isinstance(dev, torch.device) else dev
+        if idx is None:
+            idx = torch.cuda.current_device()
         if idx in _ready_devices:
             return idx
     if not torch.cuda.is_available():
@@ -578,12 +587,12 @@ class KV4Plan(NamedTuple):
 
 
 class _on:
-    """Makes the tensors' device current for a library call (nothing to do in
-    the usual case that it is)."""
+    """Makes a device current for a library call (nothing to do in the usual case
+    that it is)."""
     __slots__ = ("idx", "prev")
 
-    def __init__(self, dev: torch.device):
-        self.idx = dev.index
+    def __init__(self, idx: int):
+        self.idx = idx
 
     def __enter__(self):
         self.prev = torch.cuda.current_device()
@@ -593,6 +602,28 @@ class _on:
     def __exit__(self, *exc):
         if self.prev != self.idx:
             torch.cuda.set_device(self.prev)
+
+
+def _arg(t, dtype, name: str, ndim: int, idx: int) -> None:
+    """A contiguous tensor of dtype and ndim on GPU idx: one condition in the usual
+    case, _need and _same_device to say what is wrong. (These calls take a few
+    microseconds of GPU time at decode sizes, about what their checks do.)"""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == ndim
+            and t.get_device() == idx and t.is_contiguous()):
+        _need(t, dtype, name, ndim)
+        _same_device(torch.device("cuda", idx), t)
+
+
+def _home(t, name: str) -> int:
+    """The index of the GPU a tensor is on, which the call then runs on."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    idx = t.get_device()
+    if idx not in _ready_devices:
+        ensure_device(idx)
+    return idx
 
 
 def kv4_block_bytes(page_size: int, head_dim: int) -> int:
@@ -611,29 +642,37 @@ def kv4_pool(pages: int, n_kv: int, head_dim: int, page_size: int, device=None) 
                        device=torch.device("cuda", ensure_device(device)))
 
 
-def _kv4_page_size(pool: torch.Tensor, head_dim: int) -> int:
+_kv4_ps: dict[tuple[int, int], int] = {
+    (qz_ps * (qz_hd + 8), qz_hd): qz_ps for qz_ps in KV4_PAGE_SIZES for qz_hd in KV4_HEAD_DIMS}
+
+
+def _kv4_page_size(pool: torch.Tensor, head_dim: int, idx: int) -> int:
     """The page size of a pool (checked against head_dim)."""
-    if head_dim not in KV4_HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {KV4_HEAD_DIMS}, got {head_dim}")
-    _need(pool, torch.uint8, "pool", 3)
-    ps, rest = divmod(pool.shape[2], head_dim + 8)
-    if rest or ps not in KV4_PAGE_SIZES:
+    _arg(pool, torch.uint8, "pool", 3, idx)
+    ps = _kv4_ps.get((pool.shape[2], head_dim))
+    if ps is None:
+        if head_dim not in KV4_HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {KV4_HEAD_DIMS}, got {head_dim}")
         raise ValueError(f"pool blocks of {pool.shape[2]} bytes are no pages of head_dim {head_dim}")
     return ps
 
 
-def _kv4_rows(t: torch.Tensor, name: str) -> None:
-    """Rows [n, heads, head_dim] on the GPU, any strides with contiguous head_dim."""
+def _kv4_rows(t: torch.Tensor, name: str, idx: int) -> tuple[int, int, int]:
+    """Shape of rows [n, heads, head_dim] on GPU idx, any strides with contiguous
+    head_dim."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in _KV4_DTYPES:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() != 3:
         raise ValueError(f"{name} must be [rows, heads, head_dim], got shape {tuple(t.shape)}")
+    if t.get_device() != idx:
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        _same_device(torch.device("cuda", idx), t)
     if t.stride(2) != 1:
         raise ValueError(f"{name} must be contiguous along head_dim")
+    return t.shape
 
 
 def kv4_plan(lens, new_rows, block_table, free_pages, used, page_size, rows, lens_out=None,
@@ -648,11 +687,12 @@ def kv4_plan(lens, new_rows, block_table, free_pages, used, page_size, rows, len
     do not fit W, or for which the free pages do not last (counted in order)
     keeps its length and gets slots -1. lens_out / used_out may be lens / used
     themselves (a step captured in a CUDA graph then advances them)."""
-    _need(lens, torch.int64, "lens", 1)
-    _need(new_rows, torch.int64, "new_rows", 1)
-    _need(block_table, torch.int32, "block_table", 2)
-    _need(free_pages, torch.int32, "free_pages", 1)
-    _need(used, torch.int64, "used")
+    idx = _home(lens, "lens")
+    _arg(lens, torch.int64, "lens", 1, idx)
+    _arg(new_rows, torch.int64, "new_rows", 1, idx)
+    _arg(block_table, torch.int32, "block_table", 2, idx)
+    _arg(free_pages, torch.int32, "free_pages", 1, idx)
+    _arg(used, torch.int64, "used", 1, idx)
     B, W = block_table.shape
     rows = int(rows)
     if lens.numel() != B or new_rows.numel() != B:
@@ -661,27 +701,25 @@ def kv4_plan(lens, new_rows, block_table, free_pages, used, page_size, rows, len
         raise ValueError("used must have one element")
     if rows < 0:
         raise ValueError("rows must not be negative")
-    dev = lens.device
-    ensure_device(dev)
-    buf = torch.empty(2 * B + 2 + 2 * rows, dtype=torch.int64, device=dev)
-    cu, lo, uo, slots, positions = buf.split((B + 1, B, 1, rows, rows))
+    buf = torch.empty(2 * B + 2 + 2 * rows, dtype=torch.int64, device=lens.device)
+    cu, lo, uo, slots, positions = torch.unsafe_split_with_sizes(buf, (B + 1, B, 1, rows, rows))
     if lens_out is not None:
-        _need(lens_out, torch.int64, "lens_out", 1)
+        _arg(lens_out, torch.int64, "lens_out", 1, idx)
         if lens_out.numel() != B:
             raise ValueError(f"lens_out must have {B} elements")
         lo = lens_out
     if used_out is not None:
-        _need(used_out, torch.int64, "used_out")
+        _arg(used_out, torch.int64, "used_out", 1, idx)
         if used_out.numel() != 1:
             raise ValueError("used_out must have one element")
         uo = used_out
-    _same_device(dev, new_rows, block_table, free_pages, used, lo, uo)
-    with _on(dev):
+    at = buf.data_ptr()                    # the parts lie one behind the other
+    with _on(idx):
         _lib.check(_lib.load().qz_kv4_plan(
             lens.data_ptr(), new_rows.data_ptr(), B, block_table.data_ptr(), W,
-            free_pages.data_ptr(), free_pages.numel(), used.data_ptr(), int(page_size), rows,
-            cu.data_ptr(), lo.data_ptr(), uo.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-            _stream_ptr(dev)))
+            free_pages.data_ptr(), free_pages.numel(), used.data_ptr(), int(page_size), rows, at,
+            lo.data_ptr(), uo.data_ptr(), at + 8 * (2 * B + 2), at + 8 * (2 * B + 2 + rows),
+            _stream_ptr(lens.device)))
     return KV4Plan(cu, lo, uo, slots, positions)
 
 
@@ -691,48 +729,47 @@ def kv4_append(k, v, pool, slots) -> None:
     (int64 [n]; a slot outside the pool stores nothing). Each row of a kv head
     keeps its own bf16 step and zero; a row with a non-finite value reads back
     as NaN. A slot must not appear twice in one call."""
-    _kv4_rows(k, "k")
-    _kv4_rows(v, "v")
-    if k.shape != v.shape or k.dtype != v.dtype:
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise TypeError("k and v must be torch.Tensors")
+    idx = _home(pool, "pool")
+    n, nkv, hd = _kv4_rows(k, "k", idx)
+    _kv4_rows(v, "v", idx)
+    if k.shape != v.shape or k.dtype is not v.dtype:
         raise ValueError("k and v must have the same shape and dtype")
-    n, nkv, hd = k.shape
-    ps = _kv4_page_size(pool, hd)
+    ps = _kv4_page_size(pool, hd, idx)
     if pool.shape[1] != nkv:
         raise ValueError(f"pool has {pool.shape[1]} kv heads, k has {nkv}")
-    _need(slots, torch.int64, "slots", 1)
+    _arg(slots, torch.int64, "slots", 1, idx)
     if slots.numel() != n:
         raise ValueError(f"slots must have one element per row ({n})")
-    dev = pool.device
-    ensure_device(dev)
-    _same_device(dev, k, v, slots)
-    with _on(dev):
+    ks, vs = k.stride(), v.stride()
+    with _on(idx):
         _lib.check(_lib.load().qz_kv4_append(
-            k.data_ptr(), v.data_ptr(), _KV4_DTYPES[k.dtype], k.stride(0), k.stride(1),
-            v.stride(0), v.stride(1), n, nkv, hd, pool.data_ptr(), pool.shape[0], ps,
-            slots.data_ptr(), _stream_ptr(dev)))
+            k.data_ptr(), v.data_ptr(), _KV4_DTYPES[k.dtype], ks[0], ks[1], vs[0], vs[1], n, nkv,
+            hd, pool.data_ptr(), pool.shape[0], ps, slots.data_ptr(), _stream_ptr(pool.device)))
 
 
 def kv4_gather(pool, slots, head_dim, out=None):
     """(k, v) fp32 [n, n_kv, head_dim]: the values at slots (int64 [n]); zeros
     for a slot outside the pool. out: a pair of contiguous tensors to write."""
-    ps = _kv4_page_size(pool, int(head_dim))
-    _need(slots, torch.int64, "slots", 1)
-    dev = pool.device
-    ensure_device(dev)
+    idx = _home(pool, "pool")
+    hd = int(head_dim)
+    ps = _kv4_page_size(pool, hd, idx)
+    _arg(slots, torch.int64, "slots", 1, idx)
     n, nkv = slots.numel(), pool.shape[1]
     if out is None:
-        k, v = torch.empty((2, n, nkv, head_dim), dtype=torch.float32, device=dev).unbind(0)
+        k = torch.empty((n, nkv, hd), dtype=torch.float32, device=pool.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for t, name in ((k, "out[0]"), (v, "out[1]")):
-            _need(t, torch.float32, name, 3)
-            if tuple(t.shape) != (n, nkv, head_dim):
-                raise ValueError(f"{name} must be [{n}, {nkv}, {head_dim}], got {tuple(t.shape)}")
-    _same_device(dev, slots, k, v)
-    with _on(dev):
+            _arg(t, torch.float32, name, 3, idx)
+            if tuple(t.shape) != (n, nkv, hd):
+                raise ValueError(f"{name} must be [{n}, {nkv}, {hd}], got {tuple(t.shape)}")
+    with _on(idx):
         _lib.check(_lib.load().qz_kv4_gather(
-            pool.data_ptr(), pool.shape[0], ps, nkv, int(head_dim), slots.data_ptr(), n,
-            k.data_ptr(), v.data_ptr(), _stream_ptr(dev)))
+            pool.data_ptr(), pool.shape[0], ps, nkv, hd, slots.data_ptr(), n, k.data_ptr(),
+            v.data_ptr(), _stream_ptr(pool.device)))
     return k, v
 
 
@@ -741,13 +778,14 @@ def qk_rope_kv4(qkv, inv_freq, positions, pool, slots, n_heads, q_norm=None, k_n
     """Split projection rows qkv [M, (nq + 2 nkv) hd] (fp32) into q, normed and rotated at
     positions [M] (returned as [M, nq, hd]), and the k and v rows, which are stored
     in the paged cache at slots [M] as kv4_append would."""
+    idx = _home(pool, "pool")
+    _arg(inv_freq, torch.float32, "inv_freq", 1, idx)
     hd = 2 * inv_freq.numel()
-    ps = _kv4_page_size(pool, hd)
+    ps = _kv4_page_size(pool, hd, idx)
     nkv = pool.shape[1]
-    _need(qkv, torch.float32, "qkv", 2)
-    _need(inv_freq, torch.float32, "inv_freq", 1)
-    _need(positions, torch.int64, "positions", 1)
-    _need(slots, torch.int64, "slots", 1)
+    _arg(qkv, torch.float32, "qkv", 2, idx)
+    _arg(positions, torch.int64, "positions", 1, idx)
+    _arg(slots, torch.int64, "slots", 1, idx)
     M = qkv.shape[0]
     if qkv.shape[1] != (n_heads + 2 * nkv) * hd:
         raise ValueError(f"qkv rows must have {(n_heads + 2 * nkv) * hd} elements")
@@ -757,22 +795,22 @@ def qk_rope_kv4(qkv, inv_freq, positions, pool, slots, n_heads, q_norm=None, k_n
         raise ValueError("pass both q_norm and k_norm or neither")
     for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if t is not None:
-            _need(t, torch.float32, name, 1)
+            _arg(t, torch.float32, name, 1, idx)
             if t.numel() != hd:
                 raise ValueError(f"{name} must have head_dim elements")
-    dev = pool.device
-    ensure_device(dev)
     if q_out is None:
-        q_out = torch.empty((M, n_heads, hd), dtype=torch.float32, device=dev)
-    _need(q_out, torch.float32, "q_out")
+        q_out = torch.empty((M, n_heads, hd), dtype=torch.float32, device=pool.device)
+    elif not (isinstance(q_out, torch.Tensor) and q_out.dtype is torch.float32
+              and q_out.get_device() == idx and q_out.is_contiguous()):
+        _need(q_out, torch.float32, "q_out")
+        _same_device(pool.device, q_out)
     if q_out.numel() != M * n_heads * hd:
         raise ValueError("q_out must hold M * n_heads * head_dim elements")
-    _same_device(dev, qkv, inv_freq, positions, slots, q_norm, k_norm, q_out)
-    with _on(dev):
+    with _on(idx):
         _lib.check(_lib.load().qz_qk_rope_kv4(
             qkv.data_ptr(), _ptr(q_norm), _ptr(k_norm), inv_freq.data_ptr(), q_out.data_ptr(), M,
             n_heads, nkv, hd, positions.data_ptr(), pool.data_ptr(), pool.shape[0], ps,
-            slots.data_ptr(), float(eps), _stream_ptr(dev)))
+            slots.data_ptr(), float(eps), _stream_ptr(pool.device)))
     return q_out
 
 
@@ -792,7 +830,7 @@ def _kv4_ws_bytes(idx: int, nq: int, nkv: int, hd: int, max_rows: int) -> int:
     need = _kv4_ws_need.get(key)
     if need is None:
         b = ctypes.c_int64(0)
-        with _on(torch.device("cuda", idx)):
+        with _on(idx):
             _lib.check(_lib.load().qz_kv4_attention_workspace_bytes(nq, nkv, hd, max_rows,
                                                                     ctypes.byref(b)))
         if len(_kv4_ws_need) > 4096:
@@ -801,15 +839,16 @@ def _kv4_ws_bytes(idx: int, nq: int, nkv: int, hd: int, max_rows: int) -> int:
     return need
 
 
-def _kv4_default_ws(dev: torch.device, stream: int, need: int) -> torch.Tensor:
+def _kv4_default_ws(idx: int, stream: int, need: int) -> torch.Tensor:
     """The workspace of a call that brings none: one per device and stream. A call
     under stream capture gets its own, so that two graphs (or a graph and eager
     calls) never share one."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=dev)
-    ws = _kv4_ws.get((dev.index, stream))
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", idx))
+    ws = _kv4_ws.get((idx, stream))
     if ws is None or ws.numel() < need:
-        ws = _kv4_ws[dev.index, stream] = torch.zeros(need, dtype=torch.uint8, device=dev)
+        ws = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", idx))
+        _kv4_ws[idx, stream] = ws
     return ws
 
 
@@ -826,43 +865,42 @@ def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=No
     a request with more are not computed). scale: hd ** -0.5 unless given.
     Returns out (q's dtype); rows of no request are left as they were. out may
     be q itself."""
-    _kv4_rows(q, "q")
-    n, nq, hd = q.shape
-    ps = _kv4_page_size(pool, hd)
-    nkv = pool.shape[1]
-    _need(block_table, torch.int32, "block_table", 2)
-    _need(lens, torch.int64, "lens", 1)
+    idx = _home(pool, "pool")
+    n, nq, hd = _kv4_rows(q, "q", idx)
+    ps = _kv4_page_size(pool, hd, idx)
+    pages, nkv = pool.shape[0], pool.shape[1]
+    _arg(block_table, torch.int32, "block_table", 2, idx)
+    _arg(lens, torch.int64, "lens", 1, idx)
     B, W = block_table.shape
     if lens.numel() != B:
         raise ValueError(f"lens must have one element per table row ({B})")
     max_rows = int(max_rows)
     if cu_rows is not None:
-        _need(cu_rows, torch.int64, "cu_rows", 1)
+        _arg(cu_rows, torch.int64, "cu_rows", 1, idx)
         if cu_rows.numel() != B + 1:
             raise ValueError(f"cu_rows must have {B + 1} elements")
     if nq % nkv:
         raise ValueError(f"{nq} query heads are no multiple of {nkv} kv heads")
     scale = hd ** -0.5 if scale is None else float(scale)
-    dev = pool.device
-    ensure_device(dev)
+    qs = q.stride()
     if out is None:
-        out = torch.empty((n, nq, hd), dtype=q.dtype, device=dev)
+        out = torch.empty((n, nq, hd), dtype=q.dtype, device=pool.device)
     else:
-        _kv4_rows(out, "out")
-        if out.shape != q.shape or out.dtype != q.dtype:
+        _kv4_rows(out, "out", idx)
+        if out.shape != q.shape or out.dtype is not q.dtype:
             raise ValueError("out must have q's shape and dtype")
-        sr, sh = out.stride(0), out.stride(1)
-        if not ((nq == 1 or sh >= hd) and (n == 1 or sr >= (nq - 1) * sh + hd)
-                or (n == 1 or sr >= hd) and (nq == 1 or sh >= (n - 1) * sr + hd)):
-            raise ValueError("out's rows and heads must not overlap")
-    _same_device(dev, q, block_table, lens, cu_rows, out, workspace)
-    with _on(dev):
-        st = _stream_ptr(dev)
-        need = _kv4_ws_bytes(dev.index, nq, nkv, hd, max_rows)
-        ws = workspace if workspace is not None else _kv4_default_ws(dev, st, need)
+    os = out.stride()
+    if not ((nq == 1 or os[1] >= hd) and (n == 1 or os[0] >= (nq - 1) * os[1] + hd)
+            or (n == 1 or os[0] >= hd) and (nq == 1 or os[1] >= (n - 1) * os[0] + hd)):
+        raise ValueError("out's rows and heads must not overlap")
+    with _on(idx):
+        st = _stream_ptr(pool.device)
+        if workspace is None:
+            workspace = _kv4_default_ws(idx, st, _kv4_ws_bytes(idx, nq, nkv, hd, max_rows))
+        else:
+            _arg(workspace, torch.uint8, "workspace", 1, idx)
         _lib.check(_lib.load().qz_kv4_attention(
-            q.data_ptr(), _KV4_DTYPES[q.dtype], q.stride(0), q.stride(1), out.data_ptr(),
-            out.stride(0), out.stride(1), pool.data_ptr(), pool.shape[0], ps,
-            block_table.data_ptr(), W, lens.data_ptr(), _ptr(cu_rows), B, n, max_rows, nq, nkv,
-            hd, scale, ws.data_ptr(), ws.numel(), st))
+            q.data_ptr(), _KV4_DTYPES[q.dtype], qs[0], qs[1], out.data_ptr(), os[0], os[1],
+            pool.data_ptr(), pages, ps, block_table.data_ptr(), W, lens.data_ptr(), _ptr(cu_rows),
+            B, n, max_rows, nq, nkv, hd, scale, workspace.data_ptr(), workspace.numel(), st))
     return out
