@@ -36,6 +36,20 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+__device__ __forceinline__ f2_t f2_mul(f2_t a, f2_t b) {
+  f2_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2_t f2_add(f2_t a, f2_t b) {
+  f2_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2_t f2_set(float a, float b) {
+  return f2_pack(__float_as_uint(a), __float_as_uint(b));
+}
+
 // n consecutive elements as fp32; `vec`: p is 16-byte aligned and n * sizeof(T)
 // a multiple of 16.
 template <int n, class T>
@@ -243,6 +257,21 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// Extremes of n values, NaN if one is (three-input min and max: half the instructions).
+template <int n>
+__device__ __forceinline__ void extremes(const float (&x)[n], float& mn, float& mx) {
+  mn = mx = x[0];
+#pragma unroll
+  for (int j = 1; j + 1 < n; j += 2) {
+    asm("min.NaN.f32 %0, %0, %1, %2;" : "+f"(mn) : "f"(x[j]), "f"(x[j + 1]));
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(mx) : "f"(x[j]), "f"(x[j + 1]));
+  }
+  if constexpr (n % 2 == 0) {
+    mn = min_nan(mn, x[n - 1]);
+    mx = max_nan(mx, x[n - 1]);
+  }
+}
+
 // The parameter word and the fp32 values of s and z for a row's extremes. A row
 // with a non-finite value, or whose z or s leaves bf16's range, gets NaN for
 // both (it reads back as NaN); a row whose maximum does not exceed z gets s = 0.
@@ -260,32 +289,63 @@ __device__ __forceinline__ uint32_t row_params(float mn, float mx, float& s, flo
   return sb | (zb << 16);
 }
 
-// A value's code: clamp(round((x - z) / s), 0, 15) of the real quotient,
-// ties to even. t = (x - z) * (1 / s) in fp32 is within 3 * 2^-24 * |t| < 1e-5
-// of it, so only a t that close to the middle of two codes (1e-4 is taken) is
-// decided again in fp64, where x - z and the comparison lose nothing that
-// matters. Adding 1.5 * 2^23 rounds t to an integer in the low mantissa bits.
-__device__ __forceinline__ uint32_t code_of(float x, float s, float z, float inv, bool tiny) {
-  float t = __fsub_rn(x, z) * inv;
-  t = fminf(fmaxf(t, 0.f), 15.f);
-  const float r = __fadd_rn(t, 12582912.0f);
-  uint32_t c = __float_as_uint(r) & 15u;
-  if (tiny || fabsf(t - __fsub_rn(r, 12582912.0f)) > 0.4999f) {
-    const double d = rint((static_cast<double>(x) - static_cast<double>(z)) / static_cast<double>(s));
-    c = d >= 15.0 ? 15u : (d > 0.0 ? static_cast<uint32_t>(d) : 0u);
-  }
-  return c;
-}
-
-// Codes of n <= 16 values, value j in bits 4 j ...; zero when s is.
+// Codes of n <= 16 values, value j in bits 4 j ...: clamp(round((x - z) / s), 0, 15)
+// of the real quotient, ties to even; zero when s is. t = (x - z) * (1 / s) in fp32
+// (an approximate reciprocal) is within 4 * 2^-24 * 15.1 < 4e-6 of it, so only a t
+// within 1e-5 of the middle of two codes is decided again, by comparing x - z with
+// (m + 1/2) s in fp64, where nothing that matters is lost. s is the row's
+// (max - z) / 15 within 2^-9, so no t reaches 15.5. Adding 1.5 * 2^23 rounds t to
+// an integer in the low mantissa bits; the words are summed with their constant
+// exponent bits, which one subtraction takes out. Pairs go through the packed
+// fp32 operations: the rounds of 32 values, not HBM, bound a simpler form.
 template <int n>
 __device__ __forceinline__ uint2 codes_of(const float (&x)[n], float s, float z) {
-  if (!(s > 0.f)) return make_uint2(0u, 0u);
-  const bool tiny = s < 1e-30f;   // 1 / s would overflow
-  const float inv = tiny ? 0.f : 1.0f / s;
   uint32_t w[2] = {0u, 0u};
+  if (!(s > 0.f)) return make_uint2(0u, 0u);
+  if (s < 1e-30f) {               // 1 / s could overflow
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      float xj = x[0];
 #pragma unroll
-  for (int j = 0; j < n; ++j) w[j >> 3] |= code_of(x[j], s, z, inv, tiny) << (4 * (j & 7));
+      for (int k = 1; k < n; ++k) xj = j == k ? x[k] : xj;
+      const double d = rint((static_cast<double>(xj) - static_cast<double>(z)) / static_cast<double>(s));
+      const uint32_t c = d >= 15.0 ? 15u : (d > 0.0 ? static_cast<uint32_t>(d) : 0u);
+      if (j < 8) w[0] |= c << (4 * j); else w[1] |= c << (4 * (j - 8));
+    }
+    return make_uint2(w[0], w[1]);
+  }
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  constexpr float kMagic = 12582912.0f;   // 0x4B400000
+  const f2_t z2 = f2_set(z, z), inv2 = f2_set(inv, inv), magic2 = f2_set(kMagic, kMagic);
+  uint32_t bias[2] = {0u, 0u};
+  float border = 0.f;                     // largest distance from an integer
+#pragma unroll
+  for (int j = 0; j < n; j += 2) {
+    const float2 q = f2_unpack(f2_mul(f2_sub(f2_set(x[j], x[j + 1]), z2), inv2));
+    const f2_t t2 = f2_set(fmaxf(q.x, 0.f), fmaxf(q.y, 0.f));
+    const f2_t r2 = f2_add(t2, magic2);
+    const float2 r = f2_unpack(r2), d = f2_unpack(f2_sub(t2, f2_sub(r2, magic2)));
+    border = fmaxf(border, fmaxf(fabsf(d.x), fabsf(d.y)));
+    w[j >> 3] += __float_as_uint(r.x) << (4 * (j & 7));
+    w[j >> 3] += __float_as_uint(r.y) << (4 * ((j & 7) + 1));
+    bias[j >> 3] += (0x4B400000u << (4 * (j & 7))) + (0x4B400000u << (4 * ((j & 7) + 1)));
+  }
+  w[0] -= bias[0];
+  w[1] -= bias[1];
+  if (border > 0.49999f) {
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float t = fmaxf(__fsub_rn(x[j], z) * inv, 0.f), m = floorf(t);
+      if (fabsf(t - m - 0.5f) < 2e-5f) {
+        const double d = static_cast<double>(x[j]) - static_cast<double>(z);
+        const double half = (static_cast<double>(m) + 0.5) * static_cast<double>(s);
+        const uint32_t lo = static_cast<uint32_t>(m);
+        const uint32_t c = lo + (d > half || (d == half && (lo & 1u)) ? 1u : 0u);
+        w[j >> 3] = (w[j >> 3] & ~(15u << (4 * (j & 7)))) | (c << (4 * (j & 7)));
+      }
+    }
+  }
   return make_uint2(w[0], w[1]);
 }
 
@@ -301,6 +361,7 @@ struct AppendArgs {
 };
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendPerSm = 3;   // CTAs; 80 registers a thread
 
 // Bound by HBM (the rows are read once, hd/2 + 4 bytes written). HD / 16 lanes
 // take the K and the V row of one head, 16 values each, as 16-byte chunks dealt
@@ -309,7 +370,7 @@ constexpr int kAppendThreads = 256;
 // the slot is known to be valid, keep twice the loads in flight: 16391 rows of
 // 8 x 128 fp32 took 51 us one row at a time.
 template <class T, int HD>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, kAppendPerSm) append_kernel(const AppendArgs a) {
   constexpr int LPR = HD / 16;
   constexpr int E = 16 / sizeof(T), C = 16 / E;   // elements of a chunk, chunks of a lane
   const int lane = threadIdx.x & (LPR - 1);
@@ -344,12 +405,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     float mn[2], mx[2];
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      mn[kv] = mx[kv] = x[kv][0];
-#pragma unroll
-      for (int j = 1; j < 16; ++j) {
-        mn[kv] = min_nan(mn[kv], x[kv][j]);
-        mx[kv] = max_nan(mx[kv], x[kv][j]);
-      }
+      extremes(x[kv], mn[kv], mx[kv]);
 #pragma unroll
       for (int o = LPR / 2; o > 0; o >>= 1) {
         mn[kv] = min_nan(mn[kv], __shfl_xor_sync(0xffffffffu, mn[kv], o));
@@ -509,12 +565,8 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kv4_kernel(const RopeArg
   }
   const int64_t slot = a.slots[row];
   if (slot < 0 || slot >= a.slots_max) return;
-  float mn = x[0], mx = x[0];
-#pragma unroll
-  for (int j = 1; j < E; ++j) {
-    mn = min_nan(mn, x[j]);
-    mx = max_nan(mx, x[j]);
-  }
+  float mn, mx;
+  extremes(x, mn, mx);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));

@@ -84,7 +84,7 @@ template <class T>
 int launch_append(const DeviceInfo& d, int hd, const qz::kv4::AppendArgs& a, cudaStream_t st) {
   const int per_block = qz::kv4::kAppendThreads / (hd / 16);
   const int64_t want = qz::cdiv(a.n * a.nkv, per_block);
-  const int grid = static_cast<int>(std::min<int64_t>(want, int64_t(d.sms) * 8));
+  const int grid = static_cast<int>(std::min<int64_t>(want, int64_t(d.sms) * qz::kv4::kAppendPerSm));
   return hd == 64 ? launch_kv4(qz::kv4::append_kernel<T, 64>, grid, qz::kv4::kAppendThreads, 0, st, a)
                   : launch_kv4(qz::kv4::append_kernel<T, 128>, grid, qz::kv4::kAppendThreads, 0, st, a);
 }
