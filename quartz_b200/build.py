@@ -3,7 +3,9 @@
     python -m quartz_b200.build
 
 nvcc cross-compiles for sm_100a on a host without a GPU. The library exports
-the C ABI declared in include/quartz_b200.h.
+the C ABI declared in include/quartz_b200.h. ``quartz_b200/_fastcall.so``, a
+CPython extension over the same entry points (csrc/fastcall.cpp), is built with
+the host compiler against the installed torch.
 """
 
 from __future__ import annotations
@@ -33,6 +35,37 @@ def nvcc() -> str:
     if not os.path.exists(cand):
         raise RuntimeError("nvcc not found")
     return cand
+
+
+FAST_SRC = SRC / "fastcall.cpp"
+FAST_OUT = PKG / "_fastcall.so"
+
+
+def build_fastcall(force: bool = False) -> Path:
+    """The extension module quartz_b200._fastcall."""
+    import sysconfig
+
+    import torch
+
+    header = REPO / "include" / "quartz_b200.h"
+    if not force and FAST_OUT.exists() and all(
+            p.stat().st_mtime <= FAST_OUT.stat().st_mtime for p in (FAST_SRC, header)):
+        return FAST_OUT
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+           cuda / "include", REPO / "include", sysconfig.get_paths()["include"]]
+    lib = root / "lib"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in inc], str(FAST_SRC), "-o", str(FAST_OUT), f"-L{lib}",
+           f"-L{cuda / 'lib64'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+           "-lcudart", f"-Wl,-rpath,{lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise subprocess.CalledProcessError(r.returncode, cmd)
+    return FAST_OUT
 
 
 def sources() -> list[Path]:
@@ -74,6 +107,7 @@ def parse_ptxas(log: str) -> dict[str, dict]:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
+    build_fastcall(force)
     if not force and up_to_date():
         return OUT
     cmd = [nvcc(), "-Xptxas=-v", *NVCC_FLAGS, f"-I{REPO / 'include'}", f"-I{SRC}",

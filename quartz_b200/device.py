@@ -43,6 +43,7 @@ import torch
 from . import _lib
 
 _init_lock = threading.Lock()
+_fast = None     # the extension module _fastcall, once a device is ready
 _ready_devices: set[int] = set()
 _mlp_ws: dict[int, torch.Tensor] = {}
 _gemm_ws: dict[int, torch.Tensor] = {}
@@ -80,8 +81,26 @@ def ensure_device(dev: torch.device | int | None = None) -> int:
             if idx not in _ready_devices:
                 with torch.cuda.device(idx):
                     _lib.check(_lib.load().qz_init(idx))
+                _bind_fast(idx)
                 _ready_devices.add(idx)
     return idx
+
+
+def _bind_fast(idx: int) -> None:
+    """Give _fastcall (csrc/fastcall.cpp) the library's entry points and a ready device."""
+    global _fast
+    if _fast is None:
+        try:
+            from . import _fastcall
+        except ImportError as e:
+            raise ImportError("quartz_b200/_fastcall.so is missing or does not load: build it with "
+                              "`python -m quartz_b200.build`") from e
+        lib = _lib.load()
+        _fastcall.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+            "qz_kv4_plan", "qz_kv4_append", "qz_kv4_gather", "qz_kv4_attention",
+            "qz_kv4_attention_workspace_bytes")))
+        _fast = _fastcall
+    _fast.device_ready(idx)
 
 
 def _same_device(dev: torch.device, *ts) -> None:
@@ -687,6 +706,11 @@ def kv4_plan(lens, new_rows, block_table, free_pages, used, page_size, rows, len
     do not fit W, or for which the free pages do not last (counted in order)
     keeps its length and gets slots -1. lens_out / used_out may be lens / used
     themselves (a step captured in a CUDA graph then advances them)."""
+    if _fast is not None:
+        r = _fast.plan(lens, new_rows, block_table, free_pages, used, page_size, rows, lens_out,
+                       used_out)
+        if r is not None:
+            return KV4Plan._make(r)
     idx = _home(lens, "lens")
     _arg(lens, torch.int64, "lens", 1, idx)
     _arg(new_rows, torch.int64, "new_rows", 1, idx)
@@ -729,6 +753,8 @@ def kv4_append(k, v, pool, slots) -> None:
     (int64 [n]; a slot outside the pool stores nothing). Each row of a kv head
     keeps its own bf16 step and zero; a row with a non-finite value reads back
     as NaN. A slot must not appear twice in one call."""
+    if _fast is not None and _fast.append(k, v, pool, slots):
+        return
     if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
         raise TypeError("k and v must be torch.Tensors")
     idx = _home(pool, "pool")
@@ -752,6 +778,10 @@ def kv4_append(k, v, pool, slots) -> None:
 def kv4_gather(pool, slots, head_dim, out=None):
     """(k, v) fp32 [n, n_kv, head_dim]: the values at slots (int64 [n]); zeros
     for a slot outside the pool. out: a pair of contiguous tensors to write."""
+    if _fast is not None and out is None:
+        r = _fast.gather(pool, slots, head_dim)
+        if r is not None:
+            return r
     idx = _home(pool, "pool")
     hd = int(head_dim)
     ps = _kv4_page_size(pool, hd, idx)
@@ -849,6 +879,7 @@ def _kv4_default_ws(idx: int, stream: int, need: int) -> torch.Tensor:
     if ws is None or ws.numel() < need:
         ws = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", idx))
         _kv4_ws[idx, stream] = ws
+        _fast.workspace(idx, stream, ws.data_ptr(), ws.numel())
     return ws
 
 
@@ -865,6 +896,10 @@ def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=No
     a request with more are not computed). scale: hd ** -0.5 unless given.
     Returns out (q's dtype); rows of no request are left as they were. out may
     be q itself."""
+    if _fast is not None:
+        r = _fast.attention(q, pool, block_table, lens, cu_rows, max_rows, scale, out, workspace)
+        if r is not None:
+            return r
     idx = _home(pool, "pool")
     n, nq, hd = _kv4_rows(q, "q", idx)
     ps = _kv4_page_size(pool, hd, idx)

@@ -652,3 +652,75 @@ def test_one_workspace_for_calls_of_different_shapes():
     for _ in range(3):
         for q, pool, table, lens, cu, rows in made:
             _check_attention(q, pool, table, lens, cu, max_rows=rows, workspace=ws)
+
+
+def test_refusals_on_the_gpu():
+    """What the direct calls decline, the Python checks refuse by name; nothing is
+    written."""
+    qd, dev = _dev()
+    pool = qd.kv4_pool(4, 2, 64, 16, dev)
+    before = pool.clone()
+    f = torch.randn(3, 2, 64, device=dev)
+    i = _i64([0, 1, 2], dev)
+    table = torch.zeros(3, 2, dtype=torch.int32, device=dev)
+    free = torch.arange(4, dtype=torch.int32, device=dev)
+    one = _i64([1], dev)
+    q = torch.randn(3, 4, 64, device=dev)
+    bad = [
+        (TypeError, "int64", lambda: qd.kv4_append(f, f, pool, i.int())),
+        (ValueError, "one element per row", lambda: qd.kv4_append(f, f, pool, i[:2])),
+        (ValueError, "same shape", lambda: qd.kv4_append(f, f[:2], pool, i)),
+        (ValueError, "same shape and dtype", lambda: qd.kv4_append(f, f.half(), pool, i)),
+        (TypeError, "float32, bfloat16", lambda: qd.kv4_append(f.double(), f.double(), pool, i)),
+        (ValueError, "kv heads", lambda: qd.kv4_append(f[:, :1], f[:, :1], pool, i)),
+        (ValueError, "along head_dim", lambda: qd.kv4_append(f.transpose(0, 2), f.transpose(0, 2), pool, i)),
+        (ValueError, "head_dim", lambda: qd.kv4_gather(pool, i, 32)),
+        (ValueError, "no pages", lambda: qd.kv4_gather(pool, i, 128)),
+        (ValueError, "contiguous", lambda: qd.kv4_gather(pool[:, :1], i, 64)),
+        (ValueError, "CUDA", lambda: qd.kv4_gather(pool, i.cpu(), 64)),
+        (ValueError, "multiple", lambda: qd.kv4_attention(q[:, :3], pool, table, i)),
+        (ValueError, "per table row", lambda: qd.kv4_attention(q, pool, table, i[:2])),
+        (ValueError, "cu_rows must have", lambda: qd.kv4_attention(q, pool, table, i, cu_rows=i)),
+        (ValueError, "max_rows", lambda: qd.kv4_attention(q, pool, table, i, max_rows=0)),
+        (ValueError, "max_rows", lambda: qd.kv4_attention(q, pool, table, i, max_rows=2)),
+        (ValueError, "shape and dtype", lambda: qd.kv4_attention(q, pool, table, i, out=q[:2])),
+        (ValueError, "overlap", lambda: qd.kv4_attention(q, pool, table, i, out=q[:1].expand(3, 4, 64))),
+        (ValueError, "workspace", lambda: qd.kv4_attention(
+            q, pool, table, i, workspace=torch.zeros(256, dtype=torch.uint8, device=dev))),
+        (ValueError, "per table row", lambda: qd.kv4_plan(i[:2], i, table, free, one, 16, 4)),
+        (ValueError, "page size", lambda: qd.kv4_plan(i, i, table, free, one, 17, 4)),
+        (ValueError, "one element", lambda: qd.kv4_plan(i, i, table, free, i, 16, 4)),
+        (ValueError, "negative", lambda: qd.kv4_plan(i, i, table, free, one, 16, -1)),
+        (TypeError, "int32", lambda: qd.kv4_plan(i, i, table, free.long(), one, 16, 4)),
+    ]
+    for kind, msg, call in bad:
+        with pytest.raises(kind, match=msg):
+            call()
+    assert torch.equal(pool, before) and not table.any()
+
+
+def test_calls_on_another_stream_and_with_default_arguments():
+    """The direct calls give what the checked ones give, on side streams too."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(31)
+    lens = [100, 7]
+    pool, table = _context(lens, 2, 64, 16, g, dev)
+    q = torch.randn(2, 6, 64, generator=g, device=dev)
+    tl = _i64(lens, dev)
+    want = qd.kv4_attention(q, pool, table, tl, scale=64 ** -0.5)
+    fast, qd._fast = qd._fast, None
+    try:
+        checked = qd.kv4_attention(q, pool, table, tl)
+    finally:
+        qd._fast = fast
+    assert torch.equal(want, checked) and torch.equal(want, qd.kv4_attention(q, pool, table, tl))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [qd.kv4_attention(q, pool, table, tl) for _ in range(3)]
+        k, v = qd.kv4_gather(pool, _i64([0, 5], dev), 64)
+        other = torch.zeros_like(pool)
+        qd.kv4_append(k, v, other, _i64([3, 4], dev))
+    side.synchronize()
+    for t in got:
+        assert torch.equal(t, want)
