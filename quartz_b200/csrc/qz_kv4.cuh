@@ -613,8 +613,12 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kv4_kernel(const RopeArg
 // exact. Nibbles 1 and 5 lie four bits higher, as 16 c * 2^-24; q's values for
 // them are divided by 16. For V, pairs run along positions: one PRMT joins the
 // halves of two positions' words; 0x6400 | d is 1024 + d, and one HADD2 (HFMA2
-// for the nibbles four bits higher) leaves d - 8. Centring V keeps the running
-// sum as small as its result; the MMA's accumulation truncates. Row r of the
+// for the nibbles four bits higher) leaves d - 8. Centring V keeps the sums as
+// small as their result. An MMA's accumulation truncates (about 3e-8 of the
+// accumulator each time), so for fp32 rows at most two MMAs follow one another from
+// zero, the sums are added up in fp32, and K is centred like V: with subnormal K
+// codes and accumulation in place, results were 1.3e-6 to 2.4e-6 off 64 bits. For
+// 16-bit rows both cheaper forms are far below the output's rounding. Row r of the
 // eight positions an MMA fragment pairs up is position r / 2 + 4 (r & 1), so
 // that the V rows a quarter-warp reads are neighbours (fewer bank conflicts).
 //
@@ -656,8 +660,8 @@ struct AttnArgs {
 
 // CTAs per SM that the register file and shared memory hold.
 constexpr int kAttnMaxPerSm = 5;
-__host__ __device__ constexpr int attn_per_sm(int hd, int nb) {
-  return nb == 1 ? (hd == 64 ? 5 : 4) : (hd == 64 ? 4 : 2);
+__host__ __device__ constexpr int attn_per_sm(int hd, int nb, bool wide) {
+  return nb == 1 ? (hd == 64 ? 5 : (wide ? 3 : 4)) : (hd == 64 ? 4 : 2);
 }
 template <int HD, int NB>
 __host__ __device__ constexpr int attn_queries() { return 4 * NB; }
@@ -682,6 +686,16 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same from a zero accumulator.
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
@@ -780,11 +794,13 @@ __device__ __forceinline__ int64_t div_floor(int64_t x, int64_t y, double inv) {
 }
 
 template <class T, int HD, int NB>
-__global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) == 4)) attn_kernel(const AttnArgs a) {
   constexpr int Q = attn_queries<HD, NB>();   // queries (row, head) of an item
   constexpr int KS = HD / 16;                 // MMAs along the head dimension, and O tiles
   constexpr int KW = HD / 32;                 // K words of a lane and row
   constexpr int VW = HD / 64;                 // V words of a lane and position
+  constexpr bool kWide = sizeof(T) == 4;      // the more exact forms
+  constexpr bool kWideO = kWide && !(HD == 128 && NB == 2);   // (there it would spill)
   constexpr float kNegInf = -INFINITY;
   constexpr int SB = attn_stage_bytes<HD>();
   extern __shared__ __align__(128) uint8_t attn_sh[];
@@ -938,17 +954,17 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
       // |x| * 2^(14 - e) < 2^15 for the row's largest; e bounded so that both
       // powers of two are normal
       int e = static_cast<int>((__float_as_uint(mx) >> 23) & 255u) - 127;
-      e = e < -113 ? -113 : (e > 117 ? 117 : e);
+      e = e < -112 ? -112 : (e > 117 ? 117 : e);
       const float up = pow2i(14 - e);
-      const float f = pow2i(10 + e) * a.scale, qs = sum * a.scale;
+      const float f = pow2i(e + (kWide ? -14 : 10)) * a.scale, qs = sum * a.scale;
       F[nb] = __shfl_sync(0xffffffffu, f, 8 * i);
       Qs[nb] = __shfl_sync(0xffffffffu, qs, 8 * i);
-      // pairs (0 4) (1 5) (2 6) (3 7) of each eight; odd nibbles stand as 16 c
+      // pairs (0 4) (1 5) (2 6) (3 7) of each eight; subnormal odd nibbles are 16 c
 #pragma unroll
       for (int m = 0; m < KW; ++m)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float s = k & 1 ? up * 0.0625f : up;
+          const float s = !kWide && (k & 1) ? up * 0.0625f : up;
           const float y0 = x[8 * m + k] * s, y1 = x[8 * m + k + 4] * s;
           const __half2 hi = __floats2half2_rn(y0, y1);
           const float2 back = __half22float2(hi);
@@ -1041,18 +1057,33 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
           for (int j = 0; j < 4; ++j) sc[nb][j] = 0.f;
 #pragma unroll
         for (int w = 0; w < KW; ++w) {
-          const uint32_t c0 = k0[w], c1 = k1[w], d0 = c0 >> 8, d1 = c1 >> 8;
+          if constexpr (kWide) {
+            // two MMAs from zero for each word, summed in fp32
+            uint32_t c0[4], c1[4];
+            centred4(k0[w], c0);
+            centred4(k1[w], c1);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            mma_f16(sc[nb], c0 & 0x000F000Fu, c1 & 0x000F000Fu, c0 & 0x00F000F0u, c1 & 0x00F000F0u,
-                    qf[nb][2 * w][0], qf[nb][2 * w][1]);
-            mma_f16(sc[nb], d0 & 0x000F000Fu, d1 & 0x000F000Fu, d0 & 0x00F000F0u, d1 & 0x00F000F0u,
-                    qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
+            for (int nb = 0; nb < NB; ++nb) {
+              float d[4];
+              mma_f16_new(d, c0[0], c1[0], c0[1], c1[1], qf[nb][2 * w][0], qf[nb][2 * w][1]);
+              mma_f16(d, c0[2], c1[2], c0[3], c1[3], qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sc[nb][j] += d[j];
+            }
+          } else {
+            const uint32_t c0 = k0[w], c1 = k1[w], d0 = c0 >> 8, d1 = c1 >> 8;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              mma_f16(sc[nb], c0 & 0x000F000Fu, c1 & 0x000F000Fu, c0 & 0x00F000F0u, c1 & 0x00F000F0u,
+                      qf[nb][2 * w][0], qf[nb][2 * w][1]);
+              mma_f16(sc[nb], d0 & 0x000F000Fu, d1 & 0x000F000Fu, d0 & 0x00F000F0u, d1 & 0x00F000F0u,
+                      qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
+            }
           }
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float sk = par_s(kp[r]), zk = par_z(kp[r]);
+          const float sk = par_s(kp[r]), zk = kWide ? fmaf(8.f, sk, par_z(kp[r])) : par_z(kp[r]);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
             x[t][r][nb] = fmaf((sc[nb][2 * r] + sc[nb][2 * r + 1]) * F[nb], sk, zk * Qs[nb]);
@@ -1107,12 +1138,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
             for (int j = 0; j < 4; ++j) acc[nb][k][j] *= al * down;
         }
       }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        uint32_t v[4][VW];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) lds(base + v_at + t * k_next + r * 4 * (HD / 2), v[r]);
-        uint32_t wb[NB][2];
+      // weights of 16 positions: (hi, lo) of each row's side by side, transposed
+      auto weights = [&](int t, uint32_t (&wb)[NB][2]) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           float w[2];
@@ -1123,7 +1150,6 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
             zs[nb] = fmaf(p, fmaf(8.f, sv, par_z(vp[t][r][nb])), zs[nb]);
             w[r] = p * (sv * w_up);
           }
-          // (hi, lo) of each row's weight side by side, then transposed
           const __half2 hi = __floats2half2_rn(w[0], w[1]);
           const float2 back = __half22float2(hi);
           const __half2 lo = __floats2half2_rn(w[0] - back.x, w[1] - back.y);
@@ -1131,20 +1157,75 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB)) attn_kernel
           wb[nb][0] = trans8x8(prmt(h2, l2, 0x5410u));
           wb[nb][1] = trans8x8(prmt(h2, l2, 0x7632u));
         }
+      };
+      if constexpr (kWideO) {
+        // two MMAs from zero for each output tile, added in fp32
+        uint32_t wb[2][NB][2];
+        weights(0, wb[0]);
+        weights(1, wb[1]);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
+          uint32_t v[2][4];
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              uint32_t one[1];
+              lds(base + v_at + t * k_next + r * 4 * (HD / 2) + 4 * w, one);
+              v[t][r] = one[0];
+            }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t sel = half ? 0x7632u : 0x5410u;
-            uint32_t ha[4], hb[4];
-            centred4(prmt(v[0][w], v[1][w], sel), ha);
-            centred4(prmt(v[2][w], v[3][w], sel), hb);
+            float d[NB][2][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              uint32_t ha[4], hb[4];
+              centred4(prmt(v[t][0], v[t][1], sel), ha);
+              centred4(prmt(v[t][2], v[t][3], sel), hb);
+#pragma unroll
+              for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                  if (t == 0)
+                    mma_f16_new(d[nb][p], ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1],
+                                wb[t][nb][0], wb[t][nb][1]);
+                  else
+                    mma_f16(d[nb][p], ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1], wb[t][nb][0],
+                            wb[t][nb][1]);
+                }
+            }
 #pragma unroll
             for (int p = 0; p < 2; ++p)
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
-                mma_f16(acc[nb][w * 4 + half * 2 + p], ha[2 * p], ha[2 * p + 1], hb[2 * p],
-                        hb[2 * p + 1], wb[nb][0], wb[nb][1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[nb][w * 4 + half * 2 + p][j] += d[nb][p][j];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint32_t v[4][VW];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) lds(base + v_at + t * k_next + r * 4 * (HD / 2), v[r]);
+          uint32_t wb[NB][2];
+          weights(t, wb);
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t sel = half ? 0x7632u : 0x5410u;
+              uint32_t ha[4], hb[4];
+              centred4(prmt(v[0][w], v[1][w], sel), ha);
+              centred4(prmt(v[2][w], v[3][w], sel), hb);
+#pragma unroll
+              for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                  mma_f16(acc[nb][w * 4 + half * 2 + p], ha[2 * p], ha[2 * p + 1], hb[2 * p],
+                          hb[2 * p + 1], wb[nb][0], wb[nb][1]);
+            }
           }
         }
       }

@@ -95,16 +95,25 @@ int attn_blocks(int64_t max_rows, int group) { return max_rows * group > 4 ? 2 :
 
 struct Kv4AttnLayout {
   int grid;
-  int64_t part_off, total;
+  int64_t part_off, sums_off, total;
 };
 
-Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int nb, int hd) {
+// Requests with more rows than this (and heads that fit a tile) take the
+// tensor-core kernel's 128-row tiles, the others the split kernel.
+constexpr int kTcMinQueries = 32;
+int64_t split_rows(int group) {
+  return group > qz::kv4::kTcRows ? 0x7FFFFFFF : std::max(1, kTcMinQueries / group);
+}
+
+Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int64_t max_rows, int group, int hd, bool wide) {
+  const int nb = attn_blocks(max_rows, group);
   Kv4AttnLayout l;
-  l.grid = d.sms * qz::kv4::attn_per_sm(hd, nb);
+  l.grid = d.sms * qz::kv4::attn_per_sm(hd, nb, wide);
   // the tickets' place is the same for every variant, so that one workspace
   // serves calls of different shapes in turn
   l.part_off = qz::cdiv(int64_t(d.sms) * qz::kv4::kAttnMaxPerSm * 4, 256) * 256;
-  l.total = l.part_off + int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4;
+  l.sums_off = l.part_off + qz::cdiv(int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4, 256) * 256;
+  l.total = l.sums_off + (max_rows > split_rows(group) ? int64_t(d.sms) * qz::kv4::kTcRows * hd * 4 : 0);
   return l;
 }
 
@@ -122,13 +131,6 @@ int launch_kv4_attn_t(int hd, int nb, const qz::kv4::AttnArgs& a, int grid, cuda
   if (hd == 64)
     return nb == 1 ? launch_kv4_attn<T, 64, 1>(a, grid, st) : launch_kv4_attn<T, 64, 2>(a, grid, st);
   return nb == 1 ? launch_kv4_attn<T, 128, 1>(a, grid, st) : launch_kv4_attn<T, 128, 2>(a, grid, st);
-}
-
-// Requests with more rows than this (and heads that fit a tile) take the
-// tensor-core kernel's 128-row tiles, the others the split kernel.
-constexpr int kTcMinQueries = 32;
-int64_t split_rows(int group) {
-  return group > qz::kv4::kTcRows ? 0x7FFFFFFF : std::max(1, kTcMinQueries / group);
 }
 
 template <class T, int HD>
@@ -248,7 +250,8 @@ int qz_kv4_attention_workspace_bytes(int nq, int nkv, int hd, int64_t max_rows, 
     return fail(QZ_ERR_INVALID, "qz_kv4_attention_workspace_bytes: max_rows must be >= 1");
   DeviceInfo* d = nullptr;
   if (int rc = device_info(&d)) return rc;
-  *bytes = kv4_attn_layout(*d, attn_blocks(max_rows, nq / nkv), hd).total;
+  // (16-bit rows take the larger grid)
+  *bytes = kv4_attn_layout(*d, max_rows, nq / nkv, hd, false).total;
   return QZ_OK;
 }
 
@@ -275,7 +278,7 @@ int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_h
   DeviceInfo* d = nullptr;
   if (int rc = device_info(&d)) return rc;
   const int group = nq / nkv, nb = attn_blocks(max_rows, group);
-  const Kv4AttnLayout L = kv4_attn_layout(*d, nb, hd);
+  const Kv4AttnLayout L = kv4_attn_layout(*d, max_rows, group, hd, dtype == qz::kv4::kF32);
   if (static_cast<int64_t>(ws_bytes) < L.total || !aligned_to(ws, 256))
     return fail(QZ_ERR_INVALID, "qz_kv4_attention: workspace too small or not 256-byte aligned");
   qz::kv4::AttnArgs a{};
@@ -303,7 +306,7 @@ int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_h
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t few = split_rows(group);
   if (max_rows > few) {
-    qz::kv4::TcArgs t{a, 0};
+    qz::kv4::TcArgs t{a, 0, d->sms, reinterpret_cast<float4*>(static_cast<char*>(ws) + L.sums_off)};
     t.out_vec = rows_aligned(out, out_row_stride, out_head_stride, dtype);
     t.a.rows_lo = static_cast<int>(few);
     t.a.rows_hi = static_cast<int>(std::min<int64_t>(max_rows, 0x7FFFFFFF));

@@ -9,7 +9,8 @@
 //
 // An item is 128 (row, head) pairs of one kv head; heads of a group share the
 // keys, so a tile is 128 / group query rows. Per tile of 128 positions
-//   S [128 x 128] = Q codes(K)^T        A = Q from TMEM, B = K codes, K-major
+//   S [128 x 128] = Q codes(K)^T        A = Q from TMEM, B = K codes (fp32 rows:
+//                                       less 8), K-major
 //   O [128 x hd] += W (codes(V) - 8)    A = W from TMEM, B = V codes, MN-major
 // Both A operands live in TMEM: with Q in shared memory an MMA would read 8 KB
 // for 64 cycles of work, the whole bandwidth of shared memory, before the
@@ -55,8 +56,29 @@ constexpr uint32_t kColQ = 0, kColO = 128, kColS = 256;
 
 struct TcArgs {
   AttnArgs a;
-  int out_vec;   // out rows are 16-byte aligned
+  int out_vec;      // out rows are 16-byte aligned
+  int slots;        // places of `sums`, one for each SM
+  float4* sums;     // [slots][HD / 4][kTcRows]
 };
+
+// Tiles that O accumulates in TMEM before it is added to fp32 sums in the
+// workspace (L2). The MMA truncates its accumulator, 8 or 16 times a tile and by
+// about 3e-8 of it each time; without this, results drift by 1e-5 of themselves per
+// 40 tiles (fp32 rows; 3.4e-3 at 100000 positions). Even: the odd tiles' threads
+// do it, while the even ones work on the next tile.
+template <int L>
+__host__ __device__ constexpr int tc_flush() { return L == 2 ? 2 : 16; }
+
+// This CTA's place in the workspace: one CTA runs on an SM at a time.
+__device__ __forceinline__ uint32_t sm_id() {
+  uint32_t id;
+  asm volatile("mov.u32 %0, %%smid;" : "=r"(id));
+  return id;
+}
+template <int HD>
+__device__ __forceinline__ float4* sums_of(const TcArgs& args) {
+  return args.sums + static_cast<size_t>(sm_id()) * (HD / 4 * kTcRows);
+}
 
 template <int HD>
 __host__ __device__ constexpr int tc_tile_bytes() { return kTcKeys * HD * 2; }
@@ -68,19 +90,23 @@ __host__ __device__ constexpr int tc_raw_bytes() { return kTcKeys * (HD + 8); }
 // barriers. At least 116 KB is asked for, so that one CTA (and its 512 TMEM
 // columns) occupies an SM.
 struct TcShared {
-  float sk[kTcRing][kTcKeys], zk[kTcRing][kTcKeys];   // K's step and zero
+  float sk[kTcRing][kTcKeys], zk[kTcRing][kTcKeys];   // K's step, zero (+ 8 step if centred)
   float sv[kTcRing][kTcKeys], zc[kTcRing][kTcKeys];   // V's step * 2^(9 - ev), zero + 8 step
   alignas(16) uint32_t valid[kTcRing][4];   // positions that exist, one bit each
   float down[kTcRing];          // 2^(ev before - ev): O's factor when V's exponent grows
   float w_down[kTcRing];        // 2^(ev - 9)
   float top[2][2][kTcRows];     // [tile & 1][half]: maximum of a row's half tile
   float max[2][kTcRows];        // [tile & 1]: a row's maximum so far
-  float ex[3][4][kTcRows];      // exchange between a row's four threads
+  // exchange between a row's four threads, when q is read and at the end (a group
+  // without a tile reaches the end while others still read q)
+  float ex_q[2][4][kTcRows], ex[3][4][kTcRows];
+  float flushed[2][kTcRows];    // [half]: the maximum that a row's sums in the workspace stand relative to
+  int flushing;                 // this SM has a place in the workspace
   uint32_t odd[kTcRing];        // a V parameter of the tile is not finite
   int64_t scan[128];
   int item[6];                  // request, first row, rows, first row of q, len - rows, positions seen
   uint64_t k_full[2], v_full[2], s_full[2], p_full[2], v_empty[2], par_full[kTcRing], q_ready, drain;
-  uint64_t raw_full[kTcRaw], raw_empty[kTcRaw], t_full[2][4], m_full[2][4];
+  uint64_t raw_full[kTcRaw], raw_empty[kTcRaw], t_full[2][4], m_full[2][4], o_free;
   uint32_t raw_groups[kTcRaw];  // which 16-position groups of a packed tile exist
   uint32_t tmem;
 };
@@ -157,16 +183,22 @@ __device__ __forceinline__ bool bar_any(int id, int n, bool q) {
   return r != 0u;
 }
 
-// One word of eight codes as fp16 pairs, in nibble order 0 4 1 5 2 6 3 7: the
-// subnormals c * 2^-24 (16 c * 2^-24 for nibbles 1, 5, 3, 7) for K ...
-__device__ __forceinline__ uint4 k_pairs(uint32_t w) {
-  const uint32_t y = w >> 8;
-  return make_uint4(w & 0x000F000Fu, w & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+// The four pairs of a word's codes, in nibble order 0 4 1 5 2 6 3 7, as they lie:
+// c * 2^-24, and 16 c * 2^-24 for nibbles 1, 5, 3, 7.
+__device__ __forceinline__ void subnormal4(uint32_t x, uint32_t (&h)[4]) {
+  const uint32_t y = x >> 8;
+  h[0] = x & 0x000F000Fu;
+  h[1] = x & 0x00F000F0u;
+  h[2] = y & 0x000F000Fu;
+  h[3] = y & 0x00F000F0u;
 }
-// ... and c - 8 for V.
-__device__ __forceinline__ uint4 v_pairs(uint32_t w) {
+
+// One word of eight codes as fp16 pairs in nibble order 0 4 1 5 2 6 3 7: less 8, or
+// (SUB) as the subnormals that they are, for K of 16-bit rows (see attn_kernel).
+template <bool SUB>
+__device__ __forceinline__ uint4 pairs_of(uint32_t w) {
   uint32_t h[4];
-  centred4(w, h);
+  if constexpr (SUB) subnormal4(w, h); else centred4(w, h);
   return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
@@ -270,6 +302,7 @@ __device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, cons
                                            RowState& st) {
   uint32_t v[2][16];
   tc::tmem_ld16(taddr, v[0]);
+  f2_t l = f2_set(0.f, 0.f), zs = f2_set(0.f, 0.f);   // this tile's, then added: long sums stay exact
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     tc::tmem_wait_ld();
@@ -291,8 +324,8 @@ __device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, cons
       for (int e = 0; e < 2; ++e) {
         const f2_t p = f2_set(ex2(__uint_as_float(x[4 * q + 2 * e])),
                               ex2(__uint_as_float(x[4 * q + 2 * e + 1])));
-        st.l = f2_add(st.l, p);
-        st.zs = f2_fma(p, e ? f2_set(z.z, z.w) : f2_set(z.x, z.y), st.zs);
+        l = f2_add(l, p);
+        zs = f2_fma(p, e ? f2_set(z.z, z.w) : f2_set(z.x, z.y), zs);
         const f2_t y2 = f2_mul(p, e ? f2_set(s.z, s.w) : f2_set(s.x, s.y));
         const float2 y = f2_unpack(y2);
         const __half2 hi = __floats2half2_rn(y.x, y.y);
@@ -306,8 +339,10 @@ __device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, cons
       }
     }
 #pragma unroll
-    for (int l = 0; l < L; ++l) tmem_st8(taddr + c * (8 * L) + 8 * l, w + 8 * l);
+    for (int k = 0; k < L; ++k) tmem_st8(taddr + c * (8 * L) + 8 * k, w + 8 * k);
   }
+  st.l = f2_add(st.l, l);
+  st.zs = f2_add(st.zs, zs);
 }
 
 template <class T, int HD>
@@ -316,6 +351,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   constexpr int TB = tc_tile_bytes<HD>();
   constexpr int RB = tc_raw_bytes<HD>();
   constexpr int BLK = kTcKeys * 128;             // bytes of 64 dimensions of a tile
+  constexpr int kFlush = tc_flush<L>();
   constexpr float kNegInf = -INFINITY;
   const AttnArgs& a = args.a;
   extern __shared__ __align__(128) uint8_t tc_raw[];
@@ -344,6 +380,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   }
   if (tid == 0) {
     sh.item[0] = -1;
+    sh.flushing = sm_id() < static_cast<uint32_t>(args.slots);   // (nothing is written outside of it)
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&sh.k_full[s]), kTcConverters);
       mbar_init(smem_u32(&sh.v_full[s]), kTcConverters);
@@ -362,6 +399,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     }
     mbar_init(smem_u32(&sh.q_ready), kTcSoftmax);
     mbar_init(smem_u32(&sh.drain), 1);
+    mbar_init(smem_u32(&sh.o_free), 256);
     fence_mbar_init();
   }
   __syncthreads();
@@ -401,23 +439,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = sh.tmem;
-  const int h = blockIdx.x % a.nkv;
-  const int seen = sh.item[5], nt = (seen + kTcKeys - 1) / kTcKeys;
-
+  // (each role reads these for itself: kept from here on, they would spill)
+  auto tmem_base = [&]() -> uint32_t { return *const_cast<volatile uint32_t*>(&sh.tmem); };
+  auto item = [&](int k) -> int { return *const_cast<volatile int*>(&sh.item[k]); };
+  auto seen_by = [&]() -> int { return item(5); };
   if (warp < 16) {
     // ======================= softmax =======================================
     regs_more<88>();
     // row r of the item; quarter: which TMEM lanes; odd / half: which tiles and positions
     const int r = tid & 127, quarter = warp & 3, odd = (warp >> 2) & 1, half = warp >> 3;
     const int part = warp >> 2;               // this thread's share of the row's dimensions
-    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    const uint32_t lane_addr = tmem_base() + (static_cast<uint32_t>(32 * quarter) << 16);
+    const int nt = (seen_by() + kTcKeys - 1) / kTcKeys, h = blockIdx.x % a.nkv;
     // r / group for r < 128: the error of the rounded-up reciprocal, 128 / 65536,
     // is below 1 / group
     const uint32_t inv_group = (65535u + a.group) / a.group;
     const int rg = static_cast<int>((r * inv_group) >> 16);
-    const int row0 = sh.item[1], n = sh.item[2];
-    const int64_t r0 = sh.item[3];
+    const int row0 = item(1), n = item(2);
+    const int64_t r0 = item(3);
     const int row = row0 + rg, head = h * a.group + (r - rg * a.group);
     const bool real = r < per * a.group && row < n;
     const int sees = sh.item[4] + row + 1;          // positions [0, lim) are seen
@@ -470,25 +509,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
       float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      sh.ex[0][part][r] = mx;
-      sh.ex[1][part][r] = sum;
+      sh.ex_q[0][part][r] = mx;
+      sh.ex_q[1][part][r] = sum;
       named_bar_sync(1 + quarter, 128);
-      mx = fmaxf(fmaxf(sh.ex[0][0][r], sh.ex[0][1][r]), fmaxf(sh.ex[0][2][r], sh.ex[0][3][r]));
-      sum = (sh.ex[1][0][r] + sh.ex[1][1][r]) + (sh.ex[1][2][r] + sh.ex[1][3][r]);
+      mx = fmaxf(fmaxf(sh.ex_q[0][0][r], sh.ex_q[0][1][r]), fmaxf(sh.ex_q[0][2][r], sh.ex_q[0][3][r]));
+      sum = (sh.ex_q[1][0][r] + sh.ex_q[1][1][r]) + (sh.ex_q[1][2][r] + sh.ex_q[1][3][r]);
       int e = static_cast<int>((__float_as_uint(mx) >> 23) & 255u) - 127;
-      e = e < -113 ? -113 : (e > 117 ? 117 : e);
+      e = e < -112 ? -112 : (e > 117 ? 117 : e);
       const float up = pow2i(14 - e);
-      F = pow2i(10 + e) * a.scale;
+      F = pow2i(e + (L == 2 ? -14 : 10)) * a.scale;
       Qs = sum * a.scale;
-      // pairs (0 4) (1 5) (2 6) (3 7) of each eight; odd nibbles stand as 16 c
-      const f2_t up2 = f2_set(up, up), up16 = f2_set(up * 0.0625f, up * 0.0625f);
+      // pairs (0 4) (1 5) (2 6) (3 7) of each eight, as K's codes lie (subnormal odd
+      // nibbles are 16 c)
+      const float up_odd = L == 2 ? up : up * 0.0625f;
 #pragma unroll
       for (int m = 0; m < DP / 8; m += 2) {
         uint32_t w[L][8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int at = 8 * (m + (k >> 2)) + (k & 3);
-          const f2_t y2 = f2_mul(f2_set(x[at], x[at + 4]), k & 1 ? up16 : up2);
+          const f2_t y2 = f2_mul(f2_set(x[at], x[at + 4]), k & 1 ? f2_set(up_odd, up_odd) : f2_set(up, up));
           const float2 y = f2_unpack(y2);
           const __half2 hi = __floats2half2_rn(y.x, y.y);
           w[0][k] = *reinterpret_cast<const uint32_t*>(&hi);
@@ -549,8 +589,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       const float down = sh.down[ring];
       if (__any_sync(0xffffffffu, now != before || down != 1.f)) {
         tc_rescale<64>(cols, 1.f, now == kNegInf ? 0.f : -mu - now);
-        if (j > 0) {
-          // O holds tiles 0 .. j - 1 relative to `before`, V's steps to the old exponent
+        if (sh.flushing ? j % kFlush : j) {
+          // O holds tiles up to j - 1 relative to `before`, V's steps to the old exponent
           const bool done = warp_wait(&sh.v_empty[odd ^ 1], ((j - 1) >> 1) & 1);
           if (!done && lane == 0) report_error(ERR_WAIT_FULL, 0x401u);
           tc::tc_fence_after();
@@ -574,6 +614,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       tmem_wait_st();
       tc::tc_fence_before();
       mbar_arrive(smem_u32(&sh.p_full[odd]));
+      if (j % kFlush == kFlush - 1 && j + 1 < nt && sh.flushing) {
+        // O to the sums, this thread's half of the row; the next tile starts it anew
+        failed = !warp_wait(&sh.v_empty[odd], (j >> 1) & 1);
+        if (failed) break;
+        tc::tc_fence_after();
+        const bool first = j < kFlush;
+        const float fl = first ? kNegInf : sh.flushed[half][r];
+        const float al = fl == kNegInf ? 1.f : ex2(fl - now);
+        const float wd = sh.w_down[ring];
+        sh.flushed[half][r] = now;
+        float4* const mine = sums_of<HD>(args) + half * (HD / 8) * kTcRows + r;
+#pragma unroll 1
+        for (int c = 0; c < HD / 2; c += 16) {
+          uint32_t o[16];
+          tc::tmem_ld16(lane_addr + kColO + half * (HD / 2) + c, o);
+          float4* at = mine + c / 4 * kTcRows;
+          float4 t[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            t[k] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(at + k * kTcRows);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            __stcg(at + k * kTcRows,
+                   make_float4(fmaf(__uint_as_float(o[4 * k]), wd, t[k].x * al),
+                               fmaf(__uint_as_float(o[4 * k + 1]), wd, t[k].y * al),
+                               fmaf(__uint_as_float(o[4 * k + 2]), wd, t[k].z * al),
+                               fmaf(__uint_as_float(o[4 * k + 3]), wd, t[k].w * al)));
+        }
+        tc::tc_fence_before();
+        mbar_arrive(smem_u32(&sh.o_free));
+      }
     }
     if (failed && lane == 0) report_error(ERR_WAIT_FULL, 0x400u);
     // ---- epilogue: the four threads' sums, relative to the last maximum ------------
@@ -602,6 +674,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       // The tiles are free now: rows of 16-byte chunks (chunk c of row r at
       // c ^ (r & 7)) go through them, so that a warp stores whole rows.
       const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const bool summed = nt > kFlush && sh.flushing;
+      const float fl = summed ? sh.flushed[0][r] : kNegInf, as = fl == kNegInf ? 1.f : ex2(fl - mf);
+      const float4* const sums = sums_of<HD>(args);
 #pragma unroll
       for (int c = 0; c < DP; c += 16) {
         uint32_t u[16];
@@ -609,35 +684,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
           tc::tmem_ld16(lane_addr + kColO + part * DP + c, u);
           tc::tmem_wait_ld();
         }
-        T y[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          // column 8 w + k holds dimension 8 w + (k / 2) + (k odd ? 4 : 0)
-          const int d = (k & ~7) + ((k & 7) >> 1) + ((k & 1) << 2);
-          y[d] = from_f<T>(nt > 0 ? fmaf(__uint_as_float(u[k]), wd, zs) * inv : 0.f);
-        }
-        if (args.out_vec) {
+        for (int k8 = 0; k8 < 16; k8 += 8) {
+          T y[8];
 #pragma unroll
-          for (int k = 0; k < 16 / pv; ++k) {
-            const int ch = (part * DP + c) / pv + k;
-            *reinterpret_cast<uint4*>(tiles + r * (CH * 16) + ((ch ^ (r & 7)) << 4)) =
-                *reinterpret_cast<const uint4*>(y + k * pv);
+          for (int k4 = 0; k4 < 8; k4 += 4) {
+            const float4 t = summed ? __ldcg(sums + ((part * DP + c + k8 + k4) / 4) * kTcRows + r)
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float e[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              // column 8 w + k holds dimension 8 w + (k / 2) + (k odd ? 4 : 0)
+              const int col = k4 + k, d = (col >> 1) + ((col & 1) << 2);
+              y[d] = from_f<T>(nt > 0 ? fmaf(__uint_as_float(u[k8 + col]), wd, fmaf(e[k], as, zs)) * inv : 0.f);
+            }
           }
-        } else if (real) {
-          T* o = static_cast<T*>(a.out) + (r0 + row) * a.o_rs + head * a.o_hs + part * DP + c;
+          if (args.out_vec) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = y[k];
+            for (int k = 0; k < 8 / pv; ++k) {
+              const int ch = (part * DP + c + k8) / pv + k;
+              *reinterpret_cast<uint4*>(tiles + r * (CH * 16) + ((ch ^ (r & 7)) << 4)) =
+                  *reinterpret_cast<const uint4*>(y + k * pv);
+            }
+          } else if (r < per * a.group && item(1) + rg < item(2)) {
+            T* o = static_cast<T*>(a.out) + (static_cast<int64_t>(item(3)) + item(1) + rg) * a.o_rs +
+                   (h * a.group + (r - rg * a.group)) * a.o_hs + part * DP + c + k8;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = y[k];
+          }
         }
       }
     }
     // every softmax warp comes here, whatever happened
     if (!bar_any(6, kTcSoftmax, !ok) && args.out_vec) {
+      const int first = item(1), rows = item(2);
+      const int64_t base = item(3);
 #pragma unroll 4
       for (int i = 0; i < CH / 4; ++i) {
         const int idx = i * kTcSoftmax + tid, rr = idx / CH, c = idx % CH;
         const int g = static_cast<int>((rr * inv_group) >> 16);
-        if (rr < per * a.group && row0 + g < n)
-          *(reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (r0 + row0 + g) * a.o_rs +
+        if (rr < per * a.group && first + g < rows)
+          *(reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (base + first + g) * a.o_rs +
                                      (h * a.group + (rr - g * a.group)) * a.o_hs) + c) =
               *reinterpret_cast<const uint4*>(tiles + rr * (CH * 16) + ((c ^ (rr & 7)) << 4));
       }
@@ -645,6 +732,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   } else if (warp < 20) {
     // ======================= converters ====================================
     regs_less<72>();
+    const int nt = (seen_by() + kTcKeys - 1) / kTcKeys;
     // 16-byte chunks of code rows, LPR per row; a thread has the same chunk of
     // every RPI-th row, so its addresses are fixed. The eight threads of one
     // store phase hold two rows (hd 128) and four chunks of each; taking the
@@ -694,13 +782,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         report_error(ERR_WAIT_EMPTY, 0x410u);
         break;
       }
-      put(tiles + buf * TB, raw, groups, [](uint32_t w) { return k_pairs(w); });
+      put(tiles + buf * TB, raw, groups, [](uint32_t w) { return pairs_of<L == 1>(w); });
       mbar_arrive(smem_u32(&sh.k_full[buf]));
       if (j >= 2 && !mbar_wait(smem_u32(&sh.v_empty[buf]), ((j >> 1) - 1) & 1)) {
         report_error(ERR_WAIT_EMPTY, 0x411u);
         break;
       }
-      put(tiles + (2 + buf) * TB, raw + cnt * (HD / 2), groups, [](uint32_t w) { return v_pairs(w); });
+      put(tiles + (2 + buf) * TB, raw + cnt * (HD / 2), groups, [](uint32_t w) { return pairs_of<false>(w); });
       mbar_arrive(smem_u32(&sh.v_full[buf]));
       mbar_arrive(smem_u32(&sh.raw_empty[st]));
     }
@@ -710,6 +798,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     // ======================= parameters ====================================
     // weights are p * s_v * 2^(9 - ev), ev the largest exponent of s_v so far
     const int s7 = a.shift < 7 ? a.shift : 7, cnt = 1 << s7;
+    const int seen = seen_by(), nt = (seen + kTcKeys - 1) / kTcKeys;
     int ev = -100;
 #pragma unroll 1
     for (int j = 0; j < nt; ++j) {
@@ -748,7 +837,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         const int p = lane + 32 * k;
         const float sv = par_s(vp[k]);
         sh.sk[ring][p] = par_s(kp[k]);
-        sh.zk[ring][p] = par_z(kp[k]);
+        sh.zk[ring][p] = L == 2 ? fmaf(8.f, par_s(kp[k]), par_z(kp[k])) : par_z(kp[k]);
         sh.sv[ring][p] = sv * up;
         sh.zc[ring][p] = fmaf(8.f, sv, par_z(vp[k]));
       }
@@ -767,6 +856,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     const int64_t ps = int64_t(1) << a.shift;
     const int32_t* tab = a.table + static_cast<int64_t>(sh.item[0]) * a.width;
     const bool parts = a.shift > 7;
+    const int seen = seen_by(), nt = (seen + kTcKeys - 1) / kTcKeys, h = blockIdx.x % a.nkv;
     const int cnt = parts ? kTcKeys : 1 << a.shift, copies = parts ? 4 : kTcKeys >> a.shift;
     const int pg = parts ? 0 : lane;
     const uint32_t bytes = parts ? (lane < 2 ? kTcKeys * (HD / 2) : kTcKeys * 4) : cnt * (HD + 8);
@@ -813,8 +903,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         if (lane == 0) report_error(ERR_DRAIN, 0x414u);
         break;
       }
-  } else if (warp == 22 && nt > 0) {
+  } else if (warp == 22 && seen_by() > 0) {
     // ======================= MMA issuer ====================================
+    const int nt = (seen_by() + kTcKeys - 1) / kTcKeys;
+    const uint32_t tmem = tmem_base();
     constexpr uint32_t id_s = idesc_f16(kTcKeys, false), id_o = idesc_f16(HD, true);
     const bool leader = elect_one();
     const uint64_t kdesc = tc::smem_desc_sw128(smem_u32(tiles));
@@ -824,11 +916,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       const uint32_t d = tmem + kColS + (j & 1) * 128;
       if (leader) {
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s)
+        for (int l = L - 1; l >= 0; --l)       // low limbs first: what they truncate is small
 #pragma unroll
-          for (int l = 0; l < L; ++l)
+          for (int s = 0; s < HD / 16; ++s)
             mma_f16_ts(d, tmem + kColQ + l * (HD / 2) + s * 8,
-                       kd + (((s >> 2) * BLK + (s & 3) * 32) >> 4), id_s, (s | l) != 0);
+                       kd + (((s >> 2) * BLK + (s & 3) * 32) >> 4), id_s, s != 0 || l != L - 1);
         tc::tc_commit(smem_u32(&sh.s_full[j & 1]));
       }
       __syncwarp();
@@ -846,17 +938,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         scores(j + 1);
       }
       ok = warp_wait(&sh.v_full[j & 1], (j >> 1) & 1) && warp_wait(&sh.p_full[j & 1], (j >> 1) & 1);
+      const bool anew = sh.flushing ? j % kFlush == 0 : j == 0;
+      if (anew && j > 0) ok = ok && warp_wait(&sh.o_free, (j / kFlush - 1) & 1);
       if (!ok) break;
       tc::tc_fence_after();
       const uint64_t vd = vdesc + (j & 1) * (TB >> 4);
       const uint32_t w = tmem + kColS + (j & 1) * 128;
       if (leader) {
 #pragma unroll
-        for (int s = 0; s < kTcKeys / 16; ++s)
+        for (int l = L - 1; l >= 0; --l)
 #pragma unroll
-          for (int l = 0; l < L; ++l)
+          for (int s = 0; s < kTcKeys / 16; ++s)
             mma_f16_ts(tmem + kColO, w + (s >> 2) * 64 + (s & 3) * (8 * L) + 8 * l,
-                       vd + ((s * 2048) >> 4), id_o, (j | s | l) != 0);
+                       vd + ((s * 2048) >> 4), id_o, !anew || s != 0 || l != L - 1);
         tc::tc_commit(smem_u32(&sh.v_empty[j & 1]));
       }
       __syncwarp();
@@ -872,7 +966,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   __syncthreads();
   if (warp == 22) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, 512);
+    tc::tmem_dealloc(tmem_base(), 512);
   }
 }
 

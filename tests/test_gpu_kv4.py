@@ -724,3 +724,30 @@ def test_calls_on_another_stream_and_with_default_arguments():
     side.synchronize()
     for t in got:
         assert torch.equal(t, want)
+
+
+@pytest.mark.parametrize("hd,nq,nkv,rows,t", [(128, 8, 2, 200, 30000), (64, 4, 2, 64, 60000), (128, 4, 1, 1, 50000)])
+def test_long_contexts_do_not_drift(hd, nq, nkv, rows, t):
+    """The MMAs truncate their accumulators; results over long contexts of fp32 rows
+    stay within a few fp32 roundings all the same (the 2-norm over all rows: 4e-6,
+    where fp32 sums over 60000 positions alone leave 2e-6 and accumulation in one
+    MMA chain 4e-4)."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(t)
+    pages = -(-t // 64)
+    pool = torch.randint(0, 256, (pages, nkv, 64 * (hd + 8)), generator=g, device=dev, dtype=torch.uint8)
+    par = torch.empty(pages, nkv, 2, 64, 2, device=dev)
+    par[..., 0] = 0.2 + 0.2 * torch.rand(pages, nkv, 2, 64, generator=g, device=dev)
+    par[..., 1] = -7.5 * par[..., 0]
+    pool[..., 64 * hd:] = par.to(torch.bfloat16).view(torch.uint8).flatten(2)
+    table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+    q = torch.randn(rows, nq, hd, generator=g, device=dev)
+    got = qd.kv4_attention(q, pool, table, _i64([t], dev), cu_rows=_i64([0, rows], dev), max_rows=rows)
+    k, v = (x.transpose(0, 1).flatten(1, 2)[:, :t] for x in P.load(pool, hd))
+    hide = torch.arange(t, device=dev) > t - rows + torch.arange(rows, device=dev)[:, None]
+    ref = torch.empty(rows, nq, hd, dtype=torch.float64, device=dev)
+    for h in range(nq):
+        s = (q[:, h].double() * hd ** -0.5) @ k[h // (nq // nkv)].T
+        ref[:, h] = torch.softmax(s.masked_fill(hide, -math.inf), -1) @ v[h // (nq // nkv)]
+    err = ((got.double() - ref).norm() / ref.norm()).item()
+    assert err < 4e-6
