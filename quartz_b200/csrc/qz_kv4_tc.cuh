@@ -69,15 +69,14 @@ struct TcArgs {
 template <int L>
 __host__ __device__ constexpr int tc_flush() { return L == 2 ? 2 : 16; }
 
-// This CTA's place in the workspace: one CTA runs on an SM at a time.
 __device__ __forceinline__ uint32_t sm_id() {
   uint32_t id;
   asm volatile("mov.u32 %0, %%smid;" : "=r"(id));
   return id;
 }
 template <int HD>
-__device__ __forceinline__ float4* sums_of(const TcArgs& args) {
-  return args.sums + static_cast<size_t>(sm_id()) * (HD / 4 * kTcRows);
+__device__ __forceinline__ float4* sums_of(const TcArgs& args, int place) {
+  return args.sums + static_cast<size_t>(place < 0 ? 0 : place) * (HD / 4 * kTcRows);
 }
 
 template <int HD>
@@ -100,8 +99,9 @@ struct TcShared {
   // exchange between a row's four threads, when q is read and at the end (a group
   // without a tile reaches the end while others still read q)
   float ex_q[2][4][kTcRows], ex[3][4][kTcRows];
-  float flushed[2][kTcRows];    // [half]: the maximum that a row's sums in the workspace stand relative to
-  int flushing;                 // this SM has a place in the workspace
+  // [half]: what a row's sums in the workspace stand relative to, its maximum and w_down
+  float flushed[2][kTcRows], flushed_w[2][kTcRows];
+  int place;                    // in the workspace, or -1
   uint32_t odd[kTcRing];        // a V parameter of the tile is not finite
   int64_t scan[128];
   int item[6];                  // request, first row, rows, first row of q, len - rows, positions seen
@@ -370,8 +370,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     int64_t r0;
     return (static_cast<int>(rows_of(a, b, &r0)) + per - 1) / per;
   };
+  int64_t len0 = 0;                              // of the thread's first request
   if (tid < 128) {
     int64_t mine = 0;
+    if (static_cast<int64_t>(tid) * chunk < a.B) len0 = a.lens[static_cast<int64_t>(tid) * chunk];
     for (int k = 0; k < chunk; ++k) {
       const int64_t b = static_cast<int64_t>(tid) * chunk + k;
       if (b < a.B) mine += tiles_of(b);
@@ -380,7 +382,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   }
   if (tid == 0) {
     sh.item[0] = -1;
-    sh.flushing = sm_id() < static_cast<uint32_t>(args.slots);   // (nothing is written outside of it)
+    // one CTA runs on an SM at a time; nothing is written outside of the workspace
+    const uint32_t sm = sm_id();
+    sh.place = sm < static_cast<uint32_t>(args.slots) ? static_cast<int>(sm) : -1;
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&sh.k_full[s]), kTcConverters);
       mbar_init(smem_u32(&sh.v_full[s]), kTcConverters);
@@ -403,6 +407,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     fence_mbar_init();
   }
   __syncthreads();
+  if (warp == 22) {
+    tc::tmem_alloc(smem_u32(&sh.tmem), 512);
+    tc::tmem_relinquish();
+    tc::tc_fence_before();
+  }
   if (tid < 128) {
     int64_t before = 0, total = 0;
     for (int k = 0; k * chunk < a.B; ++k) {
@@ -420,7 +429,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
       int64_t r0;
       const int64_t n = rows_of(a, b, &r0), row0 = (t - at) * per, lim = int64_t(1) << 30;
-      const int64_t off = a.lens[b] - n, last = (row0 + per < n ? row0 + per : n) + off;
+      const int64_t len = b == static_cast<int64_t>(tid) * chunk ? len0 : a.lens[b];
+      const int64_t off = len - n, last = (row0 + per < n ? row0 + per : n) + off;
       sh.item[0] = static_cast<int>(b);
       sh.item[1] = static_cast<int>(row0);
       sh.item[2] = static_cast<int>(n);
@@ -431,14 +441,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     }
   }
   __syncthreads();
-  if (sh.item[0] < 0) return;              // the grid is an upper bound
-  if (warp == 22) {
-    tc::tmem_alloc(smem_u32(&sh.tmem), 512);
-    tc::tmem_relinquish();
-  }
-  tc::tc_fence_before();
-  __syncthreads();
   tc::tc_fence_after();
+  if (sh.item[0] < 0) {                    // the grid is an upper bound
+    if (warp == 22) tc::tmem_dealloc(*const_cast<volatile uint32_t*>(&sh.tmem), 512);
+    return;
+  }
   // (each role reads these for itself: kept from here on, they would spill)
   auto tmem_base = [&]() -> uint32_t { return *const_cast<volatile uint32_t*>(&sh.tmem); };
   auto item = [&](int k) -> int { return *const_cast<volatile int*>(&sh.item[k]); };
@@ -475,15 +482,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
           return reinterpret_cast<uint4*>(tiles + (rr < 64 ? TB : 3 * TB) + (rr & 63) * (CH * 16) +
                                           ((c ^ (rr & 7)) << 4));
         };
+        // all loads before the first store; rows that are not real read the item's last
+        // (a load under a condition would wait for the one before it)
+        uint4 u[CH / 4];
+#pragma unroll
+        for (int i = 0; i < CH / 4; ++i) {
+          const int idx = i * kTcSoftmax + tid, rr = idx / CH, c = idx % CH;
+          const int g = static_cast<int>((rr * inv_group) >> 16), gr = row0 + g < n ? g : n - 1 - row0;
+          u[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (r0 + row0 + gr) * a.q_rs +
+                                                      (h * a.group + (rr - g * a.group)) * a.q_hs) + c);
+        }
 #pragma unroll
         for (int i = 0; i < CH / 4; ++i) {
           const int idx = i * kTcSoftmax + tid, rr = idx / CH, c = idx % CH;
           const int g = static_cast<int>((rr * inv_group) >> 16);
-          uint4 u = make_uint4(0u, 0u, 0u, 0u);
-          if (rr < per * a.group && row0 + g < n)
-            u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (r0 + row0 + g) * a.q_rs +
-                                                     (h * a.group + (rr - g * a.group)) * a.q_hs) + c);
-          *at(rr, c) = u;
+          *at(rr, c) = rr < per * a.group && row0 + g < n ? u[i] : make_uint4(0u, 0u, 0u, 0u);
         }
         named_bar_sync(6, kTcSoftmax);
         constexpr int pv = 16 / sizeof(T);
@@ -589,7 +602,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       const float down = sh.down[ring];
       if (__any_sync(0xffffffffu, now != before || down != 1.f)) {
         tc_rescale<64>(cols, 1.f, now == kNegInf ? 0.f : -mu - now);
-        if (sh.flushing ? j % kFlush : j) {
+        if (sh.place >= 0 ? j % kFlush : j) {
           // O holds tiles up to j - 1 relative to `before`, V's steps to the old exponent
           const bool done = warp_wait(&sh.v_empty[odd ^ 1], ((j - 1) >> 1) & 1);
           if (!done && lane == 0) report_error(ERR_WAIT_FULL, 0x401u);
@@ -614,34 +627,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       tmem_wait_st();
       tc::tc_fence_before();
       mbar_arrive(smem_u32(&sh.p_full[odd]));
-      if (j % kFlush == kFlush - 1 && j + 1 < nt && sh.flushing) {
+      if (j % kFlush == kFlush - 1 && j + 1 < nt && sh.place >= 0) {
         // O to the sums, this thread's half of the row; the next tile starts it anew
+        const bool first = j < kFlush;
+        const float wd = sh.w_down[ring];
+        float4* const mine = sums_of<HD>(args, sh.place) + half * (HD / 8) * kTcRows + r;
+        float4 t[4];
+        auto fetch = [&](int c) {                 // sums of 16 columns, ahead of their use
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            t[k] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(mine + (4 * c + k) * kTcRows);
+        };
+        fetch(0);
+        float al = 1.f;                           // from the sums' terms to O's
+        if (!first) {
+          const float fl = sh.flushed[half][r], fw = sh.flushed_w[half][r];
+          if (fl != now && fl != kNegInf) al = ex2(fl - now);
+          if (fw != wd) al *= fw / wd;
+        }
+        sh.flushed[half][r] = now;
+        sh.flushed_w[half][r] = wd;
         failed = !warp_wait(&sh.v_empty[odd], (j >> 1) & 1);
         if (failed) break;
         tc::tc_fence_after();
-        const bool first = j < kFlush;
-        const float fl = first ? kNegInf : sh.flushed[half][r];
-        const float al = fl == kNegInf ? 1.f : ex2(fl - now);
-        const float wd = sh.w_down[ring];
-        sh.flushed[half][r] = now;
-        float4* const mine = sums_of<HD>(args) + half * (HD / 8) * kTcRows + r;
 #pragma unroll 1
-        for (int c = 0; c < HD / 2; c += 16) {
+        for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[16];
-          tc::tmem_ld16(lane_addr + kColO + half * (HD / 2) + c, o);
-          float4* at = mine + c / 4 * kTcRows;
-          float4 t[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            t[k] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(at + k * kTcRows);
+          tc::tmem_ld16(lane_addr + kColO + half * (HD / 2) + 16 * c, o);
           tc::tmem_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            __stcg(at + k * kTcRows,
-                   make_float4(fmaf(__uint_as_float(o[4 * k]), wd, t[k].x * al),
-                               fmaf(__uint_as_float(o[4 * k + 1]), wd, t[k].y * al),
-                               fmaf(__uint_as_float(o[4 * k + 2]), wd, t[k].z * al),
-                               fmaf(__uint_as_float(o[4 * k + 3]), wd, t[k].w * al)));
+          for (int k = 0; k < 4; ++k) {
+            const float4 s = t[k];
+            __stcg(mine + (4 * c + k) * kTcRows,
+                   make_float4(fmaf(s.x, al, __uint_as_float(o[4 * k])),
+                               fmaf(s.y, al, __uint_as_float(o[4 * k + 1])),
+                               fmaf(s.z, al, __uint_as_float(o[4 * k + 2])),
+                               fmaf(s.w, al, __uint_as_float(o[4 * k + 3]))));
+          }
+          if (c + 1 < HD / 32) fetch(c + 1);
         }
         tc::tc_fence_before();
         mbar_arrive(smem_u32(&sh.o_free));
@@ -663,6 +686,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       l = fmaf(sh.ex[1][k][r], al, l);
       zs = fmaf(sh.ex[2][k][r], al, zs);
     }
+    // the sums of this thread's columns, ahead of the last tile's MMAs
+    const bool summed = nt > kFlush && sh.place >= 0;
+    float4 t[DP / 4];
+#pragma unroll
+    for (int k = 0; k < DP / 4; ++k)
+      t[k] = summed ? __ldcg(sums_of<HD>(args, sh.place) + (part * DP / 4 + k) * kTcRows + r)
+                    : make_float4(0.f, 0.f, 0.f, 0.f);
     bool ok = !failed;
     if (nt > 0 && ok) ok = mbar_wait(smem_u32(&sh.v_empty[(nt - 1) & 1]), ((nt - 1) >> 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
@@ -674,9 +704,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       // The tiles are free now: rows of 16-byte chunks (chunk c of row r at
       // c ^ (r & 7)) go through them, so that a warp stores whole rows.
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      const bool summed = nt > kFlush && sh.flushing;
       const float fl = summed ? sh.flushed[0][r] : kNegInf, as = fl == kNegInf ? 1.f : ex2(fl - mf);
-      const float4* const sums = sums_of<HD>(args);
+      const float asw = summed ? as * sh.flushed_w[0][r] : 0.f;
 #pragma unroll
       for (int c = 0; c < DP; c += 16) {
         uint32_t u[16];
@@ -689,14 +718,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
           T y[8];
 #pragma unroll
           for (int k4 = 0; k4 < 8; k4 += 4) {
-            const float4 t = summed ? __ldcg(sums + ((part * DP + c + k8 + k4) / 4) * kTcRows + r)
-                                    : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float e[4] = {t.x, t.y, t.z, t.w};
+            const float4 t4 = t[(c + k8 + k4) / 4];
+            const float e[4] = {t4.x, t4.y, t4.z, t4.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               // column 8 w + k holds dimension 8 w + (k / 2) + (k odd ? 4 : 0)
               const int col = k4 + k, d = (col >> 1) + ((col & 1) << 2);
-              y[d] = from_f<T>(nt > 0 ? fmaf(__uint_as_float(u[k8 + col]), wd, fmaf(e[k], as, zs)) * inv : 0.f);
+              y[d] = from_f<T>(nt > 0 ? fmaf(__uint_as_float(u[k8 + col]), wd, fmaf(e[k], asw, zs)) * inv : 0.f);
             }
           }
           if (args.out_vec) {
@@ -767,7 +795,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
       fence_async_smem();
     };
-    if (nt > 1 && !mbar_wait(smem_u32(&sh.q_ready), 0)) report_error(ERR_WAIT_FULL, 0x415u);
 #pragma unroll 1
     for (int j = 0; j < nt; ++j) {
       const int buf = j & 1, st = j % kTcRaw;
@@ -777,6 +804,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
       const uint8_t* raw = raws + st * RB;
       const uint32_t groups = sh.raw_groups[st];
+      // q goes through the second stages
+      if (j == 1 && !mbar_wait(smem_u32(&sh.q_ready), 0)) {
+        report_error(ERR_WAIT_FULL, 0x415u);
+        break;
+      }
       // K's stage is free once S(j - 2) is done, V's once O(j - 2) is
       if (j >= 2 && !mbar_wait(smem_u32(&sh.s_full[buf]), ((j >> 1) - 1) & 1)) {
         report_error(ERR_WAIT_EMPTY, 0x410u);
@@ -938,7 +970,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         scores(j + 1);
       }
       ok = warp_wait(&sh.v_full[j & 1], (j >> 1) & 1) && warp_wait(&sh.p_full[j & 1], (j >> 1) & 1);
-      const bool anew = sh.flushing ? j % kFlush == 0 : j == 0;
+      const bool anew = sh.place >= 0 ? j % kFlush == 0 : j == 0;
       if (anew && j > 0) ok = ok && warp_wait(&sh.o_free, (j / kFlush - 1) & 1);
       if (!ok) break;
       tc::tc_fence_after();
