@@ -84,10 +84,10 @@ __device__ __forceinline__ float par_z(uint32_t w) { return __uint_as_float(w & 
 //
 // Latency-bound (a few hundred bytes to about a megabyte): one launch, no
 // atomics. Every CTA scans all requests in shared memory, then CTAs share out
-// rows (binary search of the row's request) and requests (table entries). Up
-// to kPlanCluster CTAs form one cluster whose barrier separates the reading
-// of lens / used from the writing of their successors, so both may be updated
-// in place.
+// the rows (binary search of the row's request). Where lens or used are updated
+// in place, kPlanCluster CTAs form one cluster whose barrier separates the
+// reading from the writing; else a CTA for every 1024 rows needs no barrier
+// (1024 requests, 49000 rows: 7.0 us, in a cluster of 8 13.6 us).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanPer = 4;
 constexpr int kPlanMaxB = kPlanThreads * kPlanPer;
@@ -210,36 +210,28 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     *a.used_out = used + total;
   }
   const int live = s_cu[B];
+  // A new page's first position is always one of the request's new rows: that row
+  // writes the table entry (and none of those that are read here).
+  const int top = 1 << (31 - __clz(B));
   for (int64_t r = gt; r < a.rows; r += nthreads) {
     int64_t slot = -1, pos = -1;
     if (r < live) {
-      int lo = 0, hi = B - 1;   // the first request whose rows end after r
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_cu[mid + 1] > r) hi = mid; else lo = mid + 1;
-      }
-      const int64_t l = s_len[lo];
-      pos = l + r - s_cu[lo];
-      const int32_t first = s_page[lo];
+      int b = 0;   // the last request whose rows begin at r or before
+      for (int s = top; s > 0; s >>= 1)
+        if (b + s < B && s_cu[b + s] <= r) b += s;
+      const int64_t l = s_len[b];
+      const int32_t first = s_page[b];
+      pos = l + r - s_cu[b];
       if (first >= 0) {
-        const int64_t have = (l + ps - 1) >> shift, p = pos >> shift;
-        const int64_t page = p < have ? a.table[static_cast<int64_t>(lo) * a.width + p]
-                                      : a.free_pages[first + (p - have)];
-        if (page >= 0) slot = (page << shift) + (pos & (ps - 1));
+        const int64_t have = (l + ps - 1) >> shift, p = pos >> shift, in_page = pos & (ps - 1);
+        int32_t* entry = a.table + static_cast<int64_t>(b) * a.width + p;
+        const int32_t page = p < have ? *entry : a.free_pages[first + (p - have)];
+        if (p >= have && in_page == 0) *entry = page;
+        if (page >= 0) slot = (static_cast<int64_t>(page) << shift) + in_page;
       }
     }
     a.slots[r] = slot;
     a.positions[r] = pos;
-  }
-  // new table entries (the entries read above are the ones before them)
-  const int lane = tid & 31;
-  for (int b = gt >> 5; b < B; b += nthreads >> 5) {
-    const int32_t first = s_page[b];
-    if (first < 0) continue;
-    const int64_t l = s_len[b], have = (l + ps - 1) >> shift;
-    const int64_t want = (l + (s_cu[b + 1] - s_cu[b]) + ps - 1) >> shift;
-    for (int64_t j = have + lane; j < want; j += 32)
-      a.table[static_cast<int64_t>(b) * a.width + j] = a.free_pages[first + (j - have)];
   }
 }
 

@@ -169,10 +169,18 @@ int qz_kv4_plan(const int64_t* lens, const int64_t* new_rows, int64_t B, int32_t
   const int smem = qz::kv4::plan_smem(static_cast<int>(B));
   if (smem > 48 * 1024)
     QZ_CUDA(allow_smem(qz::kv4::plan_kernel, qz::kv4::plan_smem(qz::kv4::kPlanMaxB)));
-  // one CTA writes a small plan; a large one is shared out over a cluster
-  const int grid = rows + 4 * B > 4096 ? qz::kv4::kPlanCluster : 1;
+  // One CTA writes a small plan. A large one is shared out: over a cluster where lengths
+  // or the cursor are updated in place, else over as many CTAs as give each thread a row.
+  const bool large = rows + 4 * B > 4096;
+  auto meets = [](const int64_t* p, int64_t n, const int64_t* q, int64_t m) { return p < q + m && q < p + n; };
+  const bool in_place = meets(lens_out, B, lens, B) || meets(lens_out, B, new_rows, B) ||
+                        meets(lens_out, B, used, 1) || meets(used_out, 1, lens, B) ||
+                        meets(used_out, 1, new_rows, B) || meets(used_out, 1, used, 1);
+  const int64_t ctas = (rows + qz::kv4::kPlanThreads - 1) / qz::kv4::kPlanThreads;
+  const int cluster = large && in_place ? qz::kv4::kPlanCluster : 1;
+  const int grid = !large || in_place ? cluster : static_cast<int>(ctas < 1 ? 1 : (ctas > d->sms ? d->sms : ctas));
   return launch_kv4(qz::kv4::plan_kernel, grid, qz::kv4::kPlanThreads, smem,
-                    static_cast<cudaStream_t>(stream), a, grid);
+                    static_cast<cudaStream_t>(stream), a, cluster);
 }
 
 int qz_kv4_append(const void* k, const void* v, int dtype, int64_t k_row_stride,

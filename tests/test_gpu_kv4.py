@@ -751,3 +751,23 @@ def test_long_contexts_do_not_drift(hd, nq, nkv, rows, t):
         ref[:, h] = torch.softmax(s.masked_fill(hide, -math.inf), -1) @ v[h // (nq // nkv)]
     err = ((got.double() - ref).norm() / ref.norm()).item()
     assert err < 4e-6
+
+
+@pytest.mark.parametrize("what", ["lens", "used"])
+def test_large_plan_with_one_output_in_place(what):
+    """A plan of many CTAs of which only the lengths, or only the cursor, are updated in place."""
+    qd, dev = _dev()
+    rng = random.Random(5)
+    B, page = 900, 16
+    lens = [rng.randrange(700) for _ in range(B)]
+    joins = [rng.randrange(40) for _ in range(B)]
+    table = [[rng.randrange(9999) for _ in range(64)] for _ in range(B)]
+    free, used, rows = rng.sample(range(9999), 2000), 7, sum(joins) + 3000
+    tl, tj, tu = _i64(lens, dev), _i64(joins, dev), _i64([used], dev)
+    tt = torch.tensor(table, dtype=torch.int32, device=dev)
+    p = qd.kv4_plan(tl, tj, tt, torch.tensor(free, dtype=torch.int32, device=dev), tu, page, rows,
+                    lens_out=tl if what == "lens" else None, used_out=tu if what == "used" else None)
+    got = dict(cu_rows=p.cu_rows.tolist(), lens=p.lens.tolist(), used=p.used.tolist(),
+               slots=p.slots.tolist(), positions=p.positions.tolist(), table=tt.tolist())
+    assert got == P.plan(lens, joins, table, free, used, page, rows)
+    assert (tl.tolist() == lens) == (what == "used") and (tu.item() == used) == (what == "lens")
