@@ -533,7 +533,8 @@ int qz_kv4_attention_workspace_bytes(int nq, int nkv, int hd, int64_t max_rows, 
  * with the same strides. Positions beyond the table (lens[b] > width *
  * page_size) are not seen; table entries outside [0, pages) are not read and
  * their positions count as unseen. B <= 4096, width * page_size <= 2^30.
- * The result does not depend on timing.
+ * The result does not depend on timing. n, B and max_rows choose between two
+ * kernels (few rows, or tiles of 128 queries); their results differ by rounding.
  */
 int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_head_stride,
                      void* out, int64_t out_row_stride, int64_t out_head_stride,

@@ -89,20 +89,34 @@ int launch_append(const DeviceInfo& d, int hd, const qz::kv4::AppendArgs& a, cud
                   : launch_kv4(qz::kv4::append_kernel<T, 128>, grid, qz::kv4::kAppendThreads, 0, st, a);
 }
 
-// 4 queries (row, head) of a kv head per item where no request has more, else
-// 8; the grid is the CTAs that fit the GPU at once.
-int attn_blocks(int64_t max_rows, int group) { return max_rows * group > 4 ? 2 : 1; }
+// Blocks of 4 queries (row, head) of a kv head per item of the split kernel: one where
+// no request has more than 8, else two. 8 kv heads of 128, bf16, one and two blocks:
+// 64 x 2048 positions, 8 queries 40.3 and 45.1 us, 16 59.0 and 60.9; 1 x 16384
+// positions, 8 queries 21.7 and 21.2, 16 28.5 and 26.7, 32 45.1 and 36.1.
+int attn_blocks(int64_t max_rows, int group) { return max_rows * group > 8 ? 2 : 1; }
 
 struct Kv4AttnLayout {
   int grid;
   int64_t part_off, sums_off, total;
 };
 
-// Requests with more rows than this (and heads that fit a tile) take the
-// tensor-core kernel's 128-row tiles, the others the split kernel.
-constexpr int kTcMinQueries = 32;
-int64_t split_rows(int group) {
+// Requests with more rows than this may take the tensor-core kernel, whose items are
+// 128 queries of a kv head over the whole context: with 64 of them real the split kernel
+// is as fast (64 requests x 2048 positions, fp32: 138 and 140 us; 128 queries: 250 and
+// 140). Groups that fit no tile take the split kernel.
+constexpr int kTcMinQueries = 64;
+int64_t tc_rows(int group) {
   return group > qz::kv4::kTcRows ? 0x7FFFFFFF : std::max(1, kTcMinQueries / group);
+}
+
+// ... and do where its items fill half of the GPU at least, as far as the host can tell
+// (all rows but one per request, or the most of one request). The split kernel shares out
+// positions too: 8 items over 16384 positions take it 112 us, the other 344; 64 items
+// over 2048 positions 51 and 72; a tile of the one is 2.3 us an SM, its work in the other
+// 30 ns of the whole GPU, so that they meet at 78 items.
+int64_t split_rows(const DeviceInfo& d, int64_t B, int64_t n, int64_t max_rows, int group, int nkv) {
+  const int64_t rows = std::max(n - B + 1, std::min(n, max_rows));
+  return nkv * qz::cdiv(rows * group, qz::kv4::kTcRows) < d.sms / 2 ? 0x7FFFFFFF : tc_rows(group);
 }
 
 Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int64_t max_rows, int group, int hd, bool wide) {
@@ -113,7 +127,7 @@ Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int64_t max_rows, int group, 
   // serves calls of different shapes in turn
   l.part_off = qz::cdiv(int64_t(d.sms) * qz::kv4::kAttnMaxPerSm * 4, 256) * 256;
   l.sums_off = l.part_off + qz::cdiv(int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4, 256) * 256;
-  l.total = l.sums_off + (max_rows > split_rows(group) ? int64_t(d.sms) * qz::kv4::kTcRows * hd * 4 : 0);
+  l.total = l.sums_off + (max_rows > tc_rows(group) ? int64_t(d.sms) * qz::kv4::kTcRows * hd * 4 : 0);
   return l;
 }
 
@@ -178,7 +192,7 @@ int qz_kv4_plan(const int64_t* lens, const int64_t* new_rows, int64_t B, int32_t
                         meets(used_out, 1, new_rows, B) || meets(used_out, 1, used, 1);
   const int64_t ctas = (rows + qz::kv4::kPlanThreads - 1) / qz::kv4::kPlanThreads;
   const int cluster = large && in_place ? qz::kv4::kPlanCluster : 1;
-  const int grid = !large || in_place ? cluster : static_cast<int>(ctas < 1 ? 1 : (ctas > d->sms ? d->sms : ctas));
+  const int grid = in_place ? cluster : static_cast<int>(ctas < 1 ? 1 : (ctas > d->sms ? d->sms : ctas));
   return launch_kv4(qz::kv4::plan_kernel, grid, qz::kv4::kPlanThreads, smem,
                     static_cast<cudaStream_t>(stream), a, cluster);
 }
@@ -312,8 +326,8 @@ int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_h
   a.scale = scale * 1.44269504088896341f;
   a.vec = rows_aligned(q, q_row_stride, q_head_stride, dtype);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t few = split_rows(group);
-  if (max_rows > few) {
+  const int64_t few = split_rows(*d, B, n, max_rows, group, nkv);
+  if (few < 0x7FFFFFFF && max_rows > few) {
     qz::kv4::TcArgs t{a, 0, d->sms, reinterpret_cast<float4*>(static_cast<char*>(ws) + L.sums_off)};
     t.out_vec = rows_aligned(out, out_row_stride, out_head_stride, dtype);
     t.a.rows_lo = static_cast<int>(few);
