@@ -36,6 +36,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -92,9 +93,10 @@ def _bind_fast(idx: int) -> None:
     if _fast is None:
         try:
             from . import _fastcall
-        except ImportError as e:
-            raise ImportError("quartz_b200/_fastcall.so is missing or does not load: build it with "
-                              "`python -m quartz_b200.build`") from e
+        except ImportError as e:      # the same kernels, 4 to 9 us more for each paged-cache call
+            warnings.warn(f"quartz_b200/_fastcall.so does not load ({e}): build it with "
+                          "`python -m quartz_b200.build`", RuntimeWarning, stacklevel=3)
+            return
         lib = _lib.load()
         _fastcall.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
             "qz_kv4_plan", "qz_kv4_append", "qz_kv4_gather", "qz_kv4_attention",
@@ -879,7 +881,8 @@ def _kv4_default_ws(idx: int, stream: int, need: int) -> torch.Tensor:
     if ws is None or ws.numel() < need:
         ws = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", idx))
         _kv4_ws[idx, stream] = ws
-        _fast.workspace(idx, stream, ws.data_ptr(), ws.numel())
+        if _fast is not None:
+            _fast.workspace(idx, stream, ws.data_ptr(), ws.numel())
     return ws
 
 
@@ -895,7 +898,8 @@ def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=No
     request b's. max_rows: the most rows a request has (a host number; rows of
     a request with more are not computed). scale: hd ** -0.5 unless given.
     Returns out (q's dtype); rows of no request are left as they were. out may
-    be q itself."""
+    be q itself, but must not overlap it otherwise. n, B and max_rows choose
+    between two kernels, whose results differ by rounding."""
     if _fast is not None:
         r = _fast.attention(q, pool, block_table, lens, cu_rows, max_rows, scale, out, workspace)
         if r is not None:

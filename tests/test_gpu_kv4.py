@@ -821,3 +821,30 @@ def test_few_tiles_and_many_tiles_agree():
     b = torch.full_like(q, 7.0)
     qd.kv4_attention(q, pool, table, _i64([700], dev), cu_rows=_i64([0, 300], dev), max_rows=300, out=b)
     assert (a - b[:300]).abs().max() < 2e-5 and (b[300:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+def test_any_scale(dtype, scale):
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(33)
+    lens = [200, 0, 90]
+    pool, table = _context(lens, 2, 128, 16, g, dev)
+    q = torch.randn(200, 4, 128, generator=g, device=dev).to(DTYPES[dtype])
+    _check_attention(q[:3], pool, table, lens, None, scale=scale)
+    _check_attention(q, pool, table, lens, [0, 120, 120, 200], scale=scale, max_rows=120)
+
+
+def test_lengths_below_zero_and_beyond_any_table():
+    """Lengths that no caller should hold: nothing is seen, or all that the table has."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(34)
+    pool, table = _context([64, 64, 64], 2, 64, 16, g, dev)
+    for n, pad in ((1, 0), (70, 0), (70, 6000)):
+        q = torch.randn(3 * n + pad, 4, 64, generator=g, device=dev)
+        cu = _i64([0, n, 2 * n, 3 * n], dev)
+        out = qd.kv4_attention(q, pool, table, _i64([-(1 << 62), -1, 1 << 62], dev), cu_rows=cu, max_rows=n)
+        assert (out[:2 * n] == 0).all()
+        full = qd.kv4_attention(q[2 * n:3 * n], pool, table[2:].repeat(n, 1)[:n], _i64([64] * n, dev))
+        assert (out[2 * n:3 * n] - full).abs().max() < 2e-5
+    qd.check_status()
