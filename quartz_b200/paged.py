@@ -17,7 +17,7 @@ requests; the plan advances lengths and the page cursor in place, so a replay
 needs nothing from the host. The host only keeps lengths (which it can count)
 and compacts the batch when a request ends.
 
-Differences of result from ``DecodeEngine``: K and V are 4-bit (11 to 13 % of
+Differences of result from ``DecodeEngine``: K and V are 4-bit (13 to 14 % of
 the fp32 cache's bytes), so logits differ by the quantisation.
 """
 
