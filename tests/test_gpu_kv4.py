@@ -848,3 +848,76 @@ def test_lengths_below_zero_and_beyond_any_table():
         full = qd.kv4_attention(q[2 * n:3 * n], pool, table[2:].repeat(n, 1)[:n], _i64([64] * n, dev))
         assert (out[2 * n:3 * n] - full).abs().max() < 2e-5
     qd.check_status()
+
+
+def test_the_most_requests():
+    """4096 requests in one call, some with prompts, against calls of 256 requests each."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(35)
+    rng = random.Random(35)
+    B, page, nkv, hd = 4096, 16, 2, 64
+    rows = [rng.choice([0, 1, 1, 2]) if b % 97 else 90 for b in range(B)]
+    lens = [max(n, rng.randrange(150)) for n in rows]
+    W = 10
+    table = torch.arange(B * W, dtype=torch.int32, device=dev).view(B, W)
+    pool = torch.randint(0, 256, (B * W, nkv, page * (hd + 8)), generator=g, device=dev, dtype=torch.uint8)
+    par = torch.rand(B * W, nkv, 2, page, 2, generator=g, device=dev)
+    pool[..., page * hd:] = (par - torch.tensor([0.0, 1.5], device=dev)).to(torch.bfloat16).view(torch.uint8).flatten(2)
+    cu = [0]
+    for n in rows:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1] + 5, 4, hd, generator=g, device=dev)
+    out = torch.full_like(q, 0.25)
+    qd.kv4_attention(q, pool, table, _i64(lens, dev), cu_rows=_i64(cu, dev), max_rows=90, out=out)
+    assert (out[cu[-1]:] == 0.25).all()
+    for b in range(0, B, 256):
+        c = cu[b:b + 257]
+        part = qd.kv4_attention(q[c[0]:c[-1]], pool, table[b:b + 256], _i64(lens[b:b + 256], dev),
+                                cu_rows=_i64([x - c[0] for x in c], dev), max_rows=90)
+        assert (part - out[c[0]:c[-1]]).abs().max() < 1e-4
+    with pytest.raises(ValueError, match="4096"):
+        qd.kv4_attention(q, pool, table[:1].repeat(4097, 1), torch.zeros(4097, dtype=torch.int64, device=dev),
+                         cu_rows=torch.zeros(4098, dtype=torch.int64, device=dev), max_rows=90)
+    qd.check_status()
+
+
+def test_a_plan_in_a_graph_advances_the_state():
+    """A captured plan, append and attention whose lengths and cursor are updated in place:
+    every replay is the next step."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(36)
+    B, page, nkv, hd, W = 5, 16, 2, 64, 8
+    lens, used = _i64([0, 15, 16, 3, 40], dev), _i64([0], dev)
+    start = lens.tolist()
+    free = torch.arange(60, dtype=torch.int32, device=dev)
+    table = torch.full((B, W), -1, dtype=torch.int32, device=dev)
+    pool = P.empty_pool(60, nkv, hd, page, 0, dev)
+    first = qd.kv4_plan(torch.zeros_like(lens), lens, table, free, used, page, sum(start), used_out=used)
+    held = torch.randn(sum(start), nkv, hd, generator=g, device=dev)
+    qd.kv4_append(held, -held, pool, first.slots)
+    one, k = torch.ones_like(lens), torch.randn(B, nkv, hd, generator=g, device=dev)
+    q, out = torch.randn(B, 4, hd, generator=g, device=dev), torch.zeros(B, 4, hd, device=dev)
+    ws = qd.kv4_attention_workspace(dev, 4, nkv, hd)
+
+    def step():
+        plan = qd.kv4_plan(lens, one, table, free, used, page, B, lens_out=lens, used_out=used)
+        qd.kv4_append(k, -k, pool, plan.slots)
+        qd.kv4_attention(q, pool, table, plan.lens, out=out, workspace=ws)
+
+    kept = [t.clone() for t in (lens, used, table)]
+    step()
+    for t, o in zip((lens, used, table), kept):
+        t.copy_(o)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        step()
+    for i in range(1, 30):
+        k.normal_(generator=g)
+        gr.replay()
+        now = [n + i for n in start]
+        assert lens.tolist() == now
+        assert used.item() == sum(-(-n // page) for n in now)
+        ref, _ = P.attention(q, pool, table, now, list(range(B + 1)), hd ** -0.5, out, 1)
+        assert (out - ref).abs().max() < 1e-4
+        own = [p for b, n in enumerate(now) for p in table[b, :-(-n // page)].tolist()]
+        assert len(set(own)) == len(own) and min(own) >= 0
