@@ -609,7 +609,9 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kv4_kernel(const RopeArg
 // small as their result. An MMA's accumulation truncates (about 3e-8 of the
 // accumulator each time), so for fp32 rows one or two MMAs start from zero, the sums are added up in fp32, and K is centred like V: with subnormal K
 // codes and accumulation in place, results were 1.3e-6 to 2.4e-6 off 64 bits. For
-// 16-bit rows both cheaper forms are far below the output's rounding. Row r of the
+// 16-bit rows both cheaper forms stay below the output's rounding: a CTA that takes
+// 131072 positions of a context leaves fp16 2.4e-4 off 64 bits where the rounding alone
+// is 2.1e-4 (at 2^20 positions 1.2e-3; bf16 2.1e-3 and 1.7e-3). Row r of the
 // eight positions an MMA fragment pairs up is position r / 2 + 4 (r & 1), so
 // that the V rows a quarter-warp reads are neighbours (fewer bank conflicts).
 //
