@@ -2,10 +2,11 @@
 // the paged 4-bit cache on the 5th-generation tensor cores (tcgen05 / TMEM).
 //
 // The same mathematics as attn_kernel (qz_kv4.cuh): the 4-bit codes are one
-// operand, exact in fp16; q and the weights p * s_v are the other. fp32 rows are
-// split into two fp16 limbs (22 bits); 16-bit rows take one: q then is exact
-// (bf16 and fp16 fit fp16 after the row's power of two) and the weights' 2^-11
-// is no more than the output's own rounding.
+// operand, exact in fp16; q and the weights p * s_v are the other. The weights are
+// split into two fp16 limbs (22 bits), and so is q of fp32 rows; q of 16-bit rows
+// takes one, which is exact (bf16 and fp16 fit fp16 after the row's power of two).
+// One limb for the weights of 16-bit rows would add an error of the size of fp16's
+// rounding (2^-12 each: results 2.6e-4 off 64 bits where the rounding is 2.1e-4).
 //
 // An item is 128 (row, head) pairs of one kv head; heads of a group share the
 // keys, so a tile is 128 / group query rows. Per tile of 128 positions
@@ -66,12 +67,12 @@ struct TcArgs {
 };
 
 // Tiles that O accumulates in TMEM before it is added to fp32 sums in the
-// workspace (L2). The MMA truncates its accumulator, 8 or 16 times a tile and by
-// about 3e-8 of it each time; without this, results drift by 1e-5 of themselves per
-// 40 tiles (fp32 rows; 3.4e-3 at 100000 positions). Even: the odd tiles' threads
-// do it, while the even ones work on the next tile. Every two tiles: 5e-7 off 64 bits
-// at 4096 positions, every four 1.1e-6 and 4 % faster. 16-bit rows round by 2^-12 at
-// least, 16 tiles drift by 4e-6.
+// workspace (L2). The MMA truncates its accumulator, 16 times a tile and by about
+// 3e-8 of it each time, so a chain of n tiles that grows evenly ends 16 n 3e-8 / 2
+// low: 1e-5 of itself after 40 tiles, 2e-4 after 100000 positions. Even: the odd
+// tiles' threads do it, while the even ones work on the next tile. fp32 rows, every
+// two tiles: 5e-7 off 64 bits at 4096 positions; every four 1.1e-6 and 4 % faster.
+// 16-bit rows round by 2^-12 at least, 16 tiles drift by 4e-6.
 template <int L>
 __host__ __device__ constexpr int tc_flush() { return L == 2 ? 2 : 16; }
 
@@ -300,10 +301,10 @@ __device__ __forceinline__ void tc_rescale(uint32_t taddr, float f, float d) {
   tmem_wait_st();
 }
 
-// Weights of 64 positions into TMEM, in place of x (limbs of 16 positions side by
-// side). SELECT: parameters of hidden positions may be NaN, so they are selected
+// Weights of 64 positions into TMEM, in place of x (the two limbs of 16 positions side
+// by side, as many columns as x). SELECT: parameters of hidden positions may be NaN, so they are selected
 // away; otherwise p = 0 makes their products vanish.
-template <int L, bool SELECT>
+template <bool SELECT>
 __device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, const float* zc,
                                            RowState& st) {
   uint32_t v[2][16];
@@ -314,7 +315,7 @@ __device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, cons
     tc::tmem_wait_ld();
     if (c < 3) tc::tmem_ld16(taddr + 16 * (c + 1), v[(c + 1) & 1]);
     const uint32_t(&x)[16] = v[c & 1];
-    uint32_t w[8 * L];
+    uint32_t w[16];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float4 s = reinterpret_cast<const float4*>(sv)[4 * c + q];
@@ -336,16 +337,14 @@ __device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, cons
         const float2 y = f2_unpack(y2);
         const __half2 hi = __floats2half2_rn(y.x, y.y);
         w[2 * q + e] = *reinterpret_cast<const uint32_t*>(&hi);
-        if constexpr (L == 2) {
-          const float2 back = __half22float2(hi);
-          const float2 d = f2_unpack(f2_sub(y2, f2_set(back.x, back.y)));
-          const __half2 lo = __floats2half2_rn(d.x, d.y);
-          w[8 + 2 * q + e] = *reinterpret_cast<const uint32_t*>(&lo);
-        }
+        const float2 back = __half22float2(hi);
+        const float2 d = f2_unpack(f2_sub(y2, f2_set(back.x, back.y)));
+        const __half2 lo = __floats2half2_rn(d.x, d.y);
+        w[8 + 2 * q + e] = *reinterpret_cast<const uint32_t*>(&lo);
       }
     }
-#pragma unroll
-    for (int k = 0; k < L; ++k) tmem_st8(taddr + c * (8 * L) + 8 * k, w + 8 * k);
+    tmem_st8(taddr + 16 * c, w);
+    tmem_st8(taddr + 16 * c + 8, w + 8);
   }
   st.l = f2_add(st.l, l);
   st.zs = f2_add(st.zs, zs);
@@ -353,7 +352,7 @@ __device__ __forceinline__ void tc_weights(uint32_t taddr, const float* sv, cons
 
 template <class T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs args) {
-  constexpr int L = sizeof(T) == 4 ? 2 : 1;      // fp16 limbs of q and of the weights
+  constexpr int L = sizeof(T) == 4 ? 2 : 1;      // fp16 limbs of q (the weights have two)
   constexpr int TB = tc_tile_bytes<HD>();
   constexpr int RB = tc_raw_bytes<HD>();
   constexpr int BLK = kTcKeys * 128;             // bytes of 64 dimensions of a tile
@@ -627,9 +626,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       const float* sv = sh.sv[ring] + half * 64;
       const float* zc = sh.zc[ring] + half * 64;
       if (sh.odd[ring])
-        tc_weights<L, true>(cols, sv, zc, st);
+        tc_weights<true>(cols, sv, zc, st);
       else
-        tc_weights<L, false>(cols, sv, zc, st);
+        tc_weights<false>(cols, sv, zc, st);
       tmem_wait_st();
       tc::tc_fence_before();
       mbar_arrive(smem_u32(&sh.p_full[odd]));
@@ -984,11 +983,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       const uint32_t w = tmem + kColS + (j & 1) * 128;
       if (leader) {
 #pragma unroll
-        for (int l = L - 1; l >= 0; --l)
+        for (int l = 1; l >= 0; --l)
 #pragma unroll
           for (int s = 0; s < kTcKeys / 16; ++s)
-            mma_f16_ts(tmem + kColO, w + (s >> 2) * 64 + (s & 3) * (8 * L) + 8 * l,
-                       vd + ((s * 2048) >> 4), id_o, !anew || s != 0 || l != L - 1);
+            mma_f16_ts(tmem + kColO, w + (s >> 2) * 64 + (s & 3) * 16 + 8 * l,
+                       vd + ((s * 2048) >> 4), id_o, !anew || s != 0 || l != 1);
         tc::tc_commit(smem_u32(&sh.v_empty[j & 1]));
       }
       __syncwarp();
