@@ -535,6 +535,8 @@ int qz_kv4_attention_workspace_bytes(int nq, int nkv, int hd, int64_t max_rows, 
  * their positions count as unseen. B <= 4096, width * page_size <= 2^30.
  * The result does not depend on timing. n, B and max_rows choose between two
  * kernels (few rows, or tiles of 128 queries); their results differ by rounding.
+ * What is lost of a value is relative to the row's largest p |v|, not to the largest
+ * |v|: a value of vanishing weight costs the others nothing, up to 2^90 times theirs.
  */
 int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_head_stride,
                      void* out, int64_t out_row_stride, int64_t out_head_stride,

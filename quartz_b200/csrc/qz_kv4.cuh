@@ -621,8 +621,10 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kv4_kernel(const RopeArg
 // (max, sum, accumulator) go to the workspace and the last of an item's CTAs
 // to arrive merges them in CTA order, so results do not depend on timing.
 //
-// The running maximum is only renewed when a score passes it by 2^4 (weights
-// stay below 2^4 relative to it): one vote per stage instead of a reduction.
+// The running maximum is only renewed when a score passes it by 2^3 (weights
+// stay below 2^3 relative to it): one vote per stage instead of a reduction. The
+// same vote sees to the power of two that brings a query's weights p sv into fp16's
+// range (see kAttnSpare).
 //
 // Measured: 64 x 16384 positions, 8 kv heads of 128, bf16 134 us (57 % of the copy
 // rate; ALU pipe 57 %, issue slots 57 %); 16 x 2048 fp32 17 us; one request of 131071
@@ -634,6 +636,12 @@ constexpr int kAttnStage = 32;    // positions per warp and stage
 constexpr int kAttnDepth = 3;     // stages of a warp
 constexpr int kAttnStep = kAttnWarps * kAttnStage;
 constexpr int kAttnMaxB = 4096;
+// Weights p sv enter the MMAs as fp16 pairs times up = 2^(11 - ev), so whatever lies
+// below 2^-25 of that scale is lost. ev is the exponent of the largest step sv seen, but
+// at most kAttnSpare above that of the largest p sv: a row of V with a large step and a
+// vanishing weight costs the others nothing (they keep 2^-26 of the largest weight), and
+// steps that differ by less than 2^10 need no attention from stage to stage.
+constexpr int kAttnSpare = 10;
 // What an item costs beside its positions (its query fragments, the merge), in
 // steps: the shares of short and long contexts take about as long.
 constexpr int kAttnItemUnits = 1;
@@ -719,8 +727,9 @@ __device__ __forceinline__ uint32_t split_h2(float x) {
   return pack_h2(hi, __float2half_rn(x - __half2float(hi)));
 }
 
-// 2^e for e in [-126, 127].
+// 2^e for e in [-126, 127], floor(log2 x) for a normal x >= 0 (-127 for what is smaller).
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+__device__ __forceinline__ int exponent(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127; }
 
 // The four position pairs of one 16-bit half of two rows' words, less 8:
 // h[n] = (d(row a, nibble n) - 8, d(row b, nibble n) - 8) as fp16.
@@ -805,6 +814,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
   int64_t* s_scan = reinterpret_cast<int64_t*>(attn_sh);                        // [threads]
   int64_t* s_at = reinterpret_cast<int64_t*>(attn_sh + kAttnThreads * 8);       // {b, its first unit}
   int* s_last = reinterpret_cast<int*>(s_at + 2);
+  float* s_wm = reinterpret_cast<float*>(attn_sh);                              // [threads][2], after s_scan
   float* s_o = reinterpret_cast<float*>(attn_sh + 2048);                        // [warps][Q][HD]
   float* s_ml = s_o + kAttnWarps * Q * HD;                                      // [warps][Q][2]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
@@ -983,8 +993,14 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[nb][t][j] = 0.f;
     }
-    int ev = -100;                       // weights are p * s * 2^(9 - ev)
-    float s_lim = pow2i(ev + 1), w_up = pow2i(9 - ev);
+    // a query's weights are p sv up; wm: their largest when up was last settled, without up
+    float up[NB];
+    volatile float* wm = s_wm + tid * 2;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      up[nb] = pow2i(111);               // ev = -100
+      wm[nb] = 0.f;
+    }
 
     // ---- stages of this warp ---------------------------------------------------
     const int32_t* tab = a.table + b * a.width;
@@ -1102,23 +1118,18 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
               }
           }
       }
-      float top[NB], sm = 0.f;
+      float top[NB], sm[NB];
       bool renew = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         top[nb] = fmaxf(fmaxf(x[0][0][nb], x[0][1][nb]), fmaxf(x[1][0][nb], x[1][1][nb]));
-        renew = renew || top[nb] > m[nb] + 4.f;
-        sm = fmaxf(fmaxf(sm, fmaxf(par_s(vp[0][0][nb]), par_s(vp[0][1][nb]))),
-                   fmaxf(par_s(vp[1][0][nb]), par_s(vp[1][1][nb])));
+        sm[nb] = fmaxf(fmaxf(fmaxf(0.f, par_s(vp[0][0][nb])), par_s(vp[0][1][nb])),
+                       fmaxf(par_s(vp[1][0][nb]), par_s(vp[1][1][nb])));
+        // p < 2^3 and sv up < 2^12
+        renew = renew || top[nb] > m[nb] + 3.f || sm[nb] * up[nb] >= 4096.f;
       }
-      if (__any_sync(0xffffffffu, renew || sm >= s_lim)) {
-        // new maximum per query and new exponent of V's steps
-        const int es = static_cast<int>((__reduce_max_sync(0xffffffffu, __float_as_uint(sm)) >> 23) & 255u) - 127;
-        const int ev_old = ev;
-        ev = es > ev ? (es > 127 ? 127 : es) : ev;
-        s_lim = ev >= 127 ? INFINITY : pow2i(ev + 1);
-        w_up = pow2i(9 - ev);
-        const float down = ev_old - ev < -126 ? 0.f : pow2i(ev_old - ev);
+      if (__any_sync(0xffffffffu, renew)) {
+        // new maximum and new scale of every query
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           float t = top[nb];
@@ -1128,12 +1139,29 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
           const float al = m[nb] == kNegInf ? 1.f : ex2(m[nb] - mn);
           m[nb] = mn;
           rel[nb] = mn == kNegInf ? 0.f : mn;
+          float w = wm[nb] * al, sv = sm[nb];
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) w = fmaxf(w, ex2(x[h2][r][nb] - rel[nb]) * par_s(vp[h2][r][nb]));
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+            sv = fmaxf(sv, __shfl_xor_sync(0xffffffffu, sv, o));
+          }
+          wm[nb] = w;
+          const int ew = exponent(w), ev_old = 11 - exponent(up[nb]);
+          int ev = max(ev_old, exponent(sv));
+          ev = max(ew, min(ev, ew + kAttnSpare));
+          ev = min(max(ev, -100), 127);
+          up[nb] = pow2i(11 - ev);
+          const float down = al * pow2i(min(max(ev_old - ev, -126), 127));
           l[nb] *= al;
           zs[nb] *= al;
 #pragma unroll
           for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[nb][k][j] *= al * down;
+            for (int j = 0; j < 4; ++j) acc[nb][k][j] *= down;
         }
       }
       // weights of 16 positions: (hi, lo) of each row's side by side, transposed
@@ -1146,7 +1174,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
             const float p = ex2(x[t][r][nb] - rel[nb]), sv = par_s(vp[t][r][nb]);
             l[nb] += p;
             zs[nb] = fmaf(p, fmaf(8.f, sv, par_z(vp[t][r][nb])), zs[nb]);
-            w[r] = p * (sv * w_up);
+            w[r] = (p * sv) * up[nb];
           }
           const __half2 hi = __floats2half2_rn(w[0], w[1]);
           const float2 back = __half22float2(hi);
@@ -1242,9 +1270,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
     __syncthreads();   // the rings are done with: the results take their place
 
     // ---- the warps' partials, relative to each warp's maximum -----------------
-    const float w_down = pow2i(ev - 9);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
+      const float w_down = __uint_as_float(0x7F000000u - __float_as_uint(up[nb]));   // 1 / up
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], o);

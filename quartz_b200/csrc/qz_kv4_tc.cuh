@@ -32,6 +32,15 @@
 //         memory, kTcRaw tiles ahead
 //   22    issues the MMAs: S(t + 1) before O(t), so that the next scores are
 //         ready when the softmax of this tile ends
+// A row's weights p s_v go into fp16 as p s_v 2^(10 - ev), p relative to the row's
+// running maximum (below 2^4) and ev the largest exponent so far of a position's
+// u = max(s_v, |z_v + 8 s_v| / 8), a bound of what a code can add; what lies below
+// 2^-25 of that is lost. While all u seen lie within 2^8 of each other a row's largest
+// weight keeps 2^-26 of itself, whatever its scores. Where they do not (`wide`, from
+// that tile of an item on), a row with no weight near the largest u is taken relative
+// to less than its maximum, as far as its largest p u asks for: tiles then take the
+// largest of score + log2 u of each row too.
+//
 // K and V tiles of a position row hold their dimensions in nibble order
 // (0 4 1 5 2 6 3 7 of each word); Q is stored in the same order, and the
 // epilogue puts O's columns back.
@@ -57,6 +66,7 @@ constexpr int kTcKeys = 128;    // positions per tile
 // the softmax is at most kTcRaw + 1 tiles behind.
 constexpr int kTcRing = 8;
 constexpr int kTcRaw = 3;       // stages of packed tiles
+constexpr int kTcSpare = 8;     // how far u's exponents may spread before `wide`
 constexpr uint32_t kColQ = 0, kColO = 128, kColS = 256;
 
 struct TcArgs {
@@ -97,16 +107,21 @@ __host__ __device__ constexpr int tc_raw_bytes() { return kTcKeys * (HD + 8); }
 // columns) occupies an SM.
 struct TcShared {
   float sk[kTcRing][kTcKeys], zk[kTcRing][kTcKeys];   // K's step, zero (+ 8 step if centred)
-  float sv[kTcRing][kTcKeys], zc[kTcRing][kTcKeys];   // V's step * 2^(9 - ev), zero + 8 step
+  float sv[kTcRing][kTcKeys], zc[kTcRing][kTcKeys];   // V's step * 2^(10 - ev), zero + 8 step
+  float lu[kTcRing][kTcKeys];   // log2(u) + 10 - ev
   alignas(16) uint32_t valid[kTcRing][4];   // positions that exist, one bit each
   float down[kTcRing];          // 2^(ev before - ev): O's factor when V's exponent grows
-  float w_down[kTcRing];        // 2^(ev - 9)
+  float w_down[kTcRing];        // 2^(ev - 10)
+  uint32_t wide[kTcRing];       // the u so far differ by more than 2^kTcSpare
   float top[2][2][kTcRows];     // [tile & 1][half]: maximum of a row's half tile
-  float max[2][kTcRows];        // [tile & 1]: a row's maximum so far
+  float topu[2][2][kTcRows];    // and of score + lu, of all tiles so far (wide tiles only)
+  float max[2][kTcRows];        // [tile & 1]: what a row's scores are taken relative to
+  // [tile & 1]: the largest score and score + lu so far, relative to `max` (wide tiles only)
+  float peak[2][kTcRows], peaku[2][kTcRows];
   // exchange between a row's four threads, when q is read and at the end (a group
   // without a tile reaches the end while others still read q)
   float ex_q[2][4][kTcRows], ex[3][4][kTcRows];
-  // [half]: what a row's sums in the workspace stand relative to, its maximum and w_down
+  // [half]: what a row's sums in the workspace stand relative to, and their w_down
   float flushed[2][kTcRows], flushed_w[2][kTcRows];
   int place;                    // in the workspace, or -1
   uint32_t odd[kTcRing];        // a V parameter of the tile is not finite
@@ -237,12 +252,13 @@ __device__ __forceinline__ bool warp_wait(const uint64_t* bar, uint32_t parity) 
 
 // What a thread has summed of its row, relative to 2^m.
 struct RowState {
-  float m;         // maximum
+  float m;         // what the sums stand relative to
   f2_t l, zs;      // sum of p, sum of p (z_v + 8 s_v)
 };
 
-// x = score + mu of 64 positions, in TMEM in place of S; returns their maximum. MASK: positions that do not exist (bits of
-// `valid`) or lie at `lim` or behind it, counted from the first, become -inf.
+// x = score + mu of 64 positions, in TMEM in place of S; returns their maximum. MASK: positions
+// that do not exist (bits of `valid`) or lie at `lim` or behind it, counted from the first, become
+// -inf.
 template <bool MASK>
 __device__ __forceinline__ float tc_scores(uint32_t taddr, const float* sk, const float* zk, f2_t F2,
                                            f2_t Q2, f2_t mu2, const uint32_t* valid, int lim) {
@@ -283,6 +299,20 @@ __device__ __forceinline__ float tc_scores(uint32_t taddr, const float* sk, cons
   }
   tmem_wait_st();
   return fmaxf(t0, t1);
+}
+
+// The maximum of x + lu over 64 positions.
+__device__ __forceinline__ float tc_top_u(uint32_t taddr, const float* lu) {
+  float t = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 64; c += 16) {
+    uint32_t x[16];
+    tc::tmem_ld16(taddr + c, x);
+    tc::tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t = fmaxf(t, __uint_as_float(x[k]) + lu[c + k]);
+  }
+  return t;
 }
 
 // n columns of this row times f plus d.
@@ -589,7 +619,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       const float* zk = sh.zk[ring] + half * 64;
       float top = whole ? tc_scores<false>(cols, sk, zk, F2, Q2, mu2, nullptr, 0)
                         : tc_scores<true>(cols, sk, zk, F2, Q2, mu2, &sh.valid[ring][2 * half], lim - p0);
-      // both halves' maximum; the four arrays it takes are free again once O(j) is issued
+      const bool wide = sh.wide[ring] != 0u;
+      float topu = kNegInf, peak = kNegInf;
+      if (wide) {
+        topu = tc_top_u(cols, sh.lu[ring] + half * 64);
+        if (before != kNegInf) {
+          // Of the tiles before: what was agreed on, or, when those were not wide, p in
+          // [1, 2^4] and u of 2^-kTcSpare of the largest at least.
+          const bool was = j > 0 && sh.wide[(j - 1) & (kTcRing - 1)] != 0u;
+          peak = was ? sh.peak[odd ^ 1][r] : 4.f;
+          topu = fmaxf(topu, (was ? sh.peaku[odd ^ 1][r] : 10.f - kTcSpare) + __log2f(sh.down[ring]));
+        }
+        sh.topu[odd][half][r] = topu;
+      }
+      // both halves' maximum; the arrays it takes are free again once O(j) is issued
       sh.top[odd][half][r] = top;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.t_full[odd][quarter]));
@@ -598,7 +641,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       top = fmaxf(top, sh.top[odd][half ^ 1][r]);
       // a maximum that rose by more than 2^4 is renewed (x stands relative to -mu)
       float now = before;
-      if (top > (before == kNegInf ? kNegInf : 4.f)) now = fmaxf(before, top - mu);
+      if (wide) {
+        topu = fmaxf(topu, sh.topu[odd][half ^ 1][r]);
+        peak = fmaxf(peak, top);
+        // by how much the reference moves: p u 2^(10 - ev) of 2^10 to 2^11 where it has left
+        // [2^2, 2^14], and no p above 2^90
+        float d = 0.f;
+        if (topu == kNegInf)
+          d = before == kNegInf || top > 4.f ? top : 0.f;
+        else if (before == kNegInf || topu > 14.f || topu < 2.f)
+          d = floorf(topu) - 10.f;
+        d = fmaxf(d, peak - 90.f);
+        now = (before == kNegInf ? 0.f : before) + d;
+        if (half == 0) {
+          sh.peak[odd][r] = peak - d;
+          sh.peaku[odd][r] = topu - d;
+        }
+      } else if (top > (before == kNegInf ? kNegInf : 4.f)) {
+        now = fmaxf(before, top - mu);
+      }
       if (half == 0) {
         sh.max[odd][r] = now;
         __syncwarp();
@@ -676,14 +737,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
     }
     if (failed && lane == 0) report_error(ERR_WAIT_FULL, 0x400u);
-    // ---- epilogue: the four threads' sums, relative to the last maximum ------------
+    // ---- epilogue: the four threads' sums, relative to what the last tile's are -----
     const float2 lt = f2_unpack(st.l), zt = f2_unpack(st.zs);
     sh.ex[0][part][r] = st.m;
     sh.ex[1][part][r] = lt.x + lt.y;
     sh.ex[2][part][r] = zt.x + zt.y;
     named_bar_sync(1 + quarter, 128);
-    // (odd tiles' sums have the maximum of theirs: parts 1 and 3)
-    const float mf = fmaxf(sh.ex[0][0][r], sh.ex[0][1][r]);
+    // (parts 0 and 2 had the even tiles, 1 and 3 the odd ones)
+    const float mf = sh.ex[0][(nt - 1) & 1][r];
     float l = 0.f, zs = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -833,10 +894,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   regs_less<56>();
   if (warp == 20) {
     // ======================= parameters ====================================
-    // weights are p * s_v * 2^(9 - ev), ev the largest exponent of s_v so far
+    // weights are p * s_v * 2^(10 - ev), ev the largest exponent of u so far
     const int s7 = a.shift < 7 ? a.shift : 7, cnt = 1 << s7;
     const int seen = seen_by(), nt = (seen + kTcKeys - 1) / kTcKeys;
-    int ev = -100;
+    int ev = -100, least = 127;              // the largest and the smallest exponent of u
 #pragma unroll 1
     for (int j = 0; j < nt; ++j) {
       const int ring = j & (kTcRing - 1), st = j % kTcRaw;
@@ -846,7 +907,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
       const uint32_t groups = sh.raw_groups[st];
       uint32_t kp[4], vp[4];
-      float mx = 0.f;
+      float mx = 0.f, mn = INFINITY, u[4];
       bool odd = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -860,15 +921,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         }
         const uint32_t bits = __ballot_sync(0xffffffffu, here);
         if (lane == 0) sh.valid[ring][k] = bits;
-        mx = fmaxf(mx, par_s(vp[k]));
+        u[k] = fmaxf(par_s(vp[k]), 0.125f * fabsf(fmaf(8.f, par_s(vp[k]), par_z(vp[k]))));
+        mx = fmaxf(mx, u[k]);
+        mn = here ? fminf(mn, u[k]) : mn;
         odd = odd || !isfinite(par_s(vp[k])) || !isfinite(par_z(vp[k]));
       }
       mbar_arrive(smem_u32(&sh.raw_empty[st]));
-      int e = static_cast<int>((__reduce_max_sync(0xffffffffu, __float_as_uint(mx)) >> 23) & 255u) - 127;
-      e = e > 127 ? 127 : e;
+      const int e = exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx))));
+      const int f = exponent(__uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(mn))));
       const int ev_old = ev;
-      ev = e > ev ? e : ev;
-      const float up = pow2i(9 - ev);
+      ev = min(max(e, ev), 127);
+      least = min(least, max(f, -100));
+      const float up = pow2i(10 - ev);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int p = lane + 32 * k;
@@ -877,12 +941,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         sh.zk[ring][p] = L == 2 ? fmaf(8.f, par_s(kp[k]), par_z(kp[k])) : par_z(kp[k]);
         sh.sv[ring][p] = sv * up;
         sh.zc[ring][p] = fmaf(8.f, sv, par_z(vp[k]));
+        sh.lu[ring][p] = __log2f(u[k]) + (10.f - ev);
       }
       odd = __any_sync(0xffffffffu, odd);
       if (lane == 0) {
         sh.odd[ring] = odd ? 1u : 0u;
         sh.down[ring] = j == 0 ? 1.f : (ev_old - ev < -126 ? 0.f : pow2i(ev_old - ev));
-        sh.w_down[ring] = pow2i(ev - 9);
+        sh.w_down[ring] = pow2i(ev - 10);
+        sh.wide[ring] = ev - least > kTcSpare ? 1u : 0u;
       }
       mbar_arrive(smem_u32(&sh.par_full[ring]));
     }

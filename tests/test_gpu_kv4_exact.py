@@ -69,3 +69,74 @@ def test_prompts_of_16_bits_round_once(dtype, most, hd):
     other = (got != ref.to(got.dtype)).double().mean().item()
     assert other < most, other
     qd.check_status()
+
+
+# rows of the request, heads: one row and a few take the split kernel with one and two
+# blocks of queries, 1300 rows the tiles
+FORMS = {"one": (1, 8), "few": (5, 8), "tiles": (1300, 8)}
+
+
+def _check_sums(got, ref, size, score_err):
+    """|got - ref| <= size (2 score_err + 2^-19) and the rounding: every weight is off by
+    the error of its score and 2^-20 of exponent and split, the sum of the weights too,
+    and size is the sum of the weighted |v|."""
+    eps = torch.finfo(got.dtype).eps / 2
+    bound = size * (2 * score_err + 2.0 ** -19) + ref.abs() * eps + torch.finfo(got.dtype).tiny
+    assert torch.isfinite(got).all()
+    over = ((got.double() - ref).abs() / bound).max().item()
+    assert over <= 1, over
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("at", [(0, 77), (900, 1350), (100, 2300, 4000)])
+@pytest.mark.parametrize("ratio", [12, 24, 40, 100])
+def test_a_large_value_without_weight_costs_nothing(ratio, at, form, hd, dtype):
+    """Some V rows 2^ratio times the others, with 2^-100 of the weight and less: their p |v|
+    is nothing, and the result is what fp32 sums of p v give. The ordinary scores have
+    A = scale * sum |q k| below 20 (128 products of unit normals, and 8 * 0.3), so they
+    are off by at most 4 A (hd / 16 + 8) 2^-23; those rows' A is larger, but not their
+    share."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(ratio)
+    rows, nq = FORMS[form]
+    nkv, t = 2, 1400 if max(at) < 1400 else 4200
+    k, v = (torch.randn(t, nkv, hd, generator=g, device=dev) for _ in range(2))
+    q = torch.randn(rows, nq, hd, generator=g, device=dev).to(DTYPES[dtype])
+    # along dimension 0 the queries have 8 and only those keys anything: their scores lie
+    # scale * 8 * x = 70 + ratio ln 2 below the others', about
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    for p in at:
+        k[p] = 0.0
+        k[p, :, 0] = -(70 + ratio * math.log(2)) / 8 * hd ** 0.5
+        v[p] *= 2.0 ** ratio
+    pool, table = _pool_of(k, v, 16)
+    got = qd.kv4_attention(q, pool, table, _i64([t], dev), cu_rows=_i64([0, rows], dev), max_rows=rows)
+    ref, size = _exact(q, pool, t, rows)
+    _check_sums(got, ref, size, 4 * 20 * (hd / 16 + 8) * 2.0 ** -23)
+    qd.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("kind", ["zero", "constant", "tiny"])
+def test_a_position_that_takes_the_weight_but_has_no_value(kind, form, dtype):
+    """The first position has nearly all the weight and a V row of zeros (or of one value,
+    with no steps, or of 2^-40): what the others add is small and still theirs."""
+    qd, dev = _dev()
+    hd, nkv, t = 64, 2, 1400
+    g = torch.Generator(device=dev).manual_seed(7)
+    rows, nq = FORMS[form]
+    k, v = (torch.randn(t, nkv, hd, generator=g, device=dev) for _ in range(2))
+    q = torch.randn(rows, nq, hd, generator=g, device=dev).to(DTYPES[dtype])
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[0] = 0.0
+    k[0, :, 0] = 40.0                                   # a score of 40, e^40 = 2^58
+    v[0] = {"zero": 0.0, "constant": 2.0 ** -30, "tiny": 2.0 ** -40}[kind] * (v[0] if kind == "tiny" else 1)
+    pool, table = _pool_of(k, v, 16)
+    got = qd.kv4_attention(q, pool, table, _i64([t], dev), cu_rows=_i64([0, rows], dev), max_rows=rows)
+    ref, size = _exact(q, pool, t, rows)
+    # the first position's score has A = 40, and all weights are relative to it
+    _check_sums(got, ref, size, 4 * 40 * (hd / 16 + 8) * 2.0 ** -23)
+    qd.check_status()
