@@ -516,8 +516,9 @@ int qz_qk_rope_kv4(const float* qkv, const float* q_norm_w, const float* k_norm_
                    const int64_t* slots, float eps, void* stream);
 
 /* Workspace bytes of qz_kv4_attention on the current device (256-byte aligned,
- * zeroed once before its first use and left ready for the next call; calls
- * sharing it must not overlap on the GPU). */
+ * its first QZ_KV4_WORKSPACE_HEAD bytes zeroed once before its first use and left
+ * ready for the next call; calls sharing it must not overlap on the GPU). */
+#define QZ_KV4_WORKSPACE_HEAD 16384
 int qz_kv4_attention_workspace_bytes(int nq, int nkv, int hd, int64_t max_rows, int64_t* bytes);
 
 /*

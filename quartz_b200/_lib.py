@@ -22,6 +22,8 @@ QZ_ERR_UNSUPPORTED = 3
 QZ_ACT_NONE, QZ_ACT_RMSNORM, QZ_ACT_SILU_MUL = 0, 1, 2
 # dtypes of the paged cache's rows (include/quartz_b200.h)
 QZ_F32, QZ_BF16, QZ_F16 = 0, 1, 2
+# the part of kv4_attention's workspace that starts as zeros (include/quartz_b200.h)
+QZ_KV4_WORKSPACE_HEAD = 16384
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int

@@ -607,11 +607,12 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kv4_kernel(const RopeArg
 // halves of two positions' words; 0x6400 | d is 1024 + d, and one HADD2 (HFMA2
 // for the nibbles four bits higher) leaves d - 8. Centring V keeps the sums as
 // small as their result. An MMA's accumulation truncates (about 3e-8 of the
-// accumulator each time), so for fp32 rows one or two MMAs start from zero, the sums are added up in fp32, and K is centred like V: with subnormal K
-// codes and accumulation in place, results were 1.3e-6 to 2.4e-6 off 64 bits. For
-// 16-bit rows both cheaper forms stay below the output's rounding: a CTA that takes
-// 131072 positions of a context leaves fp16 2.4e-4 off 64 bits where the rounding alone
-// is 2.1e-4 (at 2^20 positions 1.2e-3; bf16 2.1e-3 and 1.7e-3). Row r of the
+// accumulator each time), so for fp32 rows one or two MMAs start from zero, the sums
+// are added up in fp32, and K is centred like V: with subnormal K codes and
+// accumulation in place, results were 1.3e-6 to 2.4e-6 off 64 bits. 16-bit rows take
+// both cheaper forms for up to kAttnFlush stages, 128 MMAs that leave 2e-6; then a
+// warp's sums go to fp32 sums of its own in the workspace (fp32 sums in registers
+// spill at four CTAs per SM). Row r of the
 // eight positions an MMA fragment pairs up is position r / 2 + 4 (r & 1), so
 // that the V rows a quarter-warp reads are neighbours (fewer bank conflicts).
 //
@@ -636,6 +637,10 @@ constexpr int kAttnStage = 32;    // positions per warp and stage
 constexpr int kAttnDepth = 3;     // stages of a warp
 constexpr int kAttnStep = kAttnWarps * kAttnStage;
 constexpr int kAttnMaxB = 4096;
+// Steps of positions (so stages of a warp) between the places where a warp's sums of
+// 16-bit rows leave the MMA's accumulator: after steps 63, 127, ... of an item (a power
+// of two).
+constexpr int kAttnFlush = 64;
 // Weights p sv enter the MMAs as fp16 pairs times up = 2^(11 - ev), so whatever lies
 // below 2^-25 of that scale is lost. ev is the exponent of the largest step sv seen, but
 // at most kAttnSpare above that of the largest p sv: a row of V with a large step and a
@@ -655,6 +660,7 @@ struct AttnArgs {
   const int64_t* lens;
   const int64_t* cu;                // [B + 1] or null: request b has row b
   float* part;
+  float* sums;                      // [CTAs][warps][attn_sum_floats][32]; not used for fp32 rows
   unsigned int* tickets;
   int64_t pages, width, n;
   int B, nkv, group, shift;
@@ -673,6 +679,8 @@ template <int HD, int NB>
 __host__ __device__ constexpr int attn_queries() { return 4 * NB; }
 template <int HD, int NB>
 __host__ __device__ constexpr int attn_part_floats() { return 4 * NB * (HD + 2); }
+// A lane's share of a warp's sums, and the maximum of each query that they stand relative to.
+__host__ __device__ constexpr int attn_sum_floats(int hd, int nb) { return nb * (hd / 8 + 1); }
 template <int HD>
 __host__ __device__ constexpr int attn_stage_bytes() { return kAttnStage * (HD + 8); }
 constexpr int kAttnHead = kAttnThreads * 8 + 64 + kAttnWarps * kAttnDepth * 8;
@@ -1003,6 +1011,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
     }
 
     // ---- stages of this warp ---------------------------------------------------
+    float* const own_sums = a.sums + static_cast<size_t>(blockIdx.x * kAttnWarps + warp) *
+                                         (attn_sum_floats(HD, NB) * 32) + lane;
     const int32_t* tab = a.table + b * a.width;
     const int t_end = s1 * kAttnStep < seen ? s1 * kAttnStep : seen;
     int pos = s0 * kAttnStep + warp * kAttnStage;
@@ -1039,233 +1049,259 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
         k = k + 1 == kAttnDepth ? 0 : k + 1;
       }
     }
-    for (; pos < t_end; pos += kAttnStep) {
-      if (ahead < t_end) issue(st == 0 ? kAttnDepth - 1 : st - 1);   // the stage used last
-      const bool landed = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, phase));
-      if (!landed) {   // reported; the copy gets as long again before its place is used
-        if (lane == 0) report_error(ERR_WAIT_FULL, 0x430u);
-        mbar_wait(bars + 8 * st, phase);
-      }
-      const uint32_t base = ring + st * SB, half_ok = landed ? (there >> (2 * st)) & 3u : 0u;
-      const bool whole = half_ok == 3u && pos + kAttnStage <= all_see;
-      // scores of rows g, g + 8 of both halves, and their V parameters
-      float x[2][2][NB];
-      uint32_t vp[2][2][NB];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        uint32_t k0[KW], k1[KW], kp[2], one[1];
-        lds(base + k_at + t * k_next, k0);
-        lds(base + k_at + t * k_next + 8 * (HD / 2), k1);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          lds(base + p_at + t * p_next + 32 * r, one);
-          kp[r] = one[0];
-          lds(base + p_at + t * p_next + 32 * r + blk * 4, one);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) vp[t][r][nb] = one[0];
+    // 16-bit rows: where the chain of MMAs ends; whether one did
+    int stop = kWide ? t_end : min(t_end, (s0 / kAttnFlush + 1) * (kAttnFlush * kAttnStep));
+    bool flushed = false;
+#pragma unroll 1
+    while (true) {
+#pragma unroll 1
+      for (; pos < stop; pos += kAttnStep) {
+        if (ahead < t_end) issue(st == 0 ? kAttnDepth - 1 : st - 1);   // the stage used last
+        const bool landed = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, phase));
+        if (!landed) {   // reported; the copy gets as long again before its place is used
+          if (lane == 0) report_error(ERR_WAIT_FULL, 0x430u);
+          mbar_wait(bars + 8 * st, phase);
         }
-        float sc[NB][4];
+        const uint32_t base = ring + st * SB, half_ok = landed ? (there >> (2 * st)) & 3u : 0u;
+        const bool whole = half_ok == 3u && pos + kAttnStage <= all_see;
+        // scores of rows g, g + 8 of both halves, and their V parameters
+        float x[2][2][NB];
+        uint32_t vp[2][2][NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int t = 0; t < 2; ++t) {
+          uint32_t k0[KW], k1[KW], kp[2], one[1];
+          lds(base + k_at + t * k_next, k0);
+          lds(base + k_at + t * k_next + 8 * (HD / 2), k1);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sc[nb][j] = 0.f;
+          for (int r = 0; r < 2; ++r) {
+            lds(base + p_at + t * p_next + 32 * r, one);
+            kp[r] = one[0];
+            lds(base + p_at + t * p_next + 32 * r + blk * 4, one);
 #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-          if constexpr (kWide) {
-            // two MMAs from zero for each word, summed in fp32
-            uint32_t c0[4], c1[4];
-            centred4(k0[w], c0);
-            centred4(k1[w], c1);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              float d[4];
-              mma_f16_new(d, c0[0], c1[0], c0[1], c1[1], qf[nb][2 * w][0], qf[nb][2 * w][1]);
-              mma_f16(d, c0[2], c1[2], c0[3], c1[3], qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sc[nb][j] += d[j];
-            }
-          } else {
-            const uint32_t c0 = k0[w], c1 = k1[w], d0 = c0 >> 8, d1 = c1 >> 8;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              mma_f16(sc[nb], c0 & 0x000F000Fu, c1 & 0x000F000Fu, c0 & 0x00F000F0u, c1 & 0x00F000F0u,
-                      qf[nb][2 * w][0], qf[nb][2 * w][1]);
-              mma_f16(sc[nb], d0 & 0x000F000Fu, d1 & 0x000F000Fu, d0 & 0x00F000F0u, d1 & 0x00F000F0u,
-                      qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
-            }
+            for (int nb = 0; nb < NB; ++nb) vp[t][r][nb] = one[0];
           }
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float sk = par_s(kp[r]), zk = kWide ? fmaf(8.f, sk, par_z(kp[r])) : par_z(kp[r]);
+          float sc[NB][4];
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
-            x[t][r][nb] = fmaf((sc[nb][2 * r] + sc[nb][2 * r + 1]) * F[nb], sk, zk * Qs[nb]);
-        }
-      }
-      if (!whole) {
-        // hidden positions, which may hold anything: no score, no V
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+            for (int j = 0; j < 4; ++j) sc[nb][j] = 0.f;
+#pragma unroll
+          for (int w = 0; w < KW; ++w) {
+            if constexpr (kWide) {
+              // two MMAs from zero for each word, summed in fp32
+              uint32_t c0[4], c1[4];
+              centred4(k0[w], c0);
+              centred4(k1[w], c1);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                float d[4];
+                mma_f16_new(d, c0[0], c1[0], c0[1], c1[1], qf[nb][2 * w][0], qf[nb][2 * w][1]);
+                mma_f16(d, c0[2], c1[2], c0[3], c1[3], qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[nb][j] += d[j];
+              }
+            } else {
+              const uint32_t c0 = k0[w], c1 = k1[w], d0 = c0 >> 8, d1 = c1 >> 8;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                mma_f16(sc[nb], c0 & 0x000F000Fu, c1 & 0x000F000Fu, c0 & 0x00F000F0u, c1 & 0x00F000F0u,
+                        qf[nb][2 * w][0], qf[nb][2 * w][1]);
+                mma_f16(sc[nb], d0 & 0x000F000Fu, d1 & 0x000F000Fu, d0 & 0x00F000F0u, d1 & 0x00F000F0u,
+                        qf[nb][2 * w + 1][0], qf[nb][2 * w + 1][1]);
+              }
+            }
+          }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int p = (half_ok >> t) & 1u ? pos + 16 * t + 8 * r + tau : 0x7FFFFFFF;
+            const float sk = par_s(kp[r]), zk = kWide ? fmaf(8.f, sk, par_z(kp[r])) : par_z(kp[r]);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
-              if (p >= lim[nb]) {
-                x[t][r][nb] = kNegInf;
-                vp[t][r][nb] = 0u;
-              }
+              x[t][r][nb] = fmaf((sc[nb][2 * r] + sc[nb][2 * r + 1]) * F[nb], sk, zk * Qs[nb]);
           }
-      }
-      float top[NB], sm[NB];
-      bool renew = false;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        top[nb] = fmaxf(fmaxf(x[0][0][nb], x[0][1][nb]), fmaxf(x[1][0][nb], x[1][1][nb]));
-        sm[nb] = fmaxf(fmaxf(fmaxf(0.f, par_s(vp[0][0][nb])), par_s(vp[0][1][nb])),
-                       fmaxf(par_s(vp[1][0][nb]), par_s(vp[1][1][nb])));
-        // p < 2^3 and sv up < 2^12
-        renew = renew || top[nb] > m[nb] + 3.f || sm[nb] * up[nb] >= 4096.f;
-      }
-      if (__any_sync(0xffffffffu, renew)) {
-        // new maximum and new scale of every query
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float t = top[nb];
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-          const float mn = fmaxf(m[nb], t);
-          const float al = m[nb] == kNegInf ? 1.f : ex2(m[nb] - mn);
-          m[nb] = mn;
-          rel[nb] = mn == kNegInf ? 0.f : mn;
-          float w = wm[nb] * al, sv = sm[nb];
-#pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) w = fmaxf(w, ex2(x[h2][r][nb] - rel[nb]) * par_s(vp[h2][r][nb]));
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
-            sv = fmaxf(sv, __shfl_xor_sync(0xffffffffu, sv, o));
-          }
-          wm[nb] = w;
-          const int ew = exponent(w), ev_old = 11 - exponent(up[nb]);
-          int ev = max(ev_old, exponent(sv));
-          ev = max(ew, min(ev, ew + kAttnSpare));
-          ev = min(max(ev, -100), 127);
-          up[nb] = pow2i(11 - ev);
-          const float down = al * pow2i(min(max(ev_old - ev, -126), 127));
-          l[nb] *= al;
-          zs[nb] *= al;
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[nb][k][j] *= down;
         }
-      }
-      // weights of 16 positions: (hi, lo) of each row's side by side, transposed
-      auto weights = [&](int t, uint32_t (&wb)[NB][2]) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float w[2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float p = ex2(x[t][r][nb] - rel[nb]), sv = par_s(vp[t][r][nb]);
-            l[nb] += p;
-            zs[nb] = fmaf(p, fmaf(8.f, sv, par_z(vp[t][r][nb])), zs[nb]);
-            w[r] = (p * sv) * up[nb];
-          }
-          const __half2 hi = __floats2half2_rn(w[0], w[1]);
-          const float2 back = __half22float2(hi);
-          const __half2 lo = __floats2half2_rn(w[0] - back.x, w[1] - back.y);
-          const uint32_t h2 = *reinterpret_cast<const uint32_t*>(&hi), l2 = *reinterpret_cast<const uint32_t*>(&lo);
-          wb[nb][0] = trans8x8(prmt(h2, l2, 0x5410u));
-          wb[nb][1] = trans8x8(prmt(h2, l2, 0x7632u));
-        }
-      };
-      if constexpr (kPairs) {
-        // two MMAs from zero for each output tile, added in fp32
-        uint32_t wb[2][NB][2];
-        weights(0, wb[0]);
-        weights(1, wb[1]);
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          uint32_t v[2][4];
+        if (!whole) {
+          // hidden positions, which may hold anything: no score, no V
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              uint32_t one[1];
-              lds(base + v_at + t * k_next + r * 4 * (HD / 2) + 4 * w, one);
-              v[t][r] = one[0];
-            }
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t sel = half ? 0x7632u : 0x5410u;
-            float d[NB][2][4];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              uint32_t ha[4], hb[4];
-              centred4(prmt(v[t][0], v[t][1], sel), ha);
-              centred4(prmt(v[t][2], v[t][3], sel), hb);
-#pragma unroll
-              for (int p = 0; p < 2; ++p)
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                  if (t == 0)
-                    mma_f16_new(d[nb][p], ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1],
-                                wb[t][nb][0], wb[t][nb][1]);
-                  else
-                    mma_f16(d[nb][p], ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1], wb[t][nb][0],
-                            wb[t][nb][1]);
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
+            for (int r = 0; r < 2; ++r) {
+              const int p = (half_ok >> t) & 1u ? pos + 16 * t + 8 * r + tau : 0x7FFFFFFF;
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
+                if (p >= lim[nb]) {
+                  x[t][r][nb] = kNegInf;
+                  vp[t][r][nb] = 0u;
+                }
+            }
+        }
+        float top[NB], sm[NB];
+        bool renew = false;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[nb][w * 4 + half * 2 + p][j] += d[nb][p][j];
+        for (int nb = 0; nb < NB; ++nb) {
+          top[nb] = fmaxf(fmaxf(x[0][0][nb], x[0][1][nb]), fmaxf(x[1][0][nb], x[1][1][nb]));
+          sm[nb] = fmaxf(fmaxf(fmaxf(0.f, par_s(vp[0][0][nb])), par_s(vp[0][1][nb])),
+                         fmaxf(par_s(vp[1][0][nb]), par_s(vp[1][1][nb])));
+          // p < 2^3 and sv up < 2^12
+          renew = renew || top[nb] > m[nb] + 3.f || sm[nb] * up[nb] >= 4096.f;
+        }
+        if (__any_sync(0xffffffffu, renew)) {
+          // new maximum and new scale of every query
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float t = top[nb];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            const float mn = fmaxf(m[nb], t);
+            const float al = m[nb] == kNegInf ? 1.f : ex2(m[nb] - mn);
+            m[nb] = mn;
+            rel[nb] = mn == kNegInf ? 0.f : mn;
+            float w = wm[nb] * al, sv = sm[nb];
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) w = fmaxf(w, ex2(x[h2][r][nb] - rel[nb]) * par_s(vp[h2][r][nb]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+              sv = fmaxf(sv, __shfl_xor_sync(0xffffffffu, sv, o));
+            }
+            wm[nb] = w;
+            const int ew = exponent(w), ev_old = 11 - exponent(up[nb]);
+            int ev = max(ev_old, exponent(sv));
+            ev = max(ew, min(ev, ew + kAttnSpare));
+            ev = min(max(ev, -100), 127);
+            up[nb] = pow2i(11 - ev);
+            const float down = al * pow2i(min(max(ev_old - ev, -126), 127));
+            l[nb] *= al;
+            zs[nb] *= al;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[nb][k][j] *= down;
           }
         }
-      } else {
+        // weights of 16 positions: (hi, lo) of each row's side by side, transposed
+        auto weights = [&](int t, uint32_t (&wb)[NB][2]) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          uint32_t v[4][VW];
+          for (int nb = 0; nb < NB; ++nb) {
+            float w[2];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) lds(base + v_at + t * k_next + r * 4 * (HD / 2), v[r]);
-          uint32_t wb[NB][2];
-          weights(t, wb);
+            for (int r = 0; r < 2; ++r) {
+              const float p = ex2(x[t][r][nb] - rel[nb]), sv = par_s(vp[t][r][nb]);
+              l[nb] += p;
+              zs[nb] = fmaf(p, fmaf(8.f, sv, par_z(vp[t][r][nb])), zs[nb]);
+              w[r] = (p * sv) * up[nb];
+            }
+            const __half2 hi = __floats2half2_rn(w[0], w[1]);
+            const float2 back = __half22float2(hi);
+            const __half2 lo = __floats2half2_rn(w[0] - back.x, w[1] - back.y);
+            const uint32_t h2 = *reinterpret_cast<const uint32_t*>(&hi), l2 = *reinterpret_cast<const uint32_t*>(&lo);
+            wb[nb][0] = trans8x8(prmt(h2, l2, 0x5410u));
+            wb[nb][1] = trans8x8(prmt(h2, l2, 0x7632u));
+          }
+        };
+        if constexpr (kPairs) {
+          // two MMAs from zero for each output tile, added in fp32
+          uint32_t wb[2][NB][2];
+          weights(0, wb[0]);
+          weights(1, wb[1]);
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
+            uint32_t v[2][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                uint32_t one[1];
+                lds(base + v_at + t * k_next + r * 4 * (HD / 2) + 4 * w, one);
+                v[t][r] = one[0];
+              }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const uint32_t sel = half ? 0x7632u : 0x5410u;
-              uint32_t ha[4], hb[4];
-              centred4(prmt(v[0][w], v[1][w], sel), ha);
-              centred4(prmt(v[2][w], v[3][w], sel), hb);
+              float d[NB][2][4];
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                uint32_t ha[4], hb[4];
+                centred4(prmt(v[t][0], v[t][1], sel), ha);
+                centred4(prmt(v[t][2], v[t][3], sel), hb);
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                  for (int nb = 0; nb < NB; ++nb) {
+                    if (t == 0)
+                      mma_f16_new(d[nb][p], ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1],
+                                  wb[t][nb][0], wb[t][nb][1]);
+                    else
+                      mma_f16(d[nb][p], ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1], wb[t][nb][0],
+                              wb[t][nb][1]);
+                  }
+              }
 #pragma unroll
               for (int p = 0; p < 2; ++p)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                  float(&o)[4] = acc[nb][w * 4 + half * 2 + p];
-                  if constexpr (kWide) {
-                    float d[4];
-                    mma_f16_new(d, ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1], wb[nb][0], wb[nb][1]);
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[j] += d[j];
-                  } else {
-                    mma_f16(o, ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1], wb[nb][0], wb[nb][1]);
+                  for (int j = 0; j < 4; ++j) acc[nb][w * 4 + half * 2 + p][j] += d[nb][p][j];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            uint32_t v[4][VW];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds(base + v_at + t * k_next + r * 4 * (HD / 2), v[r]);
+            uint32_t wb[NB][2];
+            weights(t, wb);
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t sel = half ? 0x7632u : 0x5410u;
+                uint32_t ha[4], hb[4];
+                centred4(prmt(v[0][w], v[1][w], sel), ha);
+                centred4(prmt(v[2][w], v[3][w], sel), hb);
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                  for (int nb = 0; nb < NB; ++nb) {
+                    float(&o)[4] = acc[nb][w * 4 + half * 2 + p];
+                    if constexpr (kWide) {
+                      float d[4];
+                      mma_f16_new(d, ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1], wb[nb][0], wb[nb][1]);
+#pragma unroll
+                      for (int j = 0; j < 4; ++j) o[j] += d[j];
+                    } else {
+                      mma_f16(o, ha[2 * p], ha[2 * p + 1], hb[2 * p], hb[2 * p + 1], wb[nb][0], wb[nb][1]);
+                    }
                   }
-                }
+              }
             }
           }
         }
+        __syncwarp();                        // the stage may be copied over
+        st = st + 1 == kAttnDepth ? 0 : st + 1;
+        phase ^= st == 0 ? 1u : 0u;
       }
-      __syncwarp();                        // the stage may be copied over
-      st = st + 1 == kAttnDepth ? 0 : st + 1;
-      phase ^= st == 0 ? 1u : 0u;
+      if (kWide || pos >= t_end) break;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float w_down = __uint_as_float(0x7F000000u - __float_as_uint(up[nb]));   // 1 / up
+        float* const own_m = own_sums + (NB * KS * 2 + nb) * 32;
+        const float mf = flushed ? __ldcg(own_m) : kNegInf, f = mf == kNegInf ? 1.f : ex2(mf - m[nb]);
+        __stcg(own_m, m[nb]);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float* const at = own_sums + ((nb * KS + k) * 2 + j) * 32;
+            const float v = (acc[nb][k][2 * j] + acc[nb][k][2 * j + 1]) * w_down;
+            __stcg(at, flushed ? fmaf(__ldcg(at), f, v) : v);
+            acc[nb][k][2 * j] = acc[nb][k][2 * j + 1] = 0.f;
+          }
+      }
+      flushed = true;
+      stop = min(t_end, stop + kAttnFlush * kAttnStep);
     }
     __syncthreads();   // the rings are done with: the results take their place
 
@@ -1283,6 +1319,11 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
       for (int t = 0; t < KS; ++t) {
         o[2 * t] = fmaf(acc[nb][t][0] + acc[nb][t][1], w_down, zs[nb]);
         o[2 * t + 1] = fmaf(acc[nb][t][2] + acc[nb][t][3], w_down, zs[nb]);
+      }
+      if (flushed) {
+        const float mf = __ldcg(own_sums + (NB * KS * 2 + nb) * 32), f = mf == kNegInf ? 1.f : ex2(mf - m[nb]);
+#pragma unroll
+        for (int t = 0; t < 2 * KS; ++t) o[t] = fmaf(__ldcg(own_sums + (nb * KS * 2 + t) * 32), f, o[t]);
       }
       if (g == 0) {
         s_ml[(warp * Q + nb * 4 + i) * 2] = m[nb];

@@ -97,7 +97,7 @@ int attn_blocks(int64_t max_rows, int group) { return max_rows * group > 8 ? 2 :
 
 struct Kv4AttnLayout {
   int grid;
-  int64_t part_off, sums_off, total;
+  int64_t part_off, own_off, sums_off, total;
 };
 
 // Requests with more rows than this may take the tensor-core kernel, whose items are
@@ -124,9 +124,12 @@ Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int64_t max_rows, int group, 
   Kv4AttnLayout l;
   l.grid = d.sms * qz::kv4::attn_per_sm(hd, nb, wide);
   // the tickets' place is the same for every variant, so that one workspace
-  // serves calls of different shapes in turn
-  l.part_off = qz::cdiv(int64_t(d.sms) * qz::kv4::kAttnMaxPerSm * 4, 256) * 256;
-  l.sums_off = l.part_off + qz::cdiv(int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4, 256) * 256;
+  // serves calls of different shapes in turn; what lies behind it keeps nothing
+  // (five tickets an SM: 148 SMs take 3 KB of the head)
+  l.part_off = QZ_KV4_WORKSPACE_HEAD;
+  l.own_off = l.part_off + qz::cdiv(int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4, 256) * 256;
+  l.sums_off = l.own_off + (wide ? 0 : int64_t(l.grid) * qz::kv4::kAttnWarps *
+                                           qz::kv4::attn_sum_floats(hd, nb) * 32 * 4);
   l.total = l.sums_off + (max_rows > tc_rows(group) ? int64_t(d.sms) * qz::kv4::kTcRows * hd * 4 : 0);
   return l;
 }
@@ -316,6 +319,7 @@ int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_h
   a.cu = cu_rows;
   a.tickets = static_cast<unsigned*>(ws);
   a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + L.part_off);
+  a.sums = reinterpret_cast<float*>(static_cast<char*>(ws) + L.own_off);
   a.pages = pages;
   a.width = width;
   a.n = n;

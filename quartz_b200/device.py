@@ -875,11 +875,16 @@ def _kv4_default_ws(idx: int, stream: int, need: int) -> torch.Tensor:
     """The workspace of a call that brings none: one per device and stream. A call
     under stream capture gets its own, so that two graphs (or a graph and eager
     calls) never share one."""
+    def made():
+        ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", idx))
+        ws[:_lib.QZ_KV4_WORKSPACE_HEAD].zero_()
+        return ws
+
     if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", idx))
+        return made()
     ws = _kv4_ws.get((idx, stream))
     if ws is None or ws.numel() < need:
-        ws = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", idx))
+        ws = made()
         _kv4_ws[idx, stream] = ws
         if _fast is not None:
             _fast.workspace(idx, stream, ws.data_ptr(), ws.numel())

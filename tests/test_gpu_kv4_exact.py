@@ -140,3 +140,67 @@ def test_a_position_that_takes_the_weight_but_has_no_value(kind, form, dtype):
     # the first position's score has A = 40, and all weights are relative to it
     _check_sums(got, ref, size, 4 * 40 * (hd / 16 + 8) * 2.0 ** -23)
     qd.check_status()
+
+
+@pytest.mark.parametrize("dtype,most", [("fp16", 0.28), ("bf16", 0.035)])
+@pytest.mark.parametrize("hd,B,rows", [(64, 93, 1), (64, 40, 5), (128, 74, 1)])
+def test_long_contexts_of_16_bits_do_not_drift(hd, B, rows, dtype, most):
+    """So many requests that a CTA takes whole contexts of 2^19 positions: results are the
+    exact ones rounded once, but for a share |e| / ulp (see
+    test_prompts_of_16_bits_round_once). Here the results are small differences of the
+    sums: with steps of 0.3 and zeros of -7.5 steps, sum p s (c - 8) and sum p (z + 8 s)
+    are -0.15 and 0.15 of sum p, and the results, 1.4 times the root of
+    exp(1.4^2) / 2^19, are 5e-3 of it. A chain of 128 truncating MMAs is 128 * 3e-8 / 2 =
+    2e-6 of 0.15 low, and fp32 sums of 2^14 terms a lane are off by up to
+    128 * 2^-25 = 4e-6 of it: 9e-7 together. An ulp is 5e-3 * 2^-10.5 = 3.5e-6 (fp16) or
+    2.8e-5 (bf16): shares of 26 % and 3.2 %, with the scores' 1.2 % and 0.15 %. One chain
+    over a warp's 2^17 positions is 2^14 * 3e-8 / 2 = 2.5e-4 of 0.15 low, more than an ulp
+    of either."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(hd + B)
+    nkv, nq, t, page = 8, 16, 1 << 19, 256
+    if torch.cuda.mem_get_info(0)[0] < 8 << 30:
+        pytest.skip("needs 8 GB of device memory")
+    pages = t // page
+    pool = torch.randint(0, 256, (pages, nkv, page * (hd + 8)), generator=g, device=dev, dtype=torch.uint8)
+    par = torch.empty(pages, nkv, 2, page, 2, device=dev)
+    par[..., 0] = 0.2 + 0.2 * torch.rand(pages, nkv, 2, page, generator=g, device=dev)
+    par[..., 1] = -7.5 * par[..., 0]
+    pool[..., page * hd:] = par.to(torch.bfloat16).view(torch.uint8).flatten(2)
+    table = torch.arange(pages, dtype=torch.int32, device=dev).expand(B, pages).contiguous()
+    q = torch.randn(B * rows, nq, hd, generator=g, device=dev).to(DTYPES[dtype])
+    lens = _i64([t] * B, dev)
+    cu = _i64([b * rows for b in range(B + 1)], dev)
+    got = qd.kv4_attention(q, pool, table, lens, cu_rows=cu, max_rows=rows)
+    other = []
+    for b in (0, B // 2):
+        at = slice(b * rows, (b + 1) * rows)
+        ref, _ = _exact(q[at], pool, t, rows)
+        other.append((got[at] != ref.to(got.dtype)).double().mean().item())
+    assert max(other) < most, other
+    qd.check_status()
+
+
+def test_one_workspace_for_tiles_and_long_contexts():
+    """A workspace that calls of both kernels, head sizes and types share in turn, with
+    items longer than the places where sums are moved to it."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(24)
+    shapes = [(8, 2, 128, 1300, 1500, "fp32"), (8, 2, 64, 1300, 4500, "bf16"), (16, 8, 64, 1, 40000, "fp16"),
+              (8, 2, 64, 1300, 1400, "fp32"), (8, 2, 128, 1300, 4500, "fp16"), (4, 1, 128, 1, 40000, "bf16")]
+    ws = torch.zeros(max(qd.kv4_attention_workspace(dev, nq, nkv, hd, rows).numel()
+                         for nq, nkv, hd, rows, _, _ in shapes), dtype=torch.uint8, device=dev)
+    made = []
+    for nq, nkv, hd, rows, t, dtype in shapes:
+        k, v = (torch.randn(t, nkv, hd, generator=g, device=dev) for _ in range(2))
+        pool, table = _pool_of(k, v, 16)
+        q = torch.randn(rows, nq, hd, generator=g, device=dev).to(DTYPES[dtype])
+        args = (q, pool, table, _i64([t], dev))
+        kw = dict(cu_rows=_i64([0, rows], dev), max_rows=rows)
+        want = qd.kv4_attention(*args, **kw, workspace=qd.kv4_attention_workspace(dev, nq, nkv, hd, rows))
+        _check_sums(want, *_exact(q, pool, t, rows), 4 * 20 * (hd / 16 + 8) * 2.0 ** -23)
+        made.append((args, kw, want))
+    for _ in range(3):
+        for args, kw, want in made:
+            assert torch.equal(qd.kv4_attention(*args, **kw, workspace=ws), want)
+    qd.check_status()
