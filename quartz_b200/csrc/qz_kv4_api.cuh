@@ -125,7 +125,7 @@ Kv4AttnLayout kv4_attn_layout(const DeviceInfo& d, int64_t max_rows, int group, 
   l.grid = d.sms * qz::kv4::attn_per_sm(hd, nb, wide);
   // the tickets' place is the same for every variant, so that one workspace
   // serves calls of different shapes in turn; what lies behind it keeps nothing
-  // (five tickets an SM: 148 SMs take 3 KB of the head)
+  // (five tickets and one place of `sums` an SM: 148 SMs take 3.5 KB of the head)
   l.part_off = QZ_KV4_WORKSPACE_HEAD;
   l.own_off = l.part_off + qz::cdiv(int64_t(l.grid) * 2 * 4 * nb * (hd + 2) * 4, 256) * 256;
   l.sums_off = l.own_off + (wide ? 0 : int64_t(l.grid) * qz::kv4::kAttnWarps *
@@ -332,7 +332,8 @@ int qz_kv4_attention(const void* q, int dtype, int64_t q_row_stride, int64_t q_h
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t few = split_rows(*d, B, n, max_rows, group, nkv);
   if (few < 0x7FFFFFFF && max_rows > few) {
-    qz::kv4::TcArgs t{a, 0, d->sms, reinterpret_cast<float4*>(static_cast<char*>(ws) + L.sums_off)};
+    qz::kv4::TcArgs t{a, 0, d->sms, reinterpret_cast<float4*>(static_cast<char*>(ws) + L.sums_off),
+                        a.tickets + int64_t(d->sms) * qz::kv4::kAttnMaxPerSm};
     t.out_vec = rows_aligned(out, out_row_stride, out_head_stride, dtype);
     t.a.rows_lo = static_cast<int>(few);
     t.a.rows_hi = static_cast<int>(std::min<int64_t>(max_rows, 0x7FFFFFFF));

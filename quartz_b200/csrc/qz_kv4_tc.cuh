@@ -32,6 +32,7 @@
 //         memory, kTcRaw tiles ahead
 //   22    issues the MMAs: S(t + 1) before O(t), so that the next scores are
 //         ready when the softmax of this tile ends
+//   23    takes a place of the workspace for the item's fp32 sums
 // A row's weights p s_v go into fp16 as p s_v 2^(10 - ev), p relative to the row's
 // running maximum (below 2^4) and ev the largest exponent so far of a position's
 // u = max(s_v, |z_v + 8 s_v| / 8), a bound of what a code can add; what lies below
@@ -74,6 +75,7 @@ struct TcArgs {
   int out_vec;      // out rows are 16-byte aligned
   int slots;        // places of `sums`, one for each SM
   float4* sums;     // [slots][HD / 4][kTcRows]
+  unsigned* taken;  // [slots]: 1 while a CTA owns the place, 0 between calls
 };
 
 // Tiles that O accumulates in TMEM before it is added to fp32 sums in the
@@ -91,9 +93,30 @@ __device__ __forceinline__ uint32_t sm_id() {
   asm volatile("mov.u32 %0, %%smid;" : "=r"(id));
   return id;
 }
+// A place of `sums` for this CTA alone. At most one CTA per SM runs, so there is one that
+// is free; the SM's number only says where to look first (a CTA may be moved while it
+// runs, so the number owns nothing). -1, and an error, where a workspace is shared with a
+// call that runs at the same time.
+__device__ __forceinline__ int take_place(unsigned* taken, int slots) {
+  const unsigned first = sm_id();
+  for (unsigned k = 0; k < 64u * slots; ++k) {
+    const int p = static_cast<int>((first + k) % static_cast<unsigned>(slots));
+    if (atomicCAS(taken + p, 0u, 1u) == 0u) {
+      __threadfence();                   // what its last owner wrote comes first
+      return p;
+    }
+  }
+  report_error(ERR_WAIT_EMPTY, 0x404u);
+  return -1;
+}
+__device__ __forceinline__ void leave_place(unsigned* taken, int p) {
+  if (p < 0) return;
+  __threadfence();
+  atomicExch(taken + p, 0u);
+}
 template <int HD>
 __device__ __forceinline__ float4* sums_of(const TcArgs& args, int place) {
-  return args.sums + static_cast<size_t>(place < 0 ? 0 : place) * (HD / 4 * kTcRows);
+  return args.sums + static_cast<size_t>(place) * (HD / 4 * kTcRows);
 }
 
 template <int HD>
@@ -123,7 +146,7 @@ struct TcShared {
   float ex_q[2][4][kTcRows], ex[3][4][kTcRows];
   // [half]: what a row's sums in the workspace stand relative to, and their w_down
   float flushed[2][kTcRows], flushed_w[2][kTcRows];
-  int place;                    // in the workspace, or -1
+  int place;                    // in the workspace (or -1: none was free)
   uint32_t odd[kTcRing];        // a V parameter of the tile is not finite
   int64_t scan[128];
   int item[6];                  // request, first row, rows, first row of q, len - rows, positions seen
@@ -416,10 +439,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     sh.scan[tid] = mine;
   }
   if (tid == 0) {
-    sh.item[0] = -1;
-    // one CTA runs on an SM at a time; nothing is written outside of the workspace
-    const uint32_t sm = sm_id();
-    sh.place = sm < static_cast<uint32_t>(args.slots) ? static_cast<int>(sm) : -1;
+    sh.item[0] = sh.place = -1;
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&sh.k_full[s]), kTcConverters);
       mbar_init(smem_u32(&sh.v_full[s]), kTcConverters);
@@ -442,6 +462,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     fence_mbar_init();
   }
   __syncthreads();
+  if (tid == kTcThreads - 32) sh.place = take_place(args.taken, args.slots);
   if (warp == 22) {
     tc::tmem_alloc(smem_u32(&sh.tmem), 512);
     tc::tmem_relinquish();
@@ -479,12 +500,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   tc::tc_fence_after();
   if (sh.item[0] < 0) {                    // the grid is an upper bound
     if (warp == 22) tc::tmem_dealloc(*const_cast<volatile uint32_t*>(&sh.tmem), 512);
+    if (tid == kTcThreads - 32) leave_place(args.taken, sh.place);
     return;
   }
   // (each role reads these for itself: kept from here on, they would spill)
   auto tmem_base = [&]() -> uint32_t { return *const_cast<volatile uint32_t*>(&sh.tmem); };
   auto item = [&](int k) -> int { return *const_cast<volatile int*>(&sh.item[k]); };
   auto seen_by = [&]() -> int { return item(5); };
+  auto nt_of = [&]() -> int { return (seen_by() + kTcKeys - 1) / kTcKeys; };   // tiles of the item
   if (warp < 16) {
     // ======================= softmax =======================================
     regs_more<88>();
@@ -492,7 +515,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
     const int r = tid & 127, quarter = warp & 3, odd = (warp >> 2) & 1, half = warp >> 3;
     const int part = warp >> 2;               // this thread's share of the row's dimensions
     const uint32_t lane_addr = tmem_base() + (static_cast<uint32_t>(32 * quarter) << 16);
-    const int nt = (seen_by() + kTcKeys - 1) / kTcKeys, h = blockIdx.x % a.nkv;
+    const int nt = nt_of(), h = blockIdx.x % a.nkv;
     // r / group for r < 128: the error of the rounded-up reciprocal, 128 / 65536,
     // is below 1 / group
     const uint32_t inv_group = (65535u + a.group) / a.group;
@@ -668,7 +691,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       const float down = sh.down[ring];
       if (__any_sync(0xffffffffu, now != before || down != 1.f)) {
         tc_rescale<64>(cols, 1.f, now == kNegInf ? 0.f : -mu - now);
-        if (sh.place >= 0 ? j % kFlush : j) {
+        if (j % kFlush) {
           // O holds tiles up to j - 1 relative to `before`, V's steps to the old exponent
           const bool done = warp_wait(&sh.v_empty[odd ^ 1], ((j - 1) >> 1) & 1);
           if (!done && lane == 0) report_error(ERR_WAIT_FULL, 0x401u);
@@ -693,10 +716,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       tmem_wait_st();
       tc::tc_fence_before();
       mbar_arrive(smem_u32(&sh.p_full[odd]));
-      if (j % kFlush == kFlush - 1 && j + 1 < nt && sh.place >= 0) {
+      if (j % kFlush == kFlush - 1 && j + 1 < nt) {
         // O to the sums, this thread's half of the row; the next tile starts it anew
         const bool first = j < kFlush;
         const float wd = sh.w_down[ring];
+        failed = sh.place < 0;
+        if (failed) break;
         float4* const mine = sums_of<HD>(args, sh.place) + half * (HD / 8) * kTcRows + r;
         float4 t[4];
         auto fetch = [&](int c) {                 // sums of 16 columns, ahead of their use
@@ -753,7 +778,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       zs = fmaf(sh.ex[2][k][r], al, zs);
     }
     // the sums of this thread's columns, ahead of the last tile's MMAs
-    const bool summed = nt > kFlush && sh.place >= 0;
+    const bool summed = nt > kFlush && !failed && sh.place >= 0;
     float4 t[DP / 4];
 #pragma unroll
     for (int k = 0; k < DP / 4; ++k)
@@ -826,7 +851,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   } else if (warp < 20) {
     // ======================= converters ====================================
     regs_less<72>();
-    const int nt = (seen_by() + kTcKeys - 1) / kTcKeys;
+    const int nt = nt_of();
     // 16-byte chunks of code rows, LPR per row; a thread has the same chunk of
     // every RPI-th row, so its addresses are fixed. The eight threads of one
     // store phase hold two rows (hd 128) and four chunks of each; taking the
@@ -1008,7 +1033,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
       }
   } else if (warp == 22 && seen_by() > 0) {
     // ======================= MMA issuer ====================================
-    const int nt = (seen_by() + kTcKeys - 1) / kTcKeys;
+    const int nt = nt_of();
     const uint32_t tmem = tmem_base();
     constexpr uint32_t id_s = idesc_f16(kTcKeys, false), id_o = idesc_f16(HD, true);
     const bool leader = elect_one();
@@ -1041,7 +1066,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
         scores(j + 1);
       }
       ok = warp_wait(&sh.v_full[j & 1], (j >> 1) & 1) && warp_wait(&sh.p_full[j & 1], (j >> 1) & 1);
-      const bool anew = sh.place >= 0 ? j % kFlush == 0 : j == 0;
+      const bool anew = j % kFlush == 0;
       if (anew && j > 0) ok = ok && warp_wait(&sh.o_free, (j / kFlush - 1) & 1);
       if (!ok) break;
       tc::tc_fence_after();
@@ -1067,6 +1092,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const TcArgs arg
   }
   tc::tc_fence_before();
   __syncthreads();
+  if (tid == kTcThreads - 32) leave_place(args.taken, sh.place);
   if (warp == 22) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem_base(), 512);

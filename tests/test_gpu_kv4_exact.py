@@ -204,3 +204,30 @@ def test_one_workspace_for_tiles_and_long_contexts():
         for args, kw, want in made:
             assert torch.equal(qd.kv4_attention(*args, **kw, workspace=ws), want)
     qd.check_status()
+
+
+def test_a_place_of_the_workspace_has_one_owner():
+    """The tiles' fp32 sums go to places of the workspace (one for each SM, its last part)
+    that a CTA takes and leaves: places marked as taken stay as they are, whatever SM a
+    CTA runs on, and the others are free again afterwards."""
+    qd, dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(25)
+    rows, t, nkv, nq, hd = 1300, 4500, 2, 8, 64      # 82 tiles of 36 steps: sums every 16
+    k, v = (torch.randn(t, nkv, hd, generator=g, device=dev) for _ in range(2))
+    pool, table = _pool_of(k, v, 32)
+    q = torch.randn(rows, nq, hd, generator=g, device=dev).to(torch.bfloat16)
+    args, kw = (q, pool, table, _i64([t], dev)), dict(cu_rows=_i64([0, rows], dev), max_rows=rows)
+    want = qd.kv4_attention(*args, **kw)
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    ws = qd.kv4_attention_workspace(dev, nq, nkv, hd, rows)
+    taken = ws[20 * sms:24 * sms].view(torch.int32)  # behind five tickets an SM
+    sums = ws[-sms * 128 * hd * 4:].view(sms, -1)
+    held = torch.arange(sms, device=dev) % 3 == 0
+    assert sms - held.sum() >= 82
+    taken[held] = 1
+    sums[held] = 0xAB
+    for _ in range(3):
+        assert torch.equal(qd.kv4_attention(*args, **kw, workspace=ws), want)
+        assert torch.equal(taken, held.int()) and (sums[held] == 0xAB).all()
+    assert (sums[~held] != 0).any()
+    qd.check_status()
