@@ -94,6 +94,7 @@ class PagedEngine(_Int8Weights):
         self._ids: list[int] = []        # request id
         self._len: list[int] = []        # positions held
         self._next: list[int] = []       # the token that its next step takes
+        self._held: list[list[int]] = []  # tokens emitted during other requests' generate
         self._used = 0                   # pages handed out
         self._serial = 0
         self._graphs: dict[int, torch.cuda.CUDAGraph] = {}
@@ -207,6 +208,7 @@ class PagedEngine(_Int8Weights):
         self._ids += made
         self._len += [0] * len(prompts)
         self._next += [-1] * len(prompts)
+        self._held += [[] for _ in prompts]
         done = [0] * len(prompts)
         with torch.cuda.device(self.dev):
             while any(d < len(ids) for d, ids in zip(done, prompts)):
@@ -276,10 +278,19 @@ class PagedEngine(_Int8Weights):
     def step(self, steps: int = 1, *, graph: bool = True) -> dict[int, list[int]]:
         """Advance every running request by `steps` tokens. Returns request ->
         the tokens it emitted: the one decided before (next_token) first, so the
-        first step after add emits the first generated token."""
-        B = len(self._ids)
-        if B == 0 or steps <= 0:
+        first step after add emits the first generated token. What a request
+        emitted while generate() ran others comes in front."""
+        if not self._ids or steps <= 0:
             return {}
+        got = self._advance(steps, graph)
+        for row, r in enumerate(self._ids):
+            got[r] = self._held[row] + got[r]
+            self._held[row] = []
+        return got
+
+    def _advance(self, steps: int, graph: bool) -> dict[int, list[int]]:
+        """`steps` tokens of every running request."""
+        B = len(self._ids)
         if max(self._len) + steps > self.max_ctx:
             raise ValueError("a request would outgrow max_ctx")
         need = sum(self._pages_of(n + steps) - self._pages_of(n) for n in self._len)
@@ -316,19 +327,23 @@ class PagedEngine(_Int8Weights):
                 self.table[row].copy_(self.table[last])
                 self.lens[row:row + 1].copy_(self.lens[last:last + 1])
         self._used -= n
-        for a in (self._ids, self._len, self._next):
+        for a in (self._ids, self._len, self._next, self._held):
             a[row] = a[last]
             a.pop()
 
     def generate(self, prompts: Sequence[Sequence[int]], steps: int, *, graph: bool = True
                  ) -> list[list[int]]:
         """`steps` greedy tokens after each prompt (prompts of any lengths); the
-        requests are released afterwards. Other running requests advance too."""
+        requests are released afterwards. Other running requests advance too; the
+        next step() returns the tokens that they emit here."""
         if steps <= 0:
             return [[] for _ in prompts]
         ids = self.add(prompts)
         try:
-            got = self.step(steps, graph=graph)
+            got = self._advance(steps, graph)
+            for row, r in enumerate(self._ids):
+                if r not in ids:
+                    self._held[row] += got[r]
             return [got[r] for r in ids]
         finally:
             for r in ids:
