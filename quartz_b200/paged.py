@@ -185,7 +185,8 @@ class PagedEngine(_Int8Weights):
     def add(self, prompts: Sequence[Sequence[int]]) -> list[int]:
         """Start requests on non-empty prompts and return their ids; their prompts
         are in the cache afterwards and their first token is decided. Prompts
-        share steps of up to max_rows rows; longer ones take several."""
+        share steps of up to max_rows rows; longer ones take several. If a step
+        raises, none of the requests is left."""
         prompts = [[int(t) for t in ids] for ids in prompts]
         if not prompts:
             return []
@@ -200,6 +201,23 @@ class PagedEngine(_Int8Weights):
         need = sum(self._pages_of(len(ids)) for ids in prompts)
         if need > self.free:
             raise ValueError(f"prompts need {need} pages, {self.free} are free")
+        first, used = len(self._ids), self._used
+        try:
+            return self._add(prompts)
+        except BaseException:
+            # the pages that they took are the next of the free list again
+            for a in (self._ids, self._len, self._next, self._held):
+                del a[first:]
+            self._used = used
+            self._restore()
+            raise
+
+    def _restore(self) -> None:
+        """Lengths and cursor on the GPU as the host has them."""
+        self.lens[:len(self._len)].copy_(torch.tensor(self._len, dtype=torch.int64))
+        self.used.fill_(self._used)
+
+    def _add(self, prompts: list[list[int]]) -> list[int]:
         first = len(self._ids)
         B = first + len(prompts)
         self.lens[first:B].zero_()
@@ -296,18 +314,22 @@ class PagedEngine(_Int8Weights):
         need = sum(self._pages_of(n + steps) - self._pages_of(n) for n in self._len)
         if need > self.free:
             raise ValueError(f"the steps need {need} pages, {self.free} are free")
-        with torch.cuda.device(self.dev):
-            self.tok[:B].copy_(torch.tensor(self._next, dtype=torch.int64))
-            g = self._graph(B) if graph else None
-            out = torch.empty((steps + 1, B), dtype=torch.int64, device=self.dev)
-            out[0].copy_(self.tok[:B])
-            for i in range(steps):
-                if g is not None:
-                    g.replay()
-                else:
-                    self._decode_ops(B)
-                out[i + 1].copy_(self.tok[:B])
-            got = out.cpu().tolist()
+        try:
+            with torch.cuda.device(self.dev):
+                self.tok[:B].copy_(torch.tensor(self._next, dtype=torch.int64))
+                g = self._graph(B) if graph else None
+                out = torch.empty((steps + 1, B), dtype=torch.int64, device=self.dev)
+                out[0].copy_(self.tok[:B])
+                for i in range(steps):
+                    if g is not None:
+                        g.replay()
+                    else:
+                        self._decode_ops(B)
+                    out[i + 1].copy_(self.tok[:B])
+                got = out.cpu().tolist()
+        except BaseException:
+            self._restore()          # the requests are where they were before the call
+            raise
         self._len = [n + steps for n in self._len]
         self._used += need
         self._next = got[-1]
