@@ -189,8 +189,11 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t na) try {
   const bool no_cu = a[4] == Py_None, no_out = a[7] == Py_None, no_ws = a[8] == Py_None;
   int64_t max_rows;
   const int idx = home(pool);
-  if (idx < 0 || !rows(q, idx) || !is(table, at::kInt, 2, idx) || !is(lens, at::kLong, 1, idx) ||
-      !integer(a[5], &max_rows))
+  if (idx < 0 || !rows(q, idx) || !is(table, at::kInt, 2, idx) || !is(lens, at::kLong, 1, idx))
+    return decline();
+  if (a[5] == Py_None)
+    max_rows = no_cu || q->size(0) < 1 ? 1 : q->size(0);
+  else if (!integer(a[5], &max_rows))
     return decline();
   const int64_t n = q->size(0), nq = q->size(1), hd = q->size(2), ps = page_size(*pool, hd);
   const int64_t nkv = pool->size(1), B = table->size(0);
@@ -208,7 +211,8 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t na) try {
   at::Tensor made;
   const at::Tensor* out = no_out ? nullptr : tensor(a[7]);
   if (no_out) {
-    made = at::empty({n, nq, hd}, q->options());
+    // rows that no request has, or that are not computed, are zeros
+    made = no_cu && n <= B ? at::empty({n, nq, hd}, q->options()) : at::zeros({n, nq, hd}, q->options());
     out = &made;
   } else {
     if (!rows(out, idx) || out->scalar_type() != q->scalar_type() || out->sizes() != q->sizes())

@@ -891,7 +891,7 @@ def _kv4_default_ws(idx: int, stream: int, need: int) -> torch.Tensor:
     return ws
 
 
-def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=None, out=None,
+def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=None, scale=None, out=None,
                   workspace=None):
     """softmax(scale * q K^T) V of query rows over the paged 4-bit cache.
 
@@ -900,11 +900,13 @@ def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=No
     lens[b] positions (int64 [B], this step's included) lie in the pages
     block_table[b] (int32 [B, W]); each sees the positions up to its own, and
     one that sees none gives zeros. cu_rows (int64 [B + 1]) None: row b is
-    request b's. max_rows: the most rows a request has (a host number; rows of
-    a request with more are not computed). scale: hd ** -0.5 unless given.
-    Returns out (q's dtype); rows of no request are left as they were. out may
-    be q itself, but must not overlap it otherwise. n, B and max_rows choose
-    between two kernels, whose results differ by rounding."""
+    request b's (lens beyond the n rows are not used). max_rows: the most rows a
+    request has (a host number; rows of a request with more are not computed);
+    n unless given, 1 without cu_rows. scale: hd ** -0.5 unless given. Returns
+    out (q's dtype); rows that are not computed are left as they were, and are
+    zeros in an output that the call makes. out may be q itself, but must not
+    overlap it otherwise. n, B and max_rows choose between two kernels, whose
+    results differ by rounding."""
     if _fast is not None:
         r = _fast.attention(q, pool, block_table, lens, cu_rows, max_rows, scale, out, workspace)
         if r is not None:
@@ -918,7 +920,7 @@ def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=No
     B, W = block_table.shape
     if lens.numel() != B:
         raise ValueError(f"lens must have one element per table row ({B})")
-    max_rows = int(max_rows)
+    max_rows = (1 if cu_rows is None else max(1, n)) if max_rows is None else int(max_rows)
     if cu_rows is not None:
         _arg(cu_rows, torch.int64, "cu_rows", 1, idx)
         if cu_rows.numel() != B + 1:
@@ -928,7 +930,9 @@ def kv4_attention(q, pool, block_table, lens, cu_rows=None, max_rows=1, scale=No
     scale = hd ** -0.5 if scale is None else float(scale)
     qs = q.stride()
     if out is None:
-        out = torch.empty((n, nq, hd), dtype=q.dtype, device=pool.device)
+        # which rows are computed is in cu_rows, on the GPU
+        make = torch.empty if cu_rows is None and n <= B else torch.zeros
+        out = make((n, nq, hd), dtype=q.dtype, device=pool.device)
     else:
         _kv4_rows(out, "out", idx)
         if out.shape != q.shape or out.dtype is not q.dtype:
