@@ -5,7 +5,10 @@
 nvcc cross-compiles for sm_100a on a host without a GPU. The library exports
 the C ABI declared in include/quartz_b200.h. ``quartz_b200/_fastcall.so``, a
 CPython extension over the same entry points (csrc/fastcall.cpp), is built with
-the host compiler against the installed torch.
+the host compiler against the installed torch; without it the calls take their
+checked way through Python, so a failure to build it is a warning. It reads
+tensors by the layout of one torch's headers: a stamp in it names that torch and
+Python, and one of another is neither kept by build() nor loaded.
 """
 
 from __future__ import annotations
@@ -15,6 +18,7 @@ import re
 import shutil
 import subprocess
 import sys
+import warnings
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -41,15 +45,41 @@ FAST_SRC = SRC / "fastcall.cpp"
 FAST_OUT = PKG / "_fastcall.so"
 
 
+def fast_tag() -> str:
+    """The torch and the Python that a _fastcall.so has to be built for."""
+    import sysconfig
+
+    import torch
+
+    return (f"torch={torch.__version__};python={sysconfig.get_config_var('SOABI')};"
+            f"cxx11={int(torch._C._GLIBCXX_USE_CXX11_ABI)}")
+
+
+def fast_stamp(path: Path = FAST_OUT) -> str:
+    """The stamp of a built _fastcall.so ("" without one that can be read)."""
+    import ctypes
+
+    try:
+        return ctypes.c_char_p(ctypes.addressof(
+            ctypes.c_char.in_dll(ctypes.CDLL(str(path)), "qz_fastcall_stamp"))).value.decode()
+    except (OSError, ValueError):
+        return ""
+
+
+def fast_up_to_date() -> bool:
+    header = REPO / "include" / "quartz_b200.h"
+    return (FAST_OUT.exists()
+            and all(p.stat().st_mtime <= FAST_OUT.stat().st_mtime for p in (FAST_SRC, header, Path(__file__)))
+            and fast_stamp() == fast_tag())
+
+
 def build_fastcall(force: bool = False) -> Path:
     """The extension module quartz_b200._fastcall."""
     import sysconfig
 
     import torch
 
-    header = REPO / "include" / "quartz_b200.h"
-    if not force and FAST_OUT.exists() and all(
-            p.stat().st_mtime <= FAST_OUT.stat().st_mtime for p in (FAST_SRC, header)):
+    if not force and fast_up_to_date():
         return FAST_OUT
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
@@ -58,6 +88,7 @@ def build_fastcall(force: bool = False) -> Path:
     lib = root / "lib"
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DQZ_FASTCALL_STAMP="{fast_tag()}"',
            *[f"-I{p}" for p in inc], str(FAST_SRC), "-o", str(FAST_OUT), f"-L{lib}",
            f"-L{cuda / 'lib64'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10",
            "-lcudart", f"-Wl,-rpath,{lib}"]
@@ -107,7 +138,17 @@ def parse_ptxas(log: str) -> dict[str, dict]:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    build_fastcall(force)
+    build_library(force, verbose)
+    try:
+        build_fastcall(force)
+    except (OSError, ImportError, RuntimeError, subprocess.CalledProcessError) as e:
+        warnings.warn(f"{FAST_OUT.name} is not built, paged-cache calls take longer: {e}",
+                      RuntimeWarning, stacklevel=2)
+    return OUT
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    """libquartz_b200.so."""
     if not force and up_to_date():
         return OUT
     cmd = [nvcc(), "-Xptxas=-v", *NVCC_FLAGS, f"-I{REPO / 'include'}", f"-I{SRC}",

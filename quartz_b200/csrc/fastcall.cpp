@@ -304,4 +304,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", "Paged-cache calls wit
 
 }  // namespace
 
+// The torch and the Python whose headers this was built with (quartz_b200/build.py).
+extern "C" __attribute__((visibility("default"))) const char qz_fastcall_stamp[] = QZ_FASTCALL_STAMP;
+
 PyMODINIT_FUNC PyInit__fastcall() { return PyModule_Create(&module); }

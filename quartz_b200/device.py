@@ -92,6 +92,10 @@ def _bind_fast(idx: int) -> None:
     global _fast
     if _fast is None:
         try:
+            from . import build
+            built, want = build.fast_stamp(), build.fast_tag()
+            if built != want:
+                raise ImportError(f"built for {built or 'nothing'}, this is {want}")
             from . import _fastcall
         except ImportError as e:      # the same kernels, 4 to 9 us more for each paged-cache call
             warnings.warn(f"quartz_b200/_fastcall.so does not load ({e}): build it with "
