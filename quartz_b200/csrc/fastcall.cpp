@@ -6,8 +6,9 @@
 // (12 to 14 us a call). The functions here look at the same tensors directly and
 // call the same C entry points. They take only what is right: on anything else
 // (a wrong type or shape, another current device, stream capture without a
-// workspace, an error from the library) they return None, having queued nothing,
-// and the Python function goes through its checks and says what is wrong.
+// workspace, arguments that the library refuses) they return None, having queued
+// nothing, and the Python function goes through its checks and says what is wrong. A
+// failure of CUDA is raised here: one of a call's launches may be queued by then.
 #include <torch/csrc/autograd/python_variable.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -26,12 +27,23 @@ struct Entry {
   decltype(&qz_kv4_gather) gather;
   decltype(&qz_kv4_attention) attention;
   decltype(&qz_kv4_attention_workspace_bytes) attention_ws;
+  decltype(&qz_last_error) last_error;
 } entry{};
+PyObject* quartz_error = nullptr;   // the exception class of a CUDA failure
 
 uint64_t ready = 0;   // devices that ensure_device has seen
 std::map<std::pair<int, cudaStream_t>, std::pair<void*, size_t>> workspaces;
 
 PyObject* decline() { Py_RETURN_NONE; }
+
+// The result of a call that the library did not take.
+PyObject* failed(int rc) {
+  if (rc != QZ_ERR_CUDA) return decline();
+  char msg[512];
+  entry.last_error(msg, sizeof msg);
+  PyErr_SetString(quartz_error, msg);
+  return nullptr;
+}
 
 // The tensor behind an argument, or null.
 const at::Tensor* tensor(PyObject* o) {
@@ -119,12 +131,12 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t na) try {
   const at::Tensor buf = at::empty({2 * B + 2 + 2 * n}, lens->options());
   int64_t* p = buf.data_ptr<int64_t>();
   const int64_t at_len = B + 1, at_used = 2 * B + 1, at_slots = 2 * B + 2, at_pos = at_slots + n;
-  if (entry.plan(lens->data_ptr<int64_t>(), joins->data_ptr<int64_t>(), B, table->data_ptr<int32_t>(),
+  if (const int rc = entry.plan(lens->data_ptr<int64_t>(), joins->data_ptr<int64_t>(), B, table->data_ptr<int32_t>(),
                  table->size(1), free_pages->data_ptr<int32_t>(), free_pages->numel(),
                  used->data_ptr<int64_t>(), ps, n, p, own_lens ? p + at_len : lo->data_ptr<int64_t>(),
                  own_used ? p + at_used : uo->data_ptr<int64_t>(), p + at_slots, p + at_pos,
-                 c10::cuda::getCurrentCUDAStream(idx).stream()) != QZ_OK)
-    return decline();
+                 c10::cuda::getCurrentCUDAStream(idx).stream()))
+    return failed(rc);
   PyObject* out = PyTuple_New(5);
   if (!out) return nullptr;
   auto put = [&](int i, PyObject* o) { PyTuple_SET_ITEM(out, i, o); };
@@ -148,11 +160,11 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t na) try {
     return decline();
   const int64_t n = k->size(0), nkv = k->size(1), hd = k->size(2), ps = page_size(*pool, hd);
   if (!ps || pool->size(1) != nkv || slots->numel() != n) return decline();
-  if (entry.append(k->data_ptr(), v->data_ptr(), dtype_of(*k), k->stride(0), k->stride(1), v->stride(0),
+  if (const int rc = entry.append(k->data_ptr(), v->data_ptr(), dtype_of(*k), k->stride(0), k->stride(1), v->stride(0),
                    v->stride(1), n, static_cast<int>(nkv), static_cast<int>(hd), pool->data_ptr<uint8_t>(),
                    pool->size(0), ps, slots->data_ptr<int64_t>(),
-                   c10::cuda::getCurrentCUDAStream(idx).stream()) != QZ_OK)
-    return decline();
+                   c10::cuda::getCurrentCUDAStream(idx).stream()))
+    return failed(rc);
   Py_RETURN_TRUE;
 } catch (...) {
   return decline();
@@ -169,10 +181,10 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t na) try {
   if (!ps) return decline();
   const auto opts = pool->options().dtype(at::kFloat);
   const at::Tensor k = at::empty({n, nkv, hd}, opts), v = at::empty({n, nkv, hd}, opts);
-  if (entry.gather(pool->data_ptr<uint8_t>(), pool->size(0), ps, static_cast<int>(nkv),
+  if (const int rc = entry.gather(pool->data_ptr<uint8_t>(), pool->size(0), ps, static_cast<int>(nkv),
                    static_cast<int>(hd), slots->data_ptr<int64_t>(), n, k.data_ptr<float>(),
-                   v.data_ptr<float>(), c10::cuda::getCurrentCUDAStream(idx).stream()) != QZ_OK)
-    return decline();
+                   v.data_ptr<float>(), c10::cuda::getCurrentCUDAStream(idx).stream()))
+    return failed(rc);
   PyObject* out = PyTuple_New(2);
   if (!out) return nullptr;
   PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(k));
@@ -244,25 +256,29 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t na) try {
     ws_bytes = static_cast<size_t>(w->numel());
   }
   const auto s = q->strides(), os = out->strides();
-  if (entry.attention(q->data_ptr(), dtype_of(*q), s[0], s[1], out->data_ptr(), os[0], os[1],
+  if (const int rc = entry.attention(q->data_ptr(), dtype_of(*q), s[0], s[1], out->data_ptr(), os[0], os[1],
                       pool->data_ptr<uint8_t>(), pool->size(0), ps, table->data_ptr<int32_t>(),
                       table->size(1), lens->data_ptr<int64_t>(), no_cu ? nullptr : cu->data_ptr<int64_t>(),
                       B, n, max_rows, static_cast<int>(nq), static_cast<int>(nkv), static_cast<int>(hd),
-                      static_cast<float>(scale), ws, ws_bytes, st) != QZ_OK)
-    return decline();
+                      static_cast<float>(scale), ws, ws_bytes, st))
+    return failed(rc);
   return no_out ? THPVariable_Wrap(made) : Py_NewRef(a[7]);
 } catch (...) {
   return decline();
 }
 
-// bind(plan, append, gather, attention, attention_workspace_bytes): the entry points' addresses
+// bind(error class, plan, append, gather, attention, attention_workspace_bytes, last_error): the
+// entry points' addresses
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
-  if (na != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind takes five addresses");
+  if (na != 7 || !PyExceptionClass_Check(a[0])) {
+    PyErr_SetString(PyExc_TypeError, "bind takes an exception class and six addresses");
     return nullptr;
   }
-  void* p[5];
-  for (int i = 0; i < 5; ++i) {
+  Py_INCREF(a[0]);
+  Py_XSETREF(quartz_error, a[0]);
+  ++a;
+  void* p[6];
+  for (int i = 0; i < 6; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (!p[i]) return PyErr_Occurred() ? nullptr : decline();
   }
@@ -270,7 +286,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
                 reinterpret_cast<decltype(&qz_kv4_append)>(p[1]),
                 reinterpret_cast<decltype(&qz_kv4_gather)>(p[2]),
                 reinterpret_cast<decltype(&qz_kv4_attention)>(p[3]),
-                reinterpret_cast<decltype(&qz_kv4_attention_workspace_bytes)>(p[4])};
+                reinterpret_cast<decltype(&qz_kv4_attention_workspace_bytes)>(p[4]),
+                reinterpret_cast<decltype(&qz_last_error)>(p[5])};
   Py_RETURN_NONE;
 }
 

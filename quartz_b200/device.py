@@ -102,9 +102,10 @@ def _bind_fast(idx: int) -> None:
                           "`python -m quartz_b200.build`", RuntimeWarning, stacklevel=3)
             return
         lib = _lib.load()
-        _fastcall.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
-            "qz_kv4_plan", "qz_kv4_append", "qz_kv4_gather", "qz_kv4_attention",
-            "qz_kv4_attention_workspace_bytes")))
+        _fastcall.bind(_lib.QuartzError, *(
+            ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+                "qz_kv4_plan", "qz_kv4_append", "qz_kv4_gather", "qz_kv4_attention",
+                "qz_kv4_attention_workspace_bytes", "qz_last_error")))
         _fast = _fastcall
     _fast.device_ready(idx)
 

@@ -74,3 +74,44 @@ def test_max_rows_left_out_takes_all_rows(checked, monkeypatch):
     # no rows at all
     assert qd.kv4_attention(q[:0], pool, table, lens, cu_rows=_i64([0] * 4, dev)).shape == (0, 4, 64)
     qd.check_status()
+
+
+def test_a_cuda_failure_is_raised_and_not_tried_again(monkeypatch):
+    """A launch may be queued when the library reports a CUDA error (attention has two):
+    the direct calls raise it, and the checked ones do not run after them."""
+    import ctypes
+
+    from quartz_b200 import _lib, device as qd
+    dev, pool, table, lens, q = _setup(3)
+    want = qd.kv4_attention(q, pool, table, lens)
+    if qd._fast is None:
+        pytest.skip("the _fastcall extension is not built")
+    lib, calls = _lib.load(), []
+    names = ("qz_kv4_plan", "qz_kv4_append", "qz_kv4_gather", "qz_kv4_attention",
+             "qz_kv4_attention_workspace_bytes", "qz_last_error")
+    real = [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names]
+
+    def fails(kind):
+        sig, res = _lib.SIGNATURES[kind]
+        return ctypes.CFUNCTYPE(res, *sig)(lambda *a: calls.append(kind) or 2)     # QZ_ERR_CUDA
+
+    fakes = [fails(n) for n in names[:4]]
+    one = torch.ones(3, dtype=torch.int64, device=dev)
+    free = torch.arange(4, dtype=torch.int32, device=dev)
+    k = q[:, :2].contiguous()
+    lib.qz_kv4_gather(None, 0, 0, 0, 0, None, 0, None, None, None)      # leaves a message
+    try:
+        qd._fast.bind(_lib.QuartzError, *(ctypes.cast(f, ctypes.c_void_p).value for f in fakes), *real[4:])
+        for name in names[:4]:                                         # the library, called past the fakes
+            monkeypatch.setattr(lib, name, lambda *a: pytest.fail("tried again"))
+        for call in (lambda: qd.kv4_plan(lens, one, table, free, one[:1], 16, 4),
+                     lambda: qd.kv4_append(k, k, pool, lens),
+                     lambda: qd.kv4_gather(pool, lens, 64),
+                     lambda: qd.kv4_attention(q, pool, table, lens)):
+            with pytest.raises(_lib.QuartzError, match="n_kv"):
+                call()
+    finally:
+        qd._fast.bind(_lib.QuartzError, *real)
+    assert calls == list(names[:4])
+    monkeypatch.undo()
+    assert torch.equal(qd.kv4_attention(q, pool, table, lens), want)
