@@ -724,17 +724,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ uint32_t pack_h2(__half lo, __half hi) {
-  return static_cast<uint32_t>(__half_as_ushort(lo)) |
-         (static_cast<uint32_t>(__half_as_ushort(hi)) << 16);
-}
-
-// x as fp16 hi (low half of the word) and the fp16 of what hi leaves (high half).
-__device__ __forceinline__ uint32_t split_h2(float x) {
-  const __half hi = __float2half_rn(x);
-  return pack_h2(hi, __float2half_rn(x - __half2float(hi)));
-}
-
 // 2^e for e in [-126, 127], floor(log2 x) for a normal x >= 0 (-127 for what is smaller).
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 __device__ __forceinline__ int exponent(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127; }
