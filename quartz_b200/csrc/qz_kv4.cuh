@@ -627,9 +627,10 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kv4_kernel(const RopeArg
 // same vote sees to the power of two that brings a query's weights p sv into fp16's
 // range (see kAttnSpare).
 //
-// Measured: 64 x 16384 positions, 8 kv heads of 128, bf16 134 us (57 % of the copy
-// rate; ALU pipe 57 %, issue slots 57 %); 16 x 2048 fp32 17 us; one request of 131071
-// positions, 8 kv heads of 64, fp32 43 us (630 instructions per 32 positions and head).
+// Measured: 64 x 16384 positions, 8 kv heads of 128, bf16 139 us (56 % of the copy
+// rate; 730 instructions per 32 positions and head, issue slots 57 %, no pipe full);
+// 16 x 2048 fp32 17.4 us; one request of 131071 positions, 8 kv heads of 64, fp32 45 us
+// (635 instructions, issue 65 %). Graphs of 10 calls.
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;

@@ -188,6 +188,9 @@ int qz_kv4_plan(const int64_t* lens, const int64_t* new_rows, int64_t B, int32_t
     QZ_CUDA(allow_smem(qz::kv4::plan_kernel, qz::kv4::plan_smem(qz::kv4::kPlanMaxB)));
   // One CTA writes a small plan. A large one is shared out: over a cluster where lengths
   // or the cursor are updated in place, else over as many CTAs as give each thread a row.
+  // In place, us for one CTA / a cluster (B x rows each): 64 x 1 6.1 / 6.6, 768 x 1 6.8 / 7.3,
+  // 1 x 3048 7.1 / 6.5, 1024 x 1 7.2 / 7.8, 8 x 512 8.8 / 6.8, 4096 x 1 13.4 / 8.7,
+  // 1024 x 48 66 / 14.
   const bool large = rows + 4 * B > 4096;
   auto meets = [](const int64_t* p, int64_t n, const int64_t* q, int64_t m) { return p < q + m && q < p + n; };
   const bool in_place = meets(lens_out, B, lens, B) || meets(lens_out, B, new_rows, B) ||

@@ -46,9 +46,10 @@
 // (0 4 1 5 2 6 3 7 of each word); Q is stored in the same order, and the
 // epilogue puts O's columns back.
 //
-// Measured: a prompt of 4096, 32 heads, 8 kv heads of 128: 384 us (fp32), tensor pipe
-// 29 %; a tile takes 2.3 us (fp32) or 1.7 us (bf16), of which the MMAs are 1.1 or 0.55:
-// two tiles are in flight and each is a chain of scores, maximum, weights and sums.
+// Measured: a prompt of 4096, 32 heads, 8 kv heads of 128: 392 us (fp32), tensor pipe
+// 28 %; a tile takes 2.6 us (fp32) or 2.2 us (16 bits), of which the MMAs are 1.0 or 0.8:
+// two tiles are in flight and each is a chain of scores, maximum, weights and sums. A
+// prompt with `wide` tiles takes 424 us.
 #pragma once
 
 #include "qz_kv4.cuh"
@@ -84,7 +85,8 @@ struct TcArgs {
 // low: 1e-5 of itself after 40 tiles, 2e-4 after 100000 positions. Even: the odd
 // tiles' threads do it, while the even ones work on the next tile. fp32 rows, every
 // two tiles: 5e-7 off 64 bits at 4096 positions; every four 1.1e-6 and 4 % faster.
-// 16-bit rows round by 2^-12 at least, 16 tiles drift by 4e-6.
+// 16-bit rows round by 2^-12 at least, 16 tiles drift by 4e-6 (fp16 over 40000
+// positions 2.08e-4 off 64 bits, the rounding 2.07e-4; every 8 tiles 2.5 % slower).
 template <int L>
 __host__ __device__ constexpr int tc_flush() { return L == 2 ? 2 : 16; }
 
