@@ -1001,8 +1001,10 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
     }
 
     // ---- stages of this warp ---------------------------------------------------
-    float* const own_sums = a.sums + static_cast<size_t>(blockIdx.x * kAttnWarps + warp) *
-                                         (attn_sum_floats(HD, NB) * 32) + lane;
+    auto own_sums = [&](int k) -> float* {   // (formed where it is used: registers)
+      return a.sums + static_cast<size_t>(blockIdx.x * kAttnWarps + warp) * (attn_sum_floats(HD, NB) * 32) +
+             k * 32 + lane;
+    };
     const int32_t* tab = a.table + b * a.width;
     const int t_end = s1 * kAttnStep < seen ? s1 * kAttnStep : seen;
     int pos = s0 * kAttnStep + warp * kAttnStage;
@@ -1277,14 +1279,14 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const float w_down = __uint_as_float(0x7F000000u - __float_as_uint(up[nb]));   // 1 / up
-        float* const own_m = own_sums + (NB * KS * 2 + nb) * 32;
+        float* const own_m = own_sums(NB * KS * 2 + nb);
         const float mf = flushed ? __ldcg(own_m) : kNegInf, f = mf == kNegInf ? 1.f : ex2(mf - m[nb]);
         __stcg(own_m, m[nb]);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float* const at = own_sums + ((nb * KS + k) * 2 + j) * 32;
+            float* const at = own_sums((nb * KS + k) * 2 + j);
             const float v = (acc[nb][k][2 * j] + acc[nb][k][2 * j + 1]) * w_down;
             __stcg(at, flushed ? fmaf(__ldcg(at), f, v) : v);
             acc[nb][k][2 * j] = acc[nb][k][2 * j + 1] = 0.f;
@@ -1311,9 +1313,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_per_sm(HD, NB, sizeof(T) ==
         o[2 * t + 1] = fmaf(acc[nb][t][2] + acc[nb][t][3], w_down, zs[nb]);
       }
       if (flushed) {
-        const float mf = __ldcg(own_sums + (NB * KS * 2 + nb) * 32), f = mf == kNegInf ? 1.f : ex2(mf - m[nb]);
+        const float mf = __ldcg(own_sums(NB * KS * 2 + nb)), f = mf == kNegInf ? 1.f : ex2(mf - m[nb]);
 #pragma unroll
-        for (int t = 0; t < 2 * KS; ++t) o[t] = fmaf(__ldcg(own_sums + (nb * KS * 2 + t) * 32), f, o[t]);
+        for (int t = 0; t < 2 * KS; ++t) o[t] = fmaf(__ldcg(own_sums(nb * KS * 2 + t)), f, o[t]);
       }
       if (g == 0) {
         s_ml[(warp * Q + nb * 4 + i) * 2] = m[nb];
