@@ -231,3 +231,58 @@ def test_a_place_of_the_workspace_has_one_owner():
         assert torch.equal(taken, held.int()) and (sums[held] == 0xAB).all()
     assert (sums[~held] != 0).any()
     qd.check_status()
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_uneven_requests_of_any_scale(seed):
+    """Requests of uneven rows and lengths with V rows of very different size, rows of zeros
+    and offsets among them. Per row, an error is at most sum_t p_t max_d |v_td| times that of
+    the weights: exp(2 e) - 1 for scores off by e = 4 A (hd / 16 + 8) 2^-23, A the row's
+    largest scale * sum |q k|, and 2^-19 of exponent, split and sums; values of 2^90 times a
+    row's own may take 2^-95 of themselves; then the rounding."""
+    import random
+    qd, dev = _dev()
+    rng, g = random.Random(seed), torch.Generator(device=dev).manual_seed(seed)
+    hd, page = rng.choice([64, 128]), rng.choice([16, 32, 64, 128, 256])
+    nkv, group = rng.choice([(1, 16), (2, 4), (3, 5), (8, 2), (2, 1), (1, 3)])
+    dtype = DTYPES[rng.choice(["fp32", "fp32", "bf16"])]
+    rows = [rng.choice([0, 1, 2, 5, rng.randrange(1, 900)]) for _ in range(rng.choice([1, 2, 3, 7]))]
+    lens = [max(0, n + rng.choice([-3, 0, 0, 1, rng.randrange(3000)])) for n in rows]
+    spread, shift = rng.choice([0, 4, 12, 30, 60]), rng.choice([0, 1, 30])
+    B, width = len(rows), max(1, -(-max(lens) // page))
+    order = torch.randperm(B * width + 1, generator=g, device=dev).to(torch.int32)
+    table = order[:B * width].view(B, width).contiguous()
+    pool = P.empty_pool(B * width + 1, nkv, hd, page, 0xFF, dev)
+    for b, t in enumerate(lens):
+        if not t:
+            continue
+        k, v = (torch.randn(t, nkv, hd, generator=g, device=dev) for _ in range(2))
+        e = (torch.randn(t, nkv, 1, generator=g, device=dev) * spread).clamp(-100, 100)
+        v = (v + shift * torch.randn(t, nkv, 1, generator=g, device=dev)) * torch.exp2(e)
+        v[torch.rand(t, generator=g, device=dev) < rng.choice([0, 0.1])] = 0
+        pos = torch.arange(t, device=dev)
+        P.store(pool, hd, table[b][pos // page].long() * page + pos % page, k * rng.choice([1, 3]), v)
+    cu = [sum(rows[:b]) for b in range(B + 1)]
+    q = torch.randn(cu[-1] + rng.choice([0, 3, 2000]) + 1, nkv * group, hd, generator=g, device=dev)
+    q = (q * rng.choice([1, 4])).to(dtype)
+    out = torch.full_like(q, 0.25)
+    qd.kv4_attention(q, pool, table, _i64(lens, dev), cu_rows=_i64(cu, dev), max_rows=max(1, *rows), out=out)
+    assert (out[cu[-1]:] == 0.25).all()
+    keys, vals = P.load(pool, hd)
+    for b, (n, t) in enumerate(zip(rows, lens)):
+        pos = torch.arange(t, device=dev)
+        at = table[b][pos // page].long(), pos % page
+        hide = pos > t - n + torch.arange(n, device=dev)[:, None]
+        for h in range(nkv * group if n and t else 0):
+            k, v = keys[at[0], h // group, at[1]], vals[at[0], h // group, at[1]]
+            x = q[cu[b]:cu[b + 1], h].double() * hd ** -0.5
+            p = torch.nan_to_num(torch.softmax((x @ k.T).masked_fill(hide, -math.inf), -1), nan=0.0)
+            score = 4 * (x.abs() @ k.abs().T).masked_fill(hide, 0).amax(-1, keepdim=True) * (hd / 16 + 8) * 2.0 ** -23
+            ref, size = p @ v, p @ v.abs().amax(-1, keepdim=True)
+            bound = size * ((2 * score).exp() - 1 + 2.0 ** -19) + v.abs().max() * 2.0 ** -95
+            bound = bound + ref.abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).tiny
+            got = out[cu[b]:cu[b + 1], h].double()
+            assert ((got - ref).abs() <= bound).all(), (b, h, ((got - ref).abs() / bound).max().item())
+        if n and not t:
+            assert (out[cu[b]:cu[b + 1]] == 0).all()
+    qd.check_status()
